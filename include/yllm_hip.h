@@ -222,6 +222,96 @@ int yhip_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride,
                        uint32_t head_dim, uint32_t kv_stride, uint32_t rope, uint32_t n_rot, float theta,
                        void* stream);
 
+/* ---- Paged KV cache ---------------------------------------------------------
+ * Serving many sequences from one pool: each holds pages of `block` positions
+ * and a row of a block table with their numbers (no reference counterpart: its
+ * engine keeps one contiguous cache per sequence).  Per layer:
+ *   K : u16 f16 bits [n_blocks][n_kv_heads][block][head_dim]
+ *   V : u16 f16 bits [n_blocks][n_kv_heads][block/32][head_dim][32]
+ * so a contiguous cache (above) is a pool of one page with block = kv_stride.
+ * Position p of sequence i is slot table[i][p / block] * block + p % block.
+ * Lengths, tables, slots and positions are int32 in DEVICE memory: a step needs
+ * no copy to the host, and a captured step replays with new lengths.
+ *
+ * yhip_paged_plan: what one step needs, from the request lengths.  ctx_lens[i]
+ * positions of sequence i are stored, new_lens[i] (0 and up) come in this step.
+ * Sequence i holds ceil(ctx/block) blocks, whose entries of its table row
+ * (max_blocks entries, rows table_stride apart) are set, and gets the blocks
+ * that its new positions need, in order of i, from the end of the *n_free
+ * free_blocks (an array of free_cap entries).  Written:
+ *   block_table  the new entries (no others)
+ *   cu_new       [n_seq+1] prefix sums of new_lens: the rows of each sequence
+ *   kv_lens      [n_seq] ctx + new
+ *   slots, positions  [n_tok] of every row; rows from cu_new[n_seq] on: slot
+ *                -1, position 0
+ *   counts       [4] free blocks left, rows in all, sequences not served,
+ *                blocks missing
+ * A sequence that does not get all it needs is not served: none of its table
+ * entries is set, its kv_lens is 0 and its rows have slot -1 (so nothing of it
+ * is stored and its attention rows are zero).  That is one whose blocks,
+ * counted after those of all earlier sequences, pass the free ones or its
+ * table row, whose rows pass n_tok, or with a negative length.  The caller
+ * takes counts[0] as the next *n_free (outputs must not overlap inputs).  A
+ * value past 31 bits is reported as 2^31 - 1.
+ * block is a power of two in 64..65536, n_seq at most 8192. */
+int yhip_paged_plan(int32_t* block_table, uint32_t max_blocks, uint32_t table_stride, const int32_t* ctx_lens,
+                    const int32_t* new_lens, const int32_t* free_blocks, uint32_t free_cap, const int32_t* n_free,
+                    uint32_t n_seq, uint32_t n_tok, uint32_t block, int32_t* cu_new, int32_t* kv_lens,
+                    int32_t* slots, int32_t* positions, int32_t* counts, void* stream);
+
+/* RMSNorm of every query and key head, RoPE, and the store of K and V, in one
+ * pass (qwen35 engine.c:886-934; without the norm what yhip_rope_kv_store
+ * does).  Per head y = x / sqrt(mean(x^2) + eps) * w with w = q_norm or k_norm
+ * [head_dim] (YHIP_F32 or YHIP_F16; both NULL: no norm), then the rotation
+ * (rope, n_rot, theta as above) by positions[row]; q goes to q_out, k and v
+ * into the pages at slots[row], rounded as yhip_kv_store rounds.  A row whose
+ * slot is negative or past the n_blocks * block slots is skipped: its q_out
+ * row is left as it was.  Each slot at most once per call.  slots NULL: row r
+ * is position and slot pos_start + r (a contiguous cache: n_blocks 1, block
+ * kv_stride); positions NULL: the same positions.  Angles are
+ * pos * theta^(-2j/dn) in 64 bits (yhip_rope_kv_store rounds frequency and
+ * angle to float as the reference's CPU code does: far positions differ by up
+ * to pos * 6e-8 rad).
+ * q, k, v: rows of `dtype` (YHIP_F32 / F16 / BF16), strides in elements, so
+ * they may be slices of one projection row; q_out NULL skips q, and may be q
+ * itself with the same type and stride.  Pointers aligned to four elements
+ * (pools to 16 bytes), strides multiples of 4, block a multiple of 64, an
+ * MROPE n_rot a multiple of 8. */
+int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
+                               uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                               uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
+                               uint32_t norm_dtype, float eps, uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks,
+                               uint32_t block, const int32_t* positions, const int32_t* slots, uint32_t pos_start,
+                               uint32_t n_tok, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               uint32_t rope, uint32_t n_rot, float theta, void* stream);
+
+/* Causal attention of every sequence's new tokens over its pages: decode
+ * tokens, chunks of a prompt and whole prompts in one batch.  Rows cu_new[i]
+ * .. cu_new[i+1]-1 of q and att_out are sequence i's newest tokens; row t of n
+ * sits at position kv_lens[i] - n + t and attends to keys 0 .. that position,
+ * all stored (a negative position sees nothing: a zero row, as has a sequence
+ * with kv_lens 0).  Rows from cu_new[n_seq] on are left as they were.  dtypes,
+ * strides (multiples of 8; q, att_out and pools 16-byte aligned) and gate as in
+ * yhip_attn_prefill; att_out must not overlap q or gate.  16-bit queries:
+ * scores and P.V from f16 products with fp32 sums; fp32 queries: both at
+ * fp32-level error.  Queries must lie within the f16 range (65504).
+ *
+ * max_new and max_len bound the new tokens and the length of every sequence:
+ * longer ones are cut to them.  max_new 1 (with n_tok = n_seq) is a decode
+ * step.  Table entries outside the pool read as keys and values of zero.
+ * Needs yhip_paged_attn_workspace bytes (16-byte aligned, no initialisation)
+ * for the bounds given; a workspace sized for larger n_tok, n_seq, max_new and
+ * max_len serves smaller ones.  Calls that share a workspace must not run
+ * concurrently. */
+int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                    uint32_t q_stride, const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks,
+                    uint32_t block, const int32_t* block_table, uint32_t max_blocks, uint32_t table_stride,
+                    const int32_t* kv_lens, const int32_t* cu_new, uint32_t n_seq, uint32_t n_tok, uint32_t max_new,
+                    uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float* gate,
+                    uint32_t gate_stride, void* workspace, size_t workspace_bytes, void* stream);
+size_t yhip_paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
+                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+
 /* ---- o_proj (the step after attention) -------------------------------------
  * x[b] += W_o . att[b] for B tokens: matmul(att_out, x2, SLOT_O) then the
  * residual add (engine.c:969-973; qwen35 after its gate, 958-973), with

@@ -60,6 +60,16 @@ SIGNATURES = {
                               c_uint32, c_uint32, c_int, c_void_p]),
     "yhip_gdn_gated_norm": (c_int, [c_void_p, c_uint32, c_void_p, c_uint32, c_void_p, c_uint32, c_void_p, c_uint32,
                                     c_uint32, c_uint32, c_uint32, c_float, c_void_p]),
+    "yhip_paged_plan": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_uint32,
+                                c_uint32, c_uint32] + [c_void_p] * 6),
+    "yhip_qk_norm_rope_kv_store": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_void_p, c_uint32, c_void_p,
+                                           c_uint32, c_uint32, c_void_p, c_void_p, c_uint32, c_float, c_void_p,
+                                           c_void_p, c_uint32, c_uint32, c_void_p, c_void_p] + [c_uint32] * 7 +
+                                   [c_float, c_void_p]),
+    "yhip_paged_attn": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p, c_uint32,
+                                c_uint32, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p] + [c_uint32] * 7 +
+                        [c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
+    "yhip_paged_attn_workspace": (c_size_t, [c_uint32] * 7),
     "yhip_synth_normal": (None, [c_uint64, c_uint64, c_float, POINTER(c_float), c_uint64]),
     "yhip_synth_round_f16": (None, [POINTER(c_float), c_uint64]),
     "yhip_synth_round_bf16": (None, [POINTER(c_float), c_uint64]),
@@ -106,6 +116,42 @@ def current_stream() -> int:
     if _C is None:
         from torch import _C
     return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
+
+
+class _Here:
+    """Nothing to change: the tensors' GPU is the current one."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _gpu_of(fn: str, *tensors):
+    """A context in which the GPU that holds all the tensors (None is passed
+    over) is the current one, so that its current stream takes the launch."""
+    global _C
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise YhipError(EINVAL, f"{fn}: tensor must be on the GPU")
+        if dev is None:
+            dev = t.get_device()
+        elif t.get_device() != dev:
+            raise YhipError(EINVAL, f"{fn}: tensors are on different GPUs")
+    if _C is None:
+        from torch import _C
+    if dev == _C._cuda_getDevice():
+        return _HERE
+    import torch
+
+    return torch.cuda.device(dev)
 
 
 def check(rc: int) -> None:

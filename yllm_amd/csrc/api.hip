@@ -669,4 +669,244 @@ int yhip_gdn_gates(float* beta, float* gate, const float* alpha, const float* dt
     return done(yhip::launch_gdn_gates(beta, gate, alpha, dt_bias, ssm_a, T, n_v_heads, (hipStream_t)stream), fn);
 }
 
+// ---- paged KV cache ---------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// [p, p + n) and [q, q + m) share a byte
+bool overlap(const void* p, uint64_t n, const void* q, uint64_t m)
+{
+    return n && m && (const char*)p < (const char*)q + m && (const char*)q < (const char*)p + n;
+}
+
+// rows of `width` elements of type dt, `stride` apart
+yhip::Rows rows_of(const void* p, uint32_t dt, uint32_t stride, uint64_t width, uint64_t n)
+{
+    const uint64_t e = dt == YHIP_F32 ? 4 : 2;
+    return yhip::Rows{p, stride * e, width * e, n};
+}
+
+// log2 of the positions of a block, or an error
+int block_shift(const char* fn, uint32_t block, uint32_t& shift)
+{
+    if (block < 64 || block > 65536 || (block & (block - 1)))
+        return fail(YHIP_EINVAL, "%s: block %u must be a power of two in 64..65536", fn, block);
+    shift = (uint32_t)__builtin_ctz(block);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int yhip_paged_plan(int32_t* block_table, uint32_t max_blocks, uint32_t table_stride, const int32_t* ctx_lens,
+                    const int32_t* new_lens, const int32_t* free_blocks, uint32_t free_cap, const int32_t* n_free,
+                    uint32_t n_seq, uint32_t n_tok, uint32_t block, int32_t* cu_new, int32_t* kv_lens,
+                    int32_t* slots, int32_t* positions, int32_t* counts, void* stream)
+{
+    const char* fn = "yhip_paged_plan";
+    uint32_t shift;
+    if (int rc = block_shift(fn, block, shift)) return rc;
+    if (n_seq > yhip::kPlanSeqs) return fail(YHIP_EINVAL, "%s: n_seq %u > %u", fn, n_seq, yhip::kPlanSeqs);
+    if (n_tok > 0x7fffffffu) return fail(YHIP_EINVAL, "%s: n_tok %u does not fit 31 bits", fn, n_tok);
+    if (!n_free || !cu_new || !counts || (n_seq && (!block_table || !ctx_lens || !new_lens || !kv_lens)) ||
+        (n_tok && (!slots || !positions)) || (free_cap && !free_blocks))
+        return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    if (max_blocks == 0 || table_stride < max_blocks)
+        return fail(YHIP_EINVAL, "%s: need 1 <= max_blocks (%u) <= table_stride (%u)", fn, max_blocks, table_stride);
+    const struct { const void* p; uint64_t n; } in[] = {
+        {ctx_lens, 4ull * n_seq}, {new_lens, 4ull * n_seq}, {free_blocks, 4ull * free_cap}, {n_free, 4}},
+        out[] = {{block_table, n_seq ? 4ull * ((n_seq - 1ull) * table_stride + max_blocks) : 0}, {cu_new, 4ull * n_seq + 4},
+                 {kv_lens, 4ull * n_seq}, {slots, 4ull * n_tok}, {positions, 4ull * n_tok}, {counts, 16}};
+    for (const auto& o : out) {
+        for (const auto& i : in)
+            if (overlap(o.p, o.n, i.p, i.n)) return fail(YHIP_EINVAL, "%s: an output overlaps an input", fn);
+        for (const auto& o2 : out)
+            if (&o != &o2 && overlap(o.p, o.n, o2.p, o2.n))
+                return fail(YHIP_EINVAL, "%s: two outputs overlap", fn);
+    }
+    yhip::PagedPlanArgs a = {};
+    a.table = block_table;
+    a.ctx = ctx_lens;
+    a.fresh = new_lens;
+    a.free_list = free_blocks;
+    a.n_free = n_free;
+    a.cu_new = cu_new;
+    a.kv_lens = kv_lens;
+    a.slots = slots;
+    a.positions = positions;
+    a.counts = counts;
+    a.n_seq = n_seq;
+    a.n_tok = n_tok;
+    a.width = max_blocks;
+    a.table_stride = table_stride;
+    a.free_cap = free_cap;
+    a.shift = shift;
+    return done(yhip::launch_paged_plan(a, (hipStream_t)stream), fn);
+}
+
+int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
+                               uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                               uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
+                               uint32_t norm_dtype, float eps, uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks,
+                               uint32_t block, const int32_t* positions, const int32_t* slots, uint32_t pos_start,
+                               uint32_t n_tok, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               uint32_t rope, uint32_t n_rot, float theta, void* stream)
+{
+    const char* fn = "yhip_qk_norm_rope_kv_store";
+    // (one kv head's page takes the place of its contiguous cache)
+    if (block == 0 || block % 64) return fail(YHIP_EINVAL, "%s: block %u must be a positive multiple of 64", fn, block);
+    if (int rc = check_heads(fn, n_heads, n_kv_heads, head_dim, block)) return rc;
+    if (!k || !v || !kpool || !vpool || (q_out && !q)) return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    if (!q_norm != !k_norm) return fail(YHIP_EINVAL, "%s: q_norm and k_norm come together", fn);
+    if (!valid_dtype(dtype) || (q_out && !valid_dtype(q_out_dtype))) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
+    if (q_norm && norm_dtype != YHIP_F32 && norm_dtype != YHIP_F16)
+        return fail(YHIP_EINVAL, "%s: norm_dtype must be YHIP_F32 or YHIP_F16", fn);
+    if (q_norm && !(eps >= 0.0f)) return fail(YHIP_EINVAL, "%s: eps must not be negative", fn);
+    if (rope > YHIP_ROPE_MROPE) return fail(YHIP_EINVAL, "%s: unknown rope kind %u", fn, rope);
+    if (rope == YHIP_ROPE_MROPE && (n_rot == 0 || n_rot % 8 || n_rot > head_dim))
+        return fail(YHIP_EINVAL, "%s: n_rot %u must be a multiple of 8 and at most head_dim", fn, n_rot);
+    if (rope != YHIP_ROPE_NONE && !(theta > 0.0f)) return fail(YHIP_EINVAL, "%s: theta must be positive", fn);
+    const uint64_t kv_dim = (uint64_t)n_kv_heads * head_dim, qd = (uint64_t)n_heads * head_dim;
+    if (k_stride < kv_dim || v_stride < kv_dim || (q_out && (q_stride < qd || q_out_stride < qd)))
+        return fail(YHIP_EINVAL, "%s: strides must cover the heads", fn);
+    if ((uint64_t)n_blocks * block > 0x7fffffffull)
+        return fail(YHIP_EINVAL, "%s: %u blocks of %u positions pass 31 bits", fn, n_blocks, block);
+    if (!slots && (positions || (uint64_t)pos_start + n_tok > (uint64_t)n_blocks * block))
+        return fail(YHIP_EINVAL, "%s: without slots, rows are the positions %u.. and must fit the pool", fn, pos_start);
+    if (n_tok > 0x7fffffffu || (uint64_t)n_tok * n_heads > 0x7fffffffull)
+        return fail(YHIP_EINVAL, "%s: too many rows", fn);
+    // runs of four elements move as one access
+    const uint32_t al = dtype == YHIP_F32 ? 16u : 8u, qo_al = q_out_dtype == YHIP_F32 ? 16u : 8u,
+                   w_al = norm_dtype == YHIP_F32 ? 16u : 8u;
+    if ((uintptr_t)k % al || (uintptr_t)v % al || (uintptr_t)kpool % 16 || (uintptr_t)vpool % 16 || k_stride % 4 ||
+        v_stride % 4 || (q_out && ((uintptr_t)q % al || (uintptr_t)q_out % qo_al || q_stride % 4 || q_out_stride % 4)) ||
+        (q_norm && ((uintptr_t)q_norm % w_al || (uintptr_t)k_norm % w_al)))
+        return fail(YHIP_EINVAL, "%s: rows, weights and pools must be aligned to four elements (pools to 16 bytes)", fn);
+    if (n_tok == 0) return done(hipSuccess, "");
+    if (q_out) {
+        const yhip::Rows ro = rows_of(q_out, q_out_dtype, q_out_stride, qd, n_tok);
+        const bool same = q_out == q && q_out_dtype == dtype && q_out_stride == q_stride;
+        if ((!same && rows_overlap(ro, rows_of(q, dtype, q_stride, qd, n_tok))) ||
+            rows_overlap(ro, rows_of(k, dtype, k_stride, kv_dim, n_tok)) ||
+            rows_overlap(ro, rows_of(v, dtype, v_stride, kv_dim, n_tok)))
+            return fail(YHIP_EINVAL, "%s: q_out overlaps its inputs (it may be q itself, of the same type and stride)", fn);
+    }
+    yhip::QkNormRopeArgs a = {};
+    a.q_out = q_out;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.kc = kpool;
+    a.vc = vpool;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.positions = positions;
+    a.slots = slots;
+    a.dtype = dtype;
+    a.q_out_dtype = q_out_dtype;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.q_out_stride = q_out_stride;
+    a.norm_f16 = norm_dtype == YHIP_F16;
+    a.n_tok = n_tok;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv_heads;
+    a.D = head_dim;
+    a.block = block;
+    a.n_slots = n_blocks * block;
+    a.pos_start = pos_start;
+    a.kind = rope;
+    a.n_rot = rope == YHIP_ROPE_MROPE ? n_rot : head_dim;
+    a.eps = eps;
+    if (rope != YHIP_ROPE_NONE) {
+        // the last table is kept per thread
+        thread_local float t_theta = 0.0f;
+        thread_local uint32_t t_span = 0;
+        thread_local double t_turns[128];
+        if (t_span != a.n_rot || t_theta != theta) {
+            for (uint32_t j = 0; j < a.n_rot / 2; ++j)
+                t_turns[j] = pow((double)theta, -2.0 * j / a.n_rot) / (2.0 * M_PI);
+            t_span = a.n_rot;
+            t_theta = theta;
+        }
+        memcpy(a.turns, t_turns, sizeof(double) * (a.n_rot / 2));
+    }
+    return done(yhip::launch_qk_norm_rope(a, (hipStream_t)stream), fn);
+}
+
+size_t yhip_paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
+                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim)
+{
+    if (n_kv_heads == 0 || !valid_head_dim(head_dim)) return 0;
+    return yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
+}
+
+int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                    uint32_t q_stride, const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks,
+                    uint32_t block, const int32_t* block_table, uint32_t max_blocks, uint32_t table_stride,
+                    const int32_t* kv_lens, const int32_t* cu_new, uint32_t n_seq, uint32_t n_tok, uint32_t max_new,
+                    uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float* gate,
+                    uint32_t gate_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* fn = "yhip_paged_attn";
+    if (!att_out || !q || !kpool || !vpool || !block_table || !kv_lens || !cu_new)
+        return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    if (!valid_dtype(out_dtype) || !valid_dtype(q_dtype)) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
+    uint32_t shift;
+    if (int rc = block_shift(fn, block, shift)) return rc;
+    if (int rc = check_heads(fn, n_heads, n_kv_heads, head_dim, block)) return rc;
+    if (max_blocks == 0 || table_stride < max_blocks)
+        return fail(YHIP_EINVAL, "%s: need 1 <= max_blocks (%u) <= table_stride (%u)", fn, max_blocks, table_stride);
+    if (max_len == 0 || max_len > (uint64_t)max_blocks * block || max_len > 0x7fffffffu)
+        return fail(YHIP_EINVAL, "%s: max_len %u must be in 1..max_blocks * block", fn, max_len);
+    if (n_seq > 65535 || n_tok > 0x7fffffffu || max_new > n_tok)
+        return fail(YHIP_EINVAL, "%s: n_seq %u, n_tok %u, max_new %u out of range", fn, n_seq, n_tok, max_new);
+    const uint64_t row = (uint64_t)n_heads * head_dim;
+    if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8)
+        return fail(YHIP_EINVAL, "%s: q_stride/out_stride must be >= n_heads*head_dim and a multiple of 8", fn);
+    if (gate && gate_stride < row) return fail(YHIP_EINVAL, "%s: gate_stride too small", fn);
+    if (((uintptr_t)q | (uintptr_t)att_out | (uintptr_t)kpool | (uintptr_t)vpool) % 16)
+        return fail(YHIP_EINVAL, "%s: q, att_out and the pools must be 16-byte aligned", fn);
+    if (n_tok == 0 || n_seq == 0 || max_new == 0) return done(hipSuccess, "");
+    const yhip::Rows ro = rows_of(att_out, out_dtype, out_stride, row, n_tok);
+    if (rows_overlap(ro, rows_of(q, q_dtype, q_stride, row, n_tok)) ||
+        (gate && rows_overlap(ro, rows_of(gate, YHIP_F32, gate_stride, row, n_tok))))
+        return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
+    const size_t need = yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        return fail(YHIP_ENOSPC, "%s: %zu bytes of workspace (16-byte aligned) needed, %zu given", fn, need,
+                    workspace_bytes);
+    yhip::PagedAttnArgs a = {};
+    a.q = q;
+    a.q_dtype = q_dtype;
+    a.q_stride = q_stride;
+    a.kc = kpool;
+    a.vc = vpool;
+    a.table = block_table;
+    a.kv_lens = kv_lens;
+    a.cu_new = cu_new;
+    a.out = att_out;
+    a.out_dtype = out_dtype;
+    a.out_stride = out_stride;
+    a.gate = gate;
+    a.gate_stride = gate_stride;
+    a.table_stride = table_stride;
+    a.n_seq = n_seq;
+    a.n_tok = n_tok;
+    a.max_new = max_new;
+    a.max_len = max_len;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv_heads;
+    a.D = head_dim;
+    a.shift = shift;
+    a.n_blocks = n_blocks;
+    a.c = (float)(1.4426950408889634 / sqrt((double)head_dim));
+    a.ws = need ? workspace : nullptr;
+    return done(yhip::launch_paged_attn(a, (hipStream_t)stream), fn);
+}
+
 }  // extern "C"

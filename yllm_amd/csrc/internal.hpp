@@ -131,6 +131,66 @@ struct RopeArgs {
 };
 hipError_t launch_rope_kv(RopeArgs a, hipStream_t st);
 
+// ---- paged_plan.hip ----
+constexpr uint32_t kPlanSeqs = 8192;  // sequences of one plan (their prefix sums are held in LDS)
+struct PagedPlanArgs {
+    int* table;             // [n_seq] rows table_stride apart, width entries each
+    const int* ctx;         // [n_seq] positions stored before the step
+    const int* fresh;       // [n_seq] new tokens
+    const int* free_list;   // [free_cap]
+    const int* n_free;      // [1]
+    int* cu_new;            // [n_seq + 1]
+    int* kv_lens;           // [n_seq]
+    int* slots;             // [n_tok]
+    int* positions;         // [n_tok]
+    int* counts;            // [4]
+    uint32_t n_seq, n_tok, width, table_stride, free_cap, shift;  // block = 1 << shift
+};
+hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t st);
+
+// ---- qk_norm_rope.hip ----
+struct QkNormRopeArgs {
+    void* q_out;            // rows q_out_stride apart, dtype q_out_dtype (null: no q)
+    const void* q;          // rows of dtype `dtype`, q_stride apart
+    const void* k;
+    const void* v;
+    uint16_t* kc;           // K pages [n_blocks][n_kv][block][D]
+    uint16_t* vc;           // V pages [n_blocks][n_kv][block / 32][D][32]
+    const void* q_norm;     // [D] f32, or f16 when norm_f16; null: no norm
+    const void* k_norm;
+    const int* positions;   // [n_tok], or null: pos_start + row
+    const int* slots;       // [n_tok], or null: the position
+    uint32_t dtype, q_out_dtype, q_stride, k_stride, v_stride, q_out_stride, norm_f16;
+    uint32_t n_tok, n_heads, n_kv, D, block, n_slots, pos_start, kind, n_rot;
+    float eps;
+    // set by the launcher: waves per token, heads per wave, workgroups of each role
+    uint32_t groups, heads_per_wave, rope_blocks, v_blocks;
+    // turns[j] = theta^(-2j / span) / 2 pi for the rotated pairs j < span / 2
+    double turns[128];
+};
+hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st);
+
+// ---- attn_paged.hip ----
+struct PagedAttnArgs {
+    const void* q;
+    uint32_t q_dtype, q_stride;
+    const uint16_t* kc;     // K pages [n_blocks][n_kv][block][D]
+    const uint16_t* vc;     // V pages [n_blocks][n_kv][block / 32][D][32]
+    const int* table;       // [n_seq] rows table_stride apart
+    const int* kv_lens;     // [n_seq]
+    const int* cu_new;      // [n_seq + 1]
+    void* out;
+    uint32_t out_dtype, out_stride;
+    const float* gate;
+    uint32_t gate_stride;
+    uint32_t table_stride, n_seq, n_tok, max_new, max_len, n_heads, n_kv, D, shift, n_blocks;
+    float c;                // log2(e) / sqrt(D)
+    void* ws;
+};
+size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                            uint32_t n_kv, uint32_t D);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t st);
+
 // ---- o_proj.hip ----
 struct OProjArgs {
     float* x;               // [B] rows x_stride apart, residual in / out
