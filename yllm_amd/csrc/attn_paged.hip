@@ -7,106 +7,146 @@
 // position sees nothing and its row is zero.  Key j of a sequence is row
 // j % block of page table[j / block].
 //
-// One wave per (row, query head): scores of 64 keys at a time, one per lane,
-// the running maximum and sum of the softmax, then P.V with the lanes over
-// the dimensions.  Everything is fp32.
+// The products run on the prefill kernels (prefill_kernel.hpp) over pieces of
+// 128-row items, dealt out as paged_items.hpp says; the merge kernel here
+// joins the pieces of items that a chunk's end cut.
 #include "common.hpp"
 #include "internal.hpp"
+#include "paged_items.hpp"
+#include "prefill_kernel.hpp"
+
+#include <algorithm>
 
 namespace yhip {
 namespace {
 
-__device__ inline float sigmoid_ref(float g) { return 1.0f / (1.0f + expf(-g)); }
-
+// Workgroup (j, y): rows 32 y .. of the split item that chunk j begins, if
+// any.  Pieces are joined in their order; a thread holds four dimensions of a
+// row, and a round's loads go out together.
 template <int D>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
 {
-    __shared__ float s_q[4][D];
-    __shared__ float s_p[4][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t row = blockIdx.x, h = blockIdx.y * 4u + wave;
-    if (h >= a.n_heads) return;  // wave-uniform, and no workgroup barrier follows
-    uint32_t lo = 0, hi = a.n_seq;  // cu[lo] <= row < cu[hi]
-    if (row >= (uint32_t)max(a.cu_new[a.n_seq], 0)) return;  // rows behind the last sequence
-    while (hi - lo > 1) {
-        const uint32_t m = (lo + hi) >> 1;
-        if ((uint32_t)max(a.cu_new[m], 0) <= row) lo = m;
-        else hi = m;
-    }
-    const int len = max(0, min(a.kv_lens[lo], (int)a.max_len));
-    const int pos = len - (a.cu_new[lo + 1] - a.cu_new[lo]) + ((int)row - a.cu_new[lo]);
-    const int keys = min(pos + 1, len);
-    const int* table = a.table + (size_t)lo * a.table_stride;
-    const uint32_t kvh = h * a.n_kv / a.n_heads, mask = (1u << a.shift) - 1u;
-    for (uint32_t d = lane; d < D; d += 64)
-        s_q[wave][d] = load_as_f32(a.q, (size_t)row * a.q_stride + (size_t)h * D + d, a.q_dtype);
-    __builtin_amdgcn_wave_barrier();
-    constexpr int NO = D / 64;
-    float m = -1e30f, l = 0.0f, o[NO] = {};
-    for (int k0 = 0; k0 < keys; k0 += 64) {
-        const int key = k0 + (int)lane;
-        const uint32_t page0 = (uint32_t)table[(uint32_t)k0 >> a.shift];
-        float s = -INFINITY;
-        if (key < keys) {
-            const uint32_t page = (uint32_t)table[(uint32_t)key >> a.shift];
-            s = 0.0f;
-            if (page < a.n_blocks) {
-                const uint16_t* kr = a.kc + ((((size_t)page * a.n_kv + kvh) << a.shift) + ((uint32_t)key & mask)) * D;
-                for (int d = 0; d < D; ++d) s = fmaf(f16_bits_to_f32(kr[d]), s_q[wave][d], s);
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    constexpr uint32_t C4 = D / 4, RP = 256 / C4, kRound = 8;
+    const uint32_t j = blockIdx.x;
+    const PagedDesc d = reinterpret_cast<const PagedDesc*>(a.desc)[j];
+    if (d.n == 0) return;
+    const uint32_t dim = threadIdx.x % C4 * 4u;
+    for (uint32_t r0 = blockIdx.y * 32u; r0 < blockIdx.y * 32u + 32u; r0 += RP) {
+        const uint32_t r = r0 + threadIdx.x / C4;
+        const PagedRow rw = paged_row(a, d, r);
+        if (!rw.valid) return;
+        float M = -1e30f, L = 0.0f;
+        f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t s0 = 0; s0 < d.n; s0 += kRound) {
+            f32x2 ml[kRound];
+            f32x4 os[kRound];
+#pragma unroll
+            for (uint32_t i = 0; i < kRound; ++i) {
+                // piece s in slot 2 (j + s) + (s == 0); past the last one, the first again, counted as nothing
+                const uint32_t s = s0 + i < d.n ? s0 + i : 0u;
+                const size_t p = (size_t)(2 * (j + s) + (s == 0)) * kItemRows + r;
+                ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * p);
+                os[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + dim);
             }
-            s *= a.c;
-        }
-        float mx = s;
-        for (int i = 32; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
-        const float mn = fmaxf(m, mx), alpha = fast_exp2(m - mn);
-        const float p = key < keys ? fast_exp2(s - mn) : 0.0f;
-        m = mn;
-        l = l * alpha + p;
-        s_p[wave][lane] = p;
-        __builtin_amdgcn_wave_barrier();
-        const int nk = min(64, keys - k0);
-        for (int r = 0; r < NO; ++r) {
-            const uint32_t d = lane + 64u * r;
-            float acc = o[r] * alpha;
-            if (page0 < a.n_blocks) {  // a block is 64 positions or more: one page
-                const uint16_t* vr = a.vc + ((((size_t)page0 * a.n_kv + kvh) << a.shift) + ((uint32_t)k0 & mask)) * D;
-                for (int j = 0; j < nk; ++j)
-                    acc = fmaf(s_p[wave][j], f16_bits_to_f32(vr[(size_t)(j / 32) * 32 * D + d * 32 + j % 32]), acc);
+            float mr = M;
+#pragma unroll
+            for (uint32_t i = 0; i < kRound; ++i)
+                if (s0 + i < d.n) mr = fmaxf(mr, ml[i][0]);
+            const float co = fast_exp2(M - mr);
+            L *= co;
+            O *= co;
+#pragma unroll
+            for (uint32_t i = 0; i < kRound; ++i) {
+                if (s0 + i >= d.n) continue;
+                const float c = fast_exp2(ml[i][0] - mr);
+                L += ml[i][1] * c;
+                O += os[i] * c;
             }
-            o[r] = acc;
+            M = mr;
         }
-        __builtin_amdgcn_wave_barrier();
-    }
-    for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
-    for (int r = 0; r < NO; ++r) {
-        const uint32_t d = lane + 64u * r;
-        float v = l > 0.0f || l != l ? o[r] / l : 0.0f;
-        if (a.gate) v *= sigmoid_ref(a.gate[(size_t)row * a.gate_stride + (size_t)h * D + d]);
-        const size_t at = (size_t)row * a.out_stride + (size_t)h * D + d;
-        if (a.out_dtype == kF32) {
-            reinterpret_cast<float*>(a.out)[at] = v;
-        } else if (a.out_dtype == kF16) {
-            reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)v;
-        } else {
-            const uint32_t x = __builtin_bit_cast(uint32_t, v);
-            reinterpret_cast<uint16_t*>(a.out)[at] =
-                v != v ? (uint16_t)((x >> 16) | 0x40u) : (uint16_t)((x + 0x7fffu + ((x >> 16) & 1u)) >> 16);
+        f32x4 v = O * (L == 0.0f ? 0.0f : 1.0f / L);
+        if (a.gate) {
+            const float* gp = a.gate + (size_t)rw.b * a.gate_stride + (size_t)rw.h * D + dim;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= sigmoid_ref(gp[e]);
         }
+        store_out4(a.out, (size_t)rw.b * a.out_stride + (size_t)rw.h * D + dim, a.out_dtype, v);
     }
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 0; }
+namespace {
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t st)
+// The shortest chunk, and the longest item that is not cut, in units of 64 keys.
+constexpr uint32_t kMinUnits = 4, kSnapUnits = 4;
+
+uint32_t round8(uint64_t x) { return (uint32_t)((x + 7) / 8 * 8); }
+
+// Workgroups of a launch: what the GPU holds at once (per_cu a CU), or all that
+// the bounds on the batch can fill.
+uint32_t paged_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t per_cu)
 {
-    const dim3 grid(a.n_tok, (a.n_heads + 3) / 4);
+    const uint64_t gmax = (n_heads + n_kv - 1) / n_kv;
+    const uint64_t items = (uint64_t)n_kv * gmax * ((uint64_t)n_tok / kItemRows + n_seq);
+    const uint64_t most = items * ((max_len + kUnitKeys - 1) / kUnitKeys) / kMinUnits + 1;
+    const uint64_t full = (uint64_t)per_cu * (uint64_t)n_cus();
+    return round8(most < full ? most : full);
+}
+
+size_t align256a(size_t x) { return (x + 255) / 256 * 256; }
+
+size_t paged_bytes(uint32_t wgs, uint32_t D)
+{
+    const size_t rows = (size_t)2 * wgs * kItemRows;
+    return align256a((size_t)wgs * sizeof(PagedDesc)) + align256a(rows * 2 * sizeof(float)) + rows * D * sizeof(float);
+}
+
+template <int D, int NG, bool QS>
+void launch_tiles(const PagedAttnArgs& a, hipStream_t st)
+{
+    constexpr int threads = 256 * NG * (D > 128 ? 2 : 1);
+    hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, PagedAttnArgs>), dim3(a.n_wg), dim3(threads), 0, st, a);
+}
+
+}  // namespace
+
+size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t, uint32_t max_len, uint32_t n_heads, uint32_t n_kv,
+                            uint32_t D)
+{
+    return paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1), D);
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
+{
+    PagedAttnArgs a = in;
+    const bool qs = a.q_dtype == kF32;
+    a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
+    a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, a.D <= 128 && !qs ? 2 : 1);
+    a.min_units = kMinUnits;
+    a.snap_units = kSnapUnits;
+    char* p = reinterpret_cast<char*>(a.ws);
+    a.desc = p;
+    p += align256a((size_t)a.n_wg * sizeof(PagedDesc));
+    a.part_ml = reinterpret_cast<float*>(p);
+    a.part_o = reinterpret_cast<float*>(p + align256a((size_t)2 * a.n_wg * kItemRows * 2 * sizeof(float)));
     switch (a.D) {
-    case 64: hipLaunchKernelGGL(paged_rows_kernel<64>, grid, dim3(256), 0, st, a); break;
-    case 128: hipLaunchKernelGGL(paged_rows_kernel<128>, grid, dim3(256), 0, st, a); break;
-    case 256: hipLaunchKernelGGL(paged_rows_kernel<256>, grid, dim3(256), 0, st, a); break;
+    case 64: qs ? launch_tiles<64, 1, true>(a, st) : launch_tiles<64, 1, false>(a, st); break;
+    case 128: qs ? launch_tiles<128, 2, true>(a, st) : launch_tiles<128, 1, false>(a, st); break;
+    case 256:
+        if (qs) launch_tiles<256, 1, true>(a, st);
+        else hipLaunchKernelGGL((prefill_halves_kernel<256, false, PagedAttnArgs>), dim3(a.n_wg), dim3(512), 0, st, a);
+        break;
     default: return hipErrorInvalidValue;
+    }
+    if ((a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
+        const dim3 grid(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + 31) / 32);
+        switch (a.D) {
+        case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, st, a); break;
+        case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, st, a); break;
+        default: hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, st, a); break;
+        }
     }
     return hipGetLastError();
 }

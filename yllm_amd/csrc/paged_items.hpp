@@ -1,0 +1,284 @@
+// paged_items.hpp -- how the work of a paged attention launch is dealt out.
+//
+// A sequence's new tokens form items of up to 128 rows that share a kv head:
+// with 128 tokens or more, 128 consecutive tokens of one query head; with
+// fewer, the group's heads' tokens one after the other.  An item walks the
+// keys its last row sees, in units of 64.  All units of the launch, sequence
+// by sequence, form one line, which is cut into equal chunks, one per resident
+// workgroup: whatever the lengths of the batch, every workgroup walks the same
+// number of units.  A cut inside an item leaves partial results (running
+// maximum, sum and unnormalised output), at most one at each end of a chunk,
+// which a merge kernel joins in order; cuts inside short items move to the
+// item's start, which costs less than joining them.  Lengths are read on the
+// device, so a captured launch replays with new ones.
+#pragma once
+
+#include "common.hpp"
+#include "internal.hpp"
+
+namespace yhip {
+namespace {
+
+constexpr uint32_t kItemRows = 128;
+constexpr uint32_t kUnitKeys = 64;
+
+__device__ inline uint32_t uni(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ inline uint64_t uni64(uint64_t x) { return (uint64_t)uni((uint32_t)(x >> 32)) << 32 | uni((uint32_t)x); }
+
+// tables and lengths do not change during a launch: uniform reads may go
+// through the scalar cache
+typedef const int __attribute__((address_space(4))) * ConstInts;
+__device__ inline ConstInts const_ints(const int* p) { return (ConstInts)(uintptr_t)p; }
+
+// first query head of kv head g (common mapping h * n_kv / n_heads)
+__device__ inline uint32_t head0(const PagedAttnArgs& a, uint32_t g) { return (g * a.n_heads + a.n_kv - 1) / a.n_kv; }
+
+// A sequence's rows and keys: rows row0 .. row0 + nq - 1, token t at position
+// pos0 + t (negative: sees nothing), L keys.
+struct PagedSeq {
+    uint32_t row0, nq;
+    int pos0, L;
+};
+
+__device__ inline PagedSeq paged_seq(const PagedAttnArgs& a, int c0, int c1, int len)
+{
+    PagedSeq s;
+    s.row0 = min((uint32_t)max(c0, 0), a.n_tok);
+    const uint32_t n = min((uint32_t)max(c1, 0), a.n_tok) - s.row0;
+    s.nq = (int)n > 0 ? min(n, a.max_new) : 0u;
+    s.L = min(max(len, 0), (int)a.max_len);
+    s.pos0 = s.L - (int)((int)n > 0 ? n : 0u);
+    return s;
+}
+
+__device__ inline uint32_t units_to(int keys) { return keys > 0 ? ((uint32_t)keys + kUnitKeys - 1) / kUnitKeys : 1u; }
+
+// Units of one query head's (or one packed group's) items, in order:
+// packed items all see every key; of plain ones, block b of 128 tokens sees
+// c + 2 (b + 1) units (c: those of the keys before the new tokens), the last
+// block all.  (Tokens at negative positions are counted as if at their index;
+// the walk leaves out what is not there.)
+__device__ inline uint32_t plain_before(uint32_t b, uint32_t c) { return b * c + b * (b + 1); }
+__device__ inline uint32_t plain_last(const PagedSeq& s) { return units_to(max(s.pos0, 0) + (int)s.nq); }
+
+__device__ inline uint64_t seq_units(const PagedAttnArgs& a, const PagedSeq& s)
+{
+    if (s.nq == 0) return 0;
+    if (s.nq < kItemRows) return (uint64_t)a.n_kv * ((a.gmax * s.nq + kItemRows - 1) / kItemRows) * units_to(s.L);
+    const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows, c = ((uint32_t)max(s.pos0, 0) + kUnitKeys - 1) / kUnitKeys;
+    return (uint64_t)a.n_kv * a.gmax * (plain_before(nb - 1, c) + plain_last(s));
+}
+
+// A piece of an item: `n` key tiles from t0 on.  part: 0 the whole item, 1 its
+// first piece, 2 a later one.  idle: no key of it is seen (its tile is loaded
+// and not used).
+struct PagedItem {
+    uint32_t seq, row0, nq, kvh, h, qb, pack;
+    int pos0;
+    uint32_t kmax, t0, nt, part, idle, last;
+};
+
+// what a workgroup that begins a split item leaves for the merge
+struct PagedDesc {
+    uint32_t n;  // pieces; 0: none
+    uint32_t row0, nq, kvh, h, qb, pack, pad;
+};
+
+struct PagedCursor {
+    uint64_t u, end, first, base, units;  // next unit; chunk end and begin; the sequence's first unit and count
+    uint32_t seq, chunk, j, fresh;
+    PagedSeq s;
+};
+
+__device__ inline void cursor_seq(const PagedAttnArgs& a, PagedCursor& C)
+{
+    const ConstInts cu = const_ints(a.cu_new);
+    C.s = paged_seq(a, cu[C.seq], cu[C.seq + 1], const_ints(a.kv_lens)[C.seq]);
+    C.units = seq_units(a, C.s);
+}
+
+// This workgroup's place in the line; false if it has no chunk.  Active chunks
+// are spread over the XCDs (consecutive workgroups go to the 8 XCDs in turn),
+// neighbours on one XCD, whose L2 then holds the keys they share.  `scratch`:
+// 24 words of LDS, free again after the call's last barrier.
+template <int NT>
+__device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C)
+{
+    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+    const bool small = a.n_seq <= 64u;  // every wave scans for itself
+    const uint32_t per = small ? 1u : (a.n_seq + NT - 1) / NT;
+    const uint32_t lo = min((small ? lane : t) * per, a.n_seq), hi = min(lo + per, a.n_seq);
+    uint64_t sum = 0;
+    for (uint32_t i = lo; i < hi; ++i) sum += seq_units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
+    uint64_t inc = sum;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up((unsigned long long)inc, d);
+        if (lane >= d) inc += o;
+    }
+    uint64_t before = inc - sum, total = uni64(__shfl((unsigned long long)inc, 63));
+    if (!small) {
+        if (lane == 63) scratch[wave] = inc;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < NT / 64; ++w) {
+            if (w < wave) before += scratch[w];
+            total += scratch[w];
+        }
+        total = uni64(total);
+    }
+    const uint64_t even = (total >> 32) ? (total + a.n_wg - 1) / a.n_wg : ((uint32_t)total + a.n_wg - 1) / a.n_wg;
+    C.chunk = (uint32_t)max(even, (uint64_t)a.min_units);
+    const uint32_t active = (total >> 32) ? (uint32_t)((total + C.chunk - 1) / C.chunk)
+                                          : ((uint32_t)total + C.chunk - 1) / C.chunk;
+    const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
+    C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
+    C.first = (uint64_t)C.j * C.chunk;
+    if (C.j >= active) return false;  // workgroup-uniform
+    C.u = C.first;
+    C.end = min(C.first + C.chunk, total);
+    C.fresh = 1;
+    const bool mine = before <= C.first && C.first < before + sum;
+    if (small) {
+        const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(mine));
+        C.seq = at;
+        C.base = uni64(__shfl((unsigned long long)before, (int)at));
+    } else {
+        if (mine) {
+            uint32_t i = lo;
+            for (;; ++i) {
+                const uint64_t n = seq_units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
+                if (C.first < before + n) break;
+                before += n;
+            }
+            scratch[16] = i;
+            scratch[17] = before;
+        }
+        __syncthreads();
+        C.seq = uni((uint32_t)scratch[16]);
+        C.base = uni64(scratch[17]);
+        __syncthreads();
+    }
+    cursor_seq(a, C);
+    return true;
+}
+
+// The chunk's next piece in tiles of BN keys; false past its end.
+template <int BN>
+__device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedItem& I)
+{
+    constexpr uint32_t TU = kUnitKeys / BN;  // tiles per unit
+    for (;;) {
+        if (C.u >= C.end) return false;
+        while (C.u >= C.base + C.units) {
+            C.base += C.units;
+            ++C.seq;
+            cursor_seq(a, C);
+        }
+        const PagedSeq& s = C.s;
+        uint64_t off = C.u - C.base;
+        const uint64_t per_kv = C.units / a.n_kv;
+        uint32_t kvh = 0;
+        while (off >= per_kv) {
+            off -= per_kv;
+            ++kvh;
+        }
+        uint32_t rem = (uint32_t)off, T, t;
+        const uint32_t h0 = head0(a, kvh), h1 = head0(a, kvh + 1);
+        I.pack = s.nq < kItemRows;
+        bool none;  // an item of the fullest group that this one does not have
+        int seen;
+        if (I.pack) {
+            T = units_to(s.L);
+            I.qb = rem / T;
+            t = rem - I.qb * T;
+            I.h = h0;
+            none = I.qb * kItemRows >= (h1 - h0) * s.nq;
+            seen = s.L;
+        } else {
+            const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows,
+                           c = ((uint32_t)max(s.pos0, 0) + kUnitKeys - 1) / kUnitKeys;
+            // block b with plain_before(b) <= rem / gmax < plain_before(b + 1)
+            const uint32_t want = rem / a.gmax;
+            const float hc = 0.5f * (float)(c + 1u);
+            uint32_t b = (uint32_t)max(sqrtf(hc * hc + (float)want) - hc, 0.0f);
+            b = min(b, nb - 1);
+            while (b > 0 && plain_before(b, c) > want) --b;
+            while (b + 1 < nb && plain_before(b + 1, c) <= want) ++b;
+            rem -= a.gmax * plain_before(b, c);
+            T = b + 1 < nb ? c + 2 * (b + 1) : plain_last(s);
+            const uint32_t g = rem / T;
+            t = rem - g * T;
+            I.qb = b;
+            I.h = h0 + g;
+            none = I.h >= h1;
+            seen = s.pos0 + (int)min(s.nq, (b + 1) * kItemRows);
+        }
+        const uint64_t i0 = C.u - t, i1 = i0 + T;
+        if (C.fresh && t > 0 && T <= a.snap_units) {  // the chunk begins inside a short item: all of it
+            C.u = i0;
+            t = 0;
+        }
+        C.fresh = 0;
+        uint32_t n = T - t;
+        if (C.end < i1) {  // it ends inside one
+            if (T <= a.snap_units) {
+                C.u = C.end;
+                return false;
+            }
+            n = (uint32_t)(C.end - C.u);
+        }
+        C.u += n;
+        if (none) continue;
+        I.part = n == T ? 0u : t == 0 ? 1u : 2u;
+        I.last = C.j + (uint32_t)(i1 - 1 - C.first) / C.chunk;  // the chunk that ends the item
+        I.seq = C.seq;
+        I.row0 = s.row0;
+        I.nq = s.nq;
+        I.pos0 = s.pos0;
+        I.kvh = kvh;
+        I.kmax = (uint32_t)max(seen - 1, 0);
+        const uint32_t all = I.kmax / BN + 1;
+        I.t0 = t * TU;
+        I.idle = seen <= 0 || I.t0 >= all;
+        if (I.idle) {
+            I.t0 = all - 1;
+            I.nt = 1;
+        } else {
+            I.nt = min(all - I.t0, n * TU);
+        }
+        return true;
+    }
+}
+
+// The workgroup's last piece, which may begin a split item: what the merge
+// needs to know of it.
+__device__ inline void paged_leave(const PagedAttnArgs& a, const PagedCursor& C, const PagedItem& I)
+{
+    if (threadIdx.x != 0) return;
+    PagedDesc* d = reinterpret_cast<PagedDesc*>(a.desc) + C.j;
+    if (I.part == 1) *d = PagedDesc{I.last - C.j + 1, I.row0, I.nq, I.kvh, I.h, I.qb, I.pack, 0};
+    else d->n = 0;
+}
+
+// byte address and size (0: outside the pool) of kv head kvh's part of the
+// page that holds key `key`; K rows and V tiles of a page are the same bytes
+struct PagedTile {
+    uint64_t at;
+    uint32_t bytes;
+};
+template <int D>
+__device__ inline PagedTile paged_tile(const PagedAttnArgs& a, uint32_t page, uint32_t kvh)
+{
+    const bool in = page < a.n_blocks;
+    const uint32_t head_bytes = (uint32_t)(D * 2) << a.shift;
+    return PagedTile{in ? ((uint64_t)page * a.n_kv + kvh) * head_bytes : 0u, in ? head_bytes : 0u};
+}
+__device__ inline uint32_t paged_page(const PagedAttnArgs& a, uint32_t seq, uint32_t key)
+{
+    return (uint32_t)const_ints(a.table + (size_t)seq * a.table_stride)[key >> a.shift];
+}
+
+}  // namespace
+}  // namespace yhip
