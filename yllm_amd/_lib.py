@@ -118,37 +118,22 @@ def current_stream() -> int:
     return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
 
 
-class _Here:
-    """Nothing to change: the tensors' GPU is the current one."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def _gpu_of(fn: str, *tensors):
-    """A context in which the GPU that holds all the tensors (None is passed
-    over) is the current one, so that its current stream takes the launch."""
+def elsewhere(fn: str, dev: int, *tensors):
+    """None where all the tensors (None is passed over) are on GPU number `dev`
+    and that is the current one; a context that makes it so where it is another
+    one, so that its current stream takes the launch.  Raises for tensors in
+    host memory or on several GPUs."""
     global _C
-    dev = None
+    if dev < 0:
+        raise YhipError(EINVAL, f"{fn}: tensor must be on the GPU")
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise YhipError(EINVAL, f"{fn}: tensor must be on the GPU")
-        if dev is None:
-            dev = t.get_device()
-        elif t.get_device() != dev:
-            raise YhipError(EINVAL, f"{fn}: tensors are on different GPUs")
+        if t is not None and t.get_device() != dev:
+            raise YhipError(EINVAL, f"{fn}: tensor must be on the GPU" if t.get_device() < 0
+                            else f"{fn}: tensors are on different GPUs")
     if _C is None:
         from torch import _C
     if dev == _C._cuda_getDevice():
-        return _HERE
+        return None
     import torch
 
     return torch.cuda.device(dev)

@@ -865,6 +865,7 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
         return fail(YHIP_EINVAL, "%s: max_len %u must be in 1..max_blocks * block", fn, max_len);
     if (n_seq > 65535 || n_tok > 0x7fffffffu || max_new > n_tok)
         return fail(YHIP_EINVAL, "%s: n_seq %u, n_tok %u, max_new %u out of range", fn, n_seq, n_tok, max_new);
+    if ((uint64_t)n_blocks * n_kv_heads > 0xffffffffull) return fail(YHIP_EINVAL, "%s: too many blocks", fn);
     const uint64_t row = (uint64_t)n_heads * head_dim;
     if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8)
         return fail(YHIP_EINVAL, "%s: q_stride/out_stride must be >= n_heads*head_dim and a multiple of 8", fn);
@@ -876,6 +877,11 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     if (rows_overlap(ro, rows_of(q, q_dtype, q_stride, row, n_tok)) ||
         (gate && rows_overlap(ro, rows_of(gate, YHIP_F32, gate_stride, row, n_tok))))
         return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
+    // tiles of 64 keys that the largest sequence's 128-row items walk
+    const uint64_t nb = (max_new + 127) / 128, tiles = max_len / 64 + 1, gmax = (n_heads + n_kv_heads - 1) / n_kv_heads;
+    if ((nb * (tiles + nb + 8) + tiles) * gmax * n_kv_heads >= 1ull << 31)
+        return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
+                    max_new, max_len);
     const size_t need = yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(YHIP_ENOSPC, "%s: %zu bytes of workspace (16-byte aligned) needed, %zu given", fn, need,

@@ -20,9 +20,14 @@
 namespace yhip {
 namespace {
 
-// Workgroup (j, y): rows 32 y .. of the split item that chunk j begins, if
-// any.  Pieces are joined in their order; a thread holds four dimensions of a
-// row, and a round's loads go out together.
+constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
+
+// Workgroup (j, y): the y-th kMergeRows * 256 / (D / 4) rows of the split item
+// that chunk j begins, if any.  Pieces are joined in their order; a thread
+// holds four dimensions of its rows.  Nearly all split items have two pieces:
+// their loads, and the gate's, go out together (one row after the other, 16
+// dependent round trips: a gated chunk of 2048 tokens, 16 / 2 heads of 256,
+// merged in 22 us; so, in 19, 6 TB/s).
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
 {
@@ -31,9 +36,45 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
     const uint32_t j = blockIdx.x;
     const PagedDesc d = reinterpret_cast<const PagedDesc*>(a.desc)[j];
     if (d.n == 0) return;
-    const uint32_t dim = threadIdx.x % C4 * 4u;
-    for (uint32_t r0 = blockIdx.y * 32u; r0 < blockIdx.y * 32u + 32u; r0 += RP) {
-        const uint32_t r = r0 + threadIdx.x / C4;
+    const uint32_t dim = threadIdx.x % C4 * 4u, r0 = blockIdx.y * (kMergeRows * RP) + threadIdx.x / C4;
+    auto finish = [&](const PagedRow& rw, f32x4 O, float L, const f32x4& g) {
+        f32x4 v = O * (L == 0.0f ? 0.0f : 1.0f / L);
+        if (a.gate) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= sigmoid_ref(g[e]);
+        }
+        store_out4(a.out, (size_t)rw.b * a.out_stride + (size_t)rw.h * D + dim, a.out_dtype, v);
+    };
+    auto gate_of = [&](const PagedRow& rw) {
+        typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // gate rows are float-aligned
+        return (f32x4)*reinterpret_cast<const f32x4u*>(a.gate + (size_t)rw.b * a.gate_stride + (size_t)rw.h * D + dim);
+    };
+    if (d.n == 2) {
+        PagedRow rw[kMergeRows];
+        f32x2 ml[kMergeRows][2];
+        f32x4 os[kMergeRows][2], g[kMergeRows];
+#pragma unroll
+        for (uint32_t i = 0; i < kMergeRows; ++i) {  // rows past the item's end read its last row's
+            rw[i] = paged_row(a, d, r0 + i * RP);
+            const uint32_t r = min(r0 + i * RP, kItemRows - 1);
+            const size_t p0 = (size_t)(2 * j + 1) * kItemRows + r, p1 = (size_t)(2 * j + 2) * kItemRows + r;
+            ml[i][0] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * p0);
+            ml[i][1] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * p1);
+            os[i][0] = *reinterpret_cast<const f32x4*>(a.part_o + p0 * D + dim);
+            os[i][1] = *reinterpret_cast<const f32x4*>(a.part_o + p1 * D + dim);
+            g[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (a.gate) g[i] = gate_of(rw[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kMergeRows; ++i) {
+            const float M = fmaxf(ml[i][0][0], ml[i][1][0]);
+            const float c0 = fast_exp2(ml[i][0][0] - M), c1 = fast_exp2(ml[i][1][0] - M);
+            if (rw[i].valid) finish(rw[i], os[i][0] * c0 + os[i][1] * c1, ml[i][0][1] * c0 + ml[i][1][1] * c1, g[i]);
+        }
+        return;
+    }
+    for (uint32_t i = 0; i < kMergeRows; ++i) {
+        const uint32_t r = r0 + i * RP;
         const PagedRow rw = paged_row(a, d, r);
         if (!rw.valid) return;
         float M = -1e30f, L = 0.0f;
@@ -42,36 +83,32 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
             f32x2 ml[kRound];
             f32x4 os[kRound];
 #pragma unroll
-            for (uint32_t i = 0; i < kRound; ++i) {
+            for (uint32_t k = 0; k < kRound; ++k) {
                 // piece s in slot 2 (j + s) + (s == 0); past the last one, the first again, counted as nothing
-                const uint32_t s = s0 + i < d.n ? s0 + i : 0u;
+                const uint32_t s = s0 + k < d.n ? s0 + k : 0u;
                 const size_t p = (size_t)(2 * (j + s) + (s == 0)) * kItemRows + r;
-                ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * p);
-                os[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + dim);
+                ml[k] = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * p);
+                os[k] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + dim);
             }
             float mr = M;
 #pragma unroll
-            for (uint32_t i = 0; i < kRound; ++i)
-                if (s0 + i < d.n) mr = fmaxf(mr, ml[i][0]);
+            for (uint32_t k = 0; k < kRound; ++k)
+                if (s0 + k < d.n) mr = fmaxf(mr, ml[k][0]);
             const float co = fast_exp2(M - mr);
             L *= co;
             O *= co;
 #pragma unroll
-            for (uint32_t i = 0; i < kRound; ++i) {
-                if (s0 + i >= d.n) continue;
-                const float c = fast_exp2(ml[i][0] - mr);
-                L += ml[i][1] * c;
-                O += os[i] * c;
+            for (uint32_t k = 0; k < kRound; ++k) {
+                if (s0 + k >= d.n) continue;
+                const float c = fast_exp2(ml[k][0] - mr);
+                L += ml[k][1] * c;
+                O += os[k] * c;
             }
             M = mr;
         }
-        f32x4 v = O * (L == 0.0f ? 0.0f : 1.0f / L);
-        if (a.gate) {
-            const float* gp = a.gate + (size_t)rw.b * a.gate_stride + (size_t)rw.h * D + dim;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= sigmoid_ref(gp[e]);
-        }
-        store_out4(a.out, (size_t)rw.b * a.out_stride + (size_t)rw.h * D + dim, a.out_dtype, v);
+        f32x4 g = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (a.gate) g = gate_of(rw);
+        finish(rw, O, L, g);
     }
 }
 
@@ -141,7 +178,8 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
     default: return hipErrorInvalidValue;
     }
     if ((a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
-        const dim3 grid(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + 31) / 32);
+        const uint32_t rp = kMergeRows * 1024u / a.D;  // rows of a merge workgroup
+        const dim3 grid(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
         switch (a.D) {
         case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, st, a); break;
         case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, st, a); break;

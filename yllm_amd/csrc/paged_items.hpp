@@ -53,19 +53,27 @@ __device__ inline PagedSeq paged_seq(const PagedAttnArgs& a, int c0, int c1, int
 
 __device__ inline uint32_t units_to(int keys) { return keys > 0 ? ((uint32_t)keys + kUnitKeys - 1) / kUnitKeys : 1u; }
 
+// An item costs its tiles and kItemUnits more (queries in, first tiles, output
+// out), which the line counts as units before its first tile: without them a
+// chunk of many short items ran far longer than one of a few long ones (a
+// prompt of 8192 tokens, 32 / 8 heads of 128: 733 us, 600 with them; 12 of
+// them are too many, 5 too few).
+constexpr uint32_t kItemUnits = 8;
+
 // Units of one query head's (or one packed group's) items, in order:
 // packed items all see every key; of plain ones, block b of 128 tokens sees
-// c + 2 (b + 1) units (c: those of the keys before the new tokens), the last
+// c + 2 (b + 1) tiles (c: those of the keys before the new tokens), the last
 // block all.  (Tokens at negative positions are counted as if at their index;
 // the walk leaves out what is not there.)
+__device__ inline uint32_t plain_c(const PagedSeq& s) { return ((uint32_t)max(s.pos0, 0) + kUnitKeys - 1) / kUnitKeys + kItemUnits; }
 __device__ inline uint32_t plain_before(uint32_t b, uint32_t c) { return b * c + b * (b + 1); }
-__device__ inline uint32_t plain_last(const PagedSeq& s) { return units_to(max(s.pos0, 0) + (int)s.nq); }
+__device__ inline uint32_t plain_last(const PagedSeq& s) { return units_to(max(s.pos0, 0) + (int)s.nq) + kItemUnits; }
 
 __device__ inline uint64_t seq_units(const PagedAttnArgs& a, const PagedSeq& s)
 {
     if (s.nq == 0) return 0;
-    if (s.nq < kItemRows) return (uint64_t)a.n_kv * ((a.gmax * s.nq + kItemRows - 1) / kItemRows) * units_to(s.L);
-    const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows, c = ((uint32_t)max(s.pos0, 0) + kUnitKeys - 1) / kUnitKeys;
+    if (s.nq < kItemRows) return (uint64_t)a.n_kv * ((a.gmax * s.nq + kItemRows - 1) / kItemRows) * (units_to(s.L) + kItemUnits);
+    const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows, c = plain_c(s);
     return (uint64_t)a.n_kv * a.gmax * (plain_before(nb - 1, c) + plain_last(s));
 }
 
@@ -84,17 +92,28 @@ struct PagedDesc {
     uint32_t row0, nq, kvh, h, qb, pack, pad;
 };
 
+// Where a workgroup is in its chunk of `len` units: `done` of them are behind
+// it (negative: units taken over from the chunk before), the next is unit `off`
+// of sequence seq.
 struct PagedCursor {
-    uint64_t u, end, first, base, units;  // next unit; chunk end and begin; the sequence's first unit and count
-    uint32_t seq, chunk, j, fresh;
-    PagedSeq s;
+    uint32_t seq, off, chunk, j;
+    int done, len;
+    bool fresh;
 };
 
-__device__ inline void cursor_seq(const PagedAttnArgs& a, PagedCursor& C)
+__device__ inline PagedSeq cursor_seq(const PagedAttnArgs& a, uint32_t seq)
 {
     const ConstInts cu = const_ints(a.cu_new);
-    C.s = paged_seq(a, cu[C.seq], cu[C.seq + 1], const_ints(a.kv_lens)[C.seq]);
-    C.units = seq_units(a, C.s);
+    return paged_seq(a, cu[seq], cu[seq + 1], const_ints(a.kv_lens)[seq]);
+}
+
+// The launch's arguments, read again: kept in scalar registers from one end of
+// an item to the other they displaced what the key loop needs.
+__device__ inline const PagedAttnArgs& fresh_args(const PagedAttnArgs&)
+{
+    auto p = (const PagedAttnArgs __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedAttnArgs*)p;
 }
 
 // This workgroup's place in the line; false if it has no chunk.  Active chunks
@@ -134,33 +153,32 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
                                           : ((uint32_t)total + C.chunk - 1) / C.chunk;
     const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
     C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
-    C.first = (uint64_t)C.j * C.chunk;
+    const uint64_t begin = (uint64_t)C.j * C.chunk;
     if (C.j >= active) return false;  // workgroup-uniform
-    C.u = C.first;
-    C.end = min(C.first + C.chunk, total);
-    C.fresh = 1;
-    const bool mine = before <= C.first && C.first < before + sum;
+    C.done = 0;
+    C.len = (int)min((uint64_t)C.chunk, total - begin);
+    C.fresh = true;
+    const bool mine = before <= begin && begin < before + sum;
     if (small) {
         const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(mine));
         C.seq = at;
-        C.base = uni64(__shfl((unsigned long long)before, (int)at));
+        C.off = (uint32_t)(begin - uni64(__shfl((unsigned long long)before, (int)at)));
     } else {
         if (mine) {
             uint32_t i = lo;
             for (;; ++i) {
                 const uint64_t n = seq_units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
-                if (C.first < before + n) break;
+                if (begin < before + n) break;
                 before += n;
             }
             scratch[16] = i;
-            scratch[17] = before;
+            scratch[17] = begin - before;
         }
         __syncthreads();
         C.seq = uni((uint32_t)scratch[16]);
-        C.base = uni64(scratch[17]);
+        C.off = uni((uint32_t)scratch[17]);
         __syncthreads();
     }
-    cursor_seq(a, C);
     return true;
 }
 
@@ -170,35 +188,29 @@ __device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedI
 {
     constexpr uint32_t TU = kUnitKeys / BN;  // tiles per unit
     for (;;) {
-        if (C.u >= C.end) return false;
-        while (C.u >= C.base + C.units) {
-            C.base += C.units;
-            ++C.seq;
-            cursor_seq(a, C);
+        if (C.done >= C.len) return false;
+        PagedSeq s = cursor_seq(a, C.seq);
+        uint32_t units = (uint32_t)seq_units(a, s);  // (below 2^31, checked on the host)
+        while (C.off >= units) {
+            C.off -= units;
+            s = cursor_seq(a, ++C.seq);
+            units = (uint32_t)seq_units(a, s);
         }
-        const PagedSeq& s = C.s;
-        uint64_t off = C.u - C.base;
-        const uint64_t per_kv = C.units / a.n_kv;
-        uint32_t kvh = 0;
-        while (off >= per_kv) {
-            off -= per_kv;
-            ++kvh;
-        }
-        uint32_t rem = (uint32_t)off, T, t;
+        const uint32_t per_kv = units / a.n_kv, kvh = C.off / per_kv;
+        uint32_t rem = C.off - kvh * per_kv, T, t;
         const uint32_t h0 = head0(a, kvh), h1 = head0(a, kvh + 1);
         I.pack = s.nq < kItemRows;
         bool none;  // an item of the fullest group that this one does not have
         int seen;
         if (I.pack) {
-            T = units_to(s.L);
+            T = units_to(s.L) + kItemUnits;
             I.qb = rem / T;
             t = rem - I.qb * T;
             I.h = h0;
             none = I.qb * kItemRows >= (h1 - h0) * s.nq;
             seen = s.L;
         } else {
-            const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows,
-                           c = ((uint32_t)max(s.pos0, 0) + kUnitKeys - 1) / kUnitKeys;
+            const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows, c = plain_c(s);
             // block b with plain_before(b) <= rem / gmax < plain_before(b + 1)
             const uint32_t want = rem / a.gmax;
             const float hc = 0.5f * (float)(c + 1u);
@@ -215,24 +227,30 @@ __device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedI
             none = I.h >= h1;
             seen = s.pos0 + (int)min(s.nq, (b + 1) * kItemRows);
         }
-        const uint64_t i0 = C.u - t, i1 = i0 + T;
-        if (C.fresh && t > 0 && T <= a.snap_units) {  // the chunk begins inside a short item: all of it
-            C.u = i0;
+        // cuts inside short items, and near an item's start, move to its start
+        auto at_start = [&](uint32_t cut) { return T <= a.snap_units + kItemUnits || cut <= kItemUnits + 1; };
+        if (C.fresh && t > 0 && at_start(t)) {
+            C.off -= t;
+            C.done -= (int)t;
             t = 0;
         }
-        C.fresh = 0;
+        C.fresh = false;
+        const int to_end = C.done + (int)(T - t);  // of the chunk, at the item's end
         uint32_t n = T - t;
-        if (C.end < i1) {  // it ends inside one
-            if (T <= a.snap_units) {
-                C.u = C.end;
+        if (to_end > C.len) {  // the chunk ends inside the item
+            n = (uint32_t)(C.len - C.done);
+            if (at_start(t + n)) {
+                C.done = C.len;
                 return false;
             }
-            n = (uint32_t)(C.end - C.u);
         }
-        C.u += n;
+        I.last = C.j + (uint32_t)(to_end - 1) / C.chunk;  // the chunk that ends the item
+        C.off += n;
+        C.done += (int)n;
         if (none) continue;
         I.part = n == T ? 0u : t == 0 ? 1u : 2u;
-        I.last = C.j + (uint32_t)(i1 - 1 - C.first) / C.chunk;  // the chunk that ends the item
+        const uint32_t tile0 = t ? t - kItemUnits : 0u;  // the piece's tiles of 64 keys
+        n -= t ? 0u : kItemUnits;
         I.seq = C.seq;
         I.row0 = s.row0;
         I.nq = s.nq;
@@ -240,7 +258,7 @@ __device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedI
         I.kvh = kvh;
         I.kmax = (uint32_t)max(seen - 1, 0);
         const uint32_t all = I.kmax / BN + 1;
-        I.t0 = t * TU;
+        I.t0 = tile0 * TU;
         I.idle = seen <= 0 || I.t0 >= all;
         if (I.idle) {
             I.t0 = all - 1;
@@ -272,8 +290,8 @@ template <int D>
 __device__ inline PagedTile paged_tile(const PagedAttnArgs& a, uint32_t page, uint32_t kvh)
 {
     const bool in = page < a.n_blocks;
-    const uint32_t head_bytes = (uint32_t)(D * 2) << a.shift;
-    return PagedTile{in ? ((uint64_t)page * a.n_kv + kvh) * head_bytes : 0u, in ? head_bytes : 0u};
+    const uint32_t lg = a.shift + (D == 64 ? 7 : D == 128 ? 8 : 9);  // (n_blocks * n_kv fits 32 bits, checked on the host)
+    return PagedTile{(uint64_t)(in ? page * a.n_kv + kvh : 0u) << lg, in ? 1u << lg : 0u};
 }
 __device__ inline uint32_t paged_page(const PagedAttnArgs& a, uint32_t seq, uint32_t key)
 {

@@ -144,6 +144,66 @@ __device__ inline int chunk_swz(int r)
     else return (((r >> 1) ^ (r >> 3)) & 1) | ((r >> 1) & 2);
 }
 
+// Values that a query does not see must not reach its output, whatever their
+// bits: a masked key's probability is 0, but 0 * inf and 0 * NaN are NaN.
+// Paged items look over the V tiles that their mask cuts (in LDS, before the
+// product) and clear inf and NaN there; an item in which some were found adds
+// them at its end, from the cache, to the rows that do see them.
+// clean_v: LDS chunk `ch`, keys 8 c .. of a tile with `valid` stored keys;
+// true if it held an inf or NaN and `cut`.
+__device__ inline bool clean_v(f16x8* ch, int c, uint32_t valid, bool cut)
+{
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 v = *reinterpret_cast<u16x8*>(ch);
+    const u16x8 b = v & (uint16_t)0x7fff;
+    uint16_t top = 0;  // nearly always, the chunk is finite and wanted
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, b[e]);
+    if (top < 0x7c00 && (uint32_t)(8 * c + 8) <= valid) return false;
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool special = b[e] >= 0x7c00, past = (uint32_t)(8 * c + e) >= valid;
+        odd = odd || (special && !past);
+        v[e] = (special && cut) || past ? 0 : v[e];
+    }
+    *reinterpret_cast<u16x8*>(ch) = v;
+    return odd && cut;
+}
+// Values for the product with the probabilities' lo parts: an inf or NaN as a
+// finite value.  The hi parts bring it in; with a lo part, 0 or negative
+// beside a positive hi, the same inf would make NaN.
+__device__ inline f16x8 bounded(const f16x8& v)
+{
+    const f16x8 top = {65504, 65504, 65504, 65504, 65504, 65504, 65504, 65504};
+    return __builtin_elementwise_max(__builtin_elementwise_min(v, top), -top);
+}
+// The sum of the infs and NaNs among the values of dimension d that a query at
+// position pos sees of keys lo .. hi of the item.
+template <int D>
+__device__ float special_sum(const PagedAttnArgs& a, const PagedItem& I, uint32_t d, int pos, uint32_t lo, uint32_t hi)
+{
+    float s = 0.0f;
+#pragma unroll 1
+    for (uint32_t k = lo; k <= hi && (int)k <= pos; ++k) {
+        const PagedTile t = paged_tile<D>(a, (uint32_t)a.table[(size_t)I.seq * a.table_stride + (k >> a.shift)], I.kvh);
+        if (t.bytes == 0) continue;
+        const uint32_t off = k & ((1u << a.shift) - 1u);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc) + t.at);
+        const uint16_t b = p[(size_t)(off & ~31u) * D + d * kVTile + (off & 31u)];
+        if ((b & 0x7fff) >= 0x7c00) s += f16_bits_to_f32(b);
+    }
+    return s;
+}
+// the first tile of BN keys that an item's mask cuts; ~0 if its piece has none
+template <int BN>
+__device__ inline uint32_t cut_from(const PagedItem& I)
+{
+    const int first = I.pos0 + (I.pack ? 0 : (int)(I.qb * BM));  // its first query's position
+    const uint32_t t = max(I.t0, (uint32_t)max(first + 1, 0) / BN);
+    return I.idle || (int)I.kmax <= first || t >= I.t0 + I.nt ? ~0u : t;
+}
+
 // Schedule of one key step's MFMAs: NQ score MFMAs of the next tile and NPV
 // P.V MFMAs of this tile (k-slot kc = n / NDB of NKC uses the probabilities
 // 8 kc .. 8 kc + 7), with the tile's 8 NKC probabilities spread over them.
@@ -187,6 +247,9 @@ struct FusedSchedule {
 // first query head of kv head g: heads h with h*n_kv/n_heads == g are
 // [head0(g), head0(g+1)) (engine.c:537)
 __device__ inline uint32_t head0(const PrefillArgs& a, uint32_t g) { return (g * a.n_heads + a.n_kv - 1) / a.n_kv; }
+
+// (paged launches read their arguments again, paged_items.hpp)
+__device__ inline const PrefillArgs& fresh_args(const PrefillArgs& a) { return a; }
 
 // A work item: query block qb (plain rows) or row block qb (packed rows) of
 // kv head kvh, key split `split`; h is the query head of plain rows.
@@ -370,7 +433,7 @@ __device__ inline bool split_item(const PrefillArgs& a, PItem& I)
 // plain mode walks items.  fp32 queries then also take their probabilities as
 // f16 hi + lo parts (PS), so that the output keeps fp32-level error.
 template <int D, int NG, bool SPLIT, bool QS = false, class A = PrefillArgs>
-__global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 && !QS) ? 2 : 1) void prefill_kernel(A a)
+__global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 && !QS) ? 2 : 1) void prefill_kernel(A args)
 {
     constexpr bool PAGED = std::is_same<A, PagedAttnArgs>::value;
     constexpr bool PS = PAGED && QS;
@@ -432,7 +495,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // [parity][wave][float4 j][lane] (consecutive lanes, consecutive 16
     // bytes).  Two key groups: (max, sum) of group 1's queries for the merge.
     // (One array: pair mode fills the 160 KB of LDS exactly.)
-    __shared__ f32x4 Xl[PAIR ? 2 * 8 * 4 * NS * 64 : NG > 1 && !QL ? 128 : 1];
+    __shared__ f32x4 Xl[PAIR ? 2 * 8 * 4 * NS * 64 : NG > 1 && !QL ? 128 : 1];  // (paged: one flag a wave, at least)
     // [query wave][k-chunk][lane]; between items it holds (max, sum) for the merge
     __shared__ f16x8 Qlo[QL ? 4 : 1][QL ? NKK : 1][QL ? 64 : 1];
     float* const s_ml = QL ? reinterpret_cast<float*>(&Qlo[0][0][0]) : reinterpret_cast<float*>(&Xl[0]);
@@ -445,6 +508,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // item `it` of this workgroup (paged: the next one); false past the last
     PagedCursor C;
     auto item_of = [&](uint32_t it, Item& I) -> bool {
+        const A& a = fresh_args(args);
         if constexpr (PAGED) return paged_next<BN>(a, C, I);
         else if constexpr (SPLIT) return it == 0 && split_item(a, I);  // one item per workgroup
         else return plain_item(a, (a.B + BM - 1) / BM, it, I);
@@ -459,19 +523,20 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // stores.  With a gate the epilogue loads the gate values, which would
     // then wait behind these loads; such items issue their loads at their
     // own start.
-    const bool early = a.gate == nullptr && !PAIR;
+    const bool early = args.gate == nullptr && !PAIR;
     Item cur;
     if constexpr (PAGED) {
-        const bool any = paged_start<256 * NG * (PAIR ? 2 : 1)>(a, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C) &&
+        const bool any = paged_start<256 * NG * (PAIR ? 2 : 1)>(fresh_args(args), reinterpret_cast<uint64_t*>(&Kl0[0][0]), C) &&
                          item_of(0, cur);
         if (!any) {
-            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(a.desc)[C.j].n = 0;
+            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
             return;
         }
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
     for (uint32_t it = 0;; ++it) {
+        const A& a = fresh_args(args);
         // Thread indices pass through an opaque move each item so that nothing
         // derived from them is hoisted out of the item loop: the key loop's
         // register budget stays that of a single item.
@@ -488,8 +553,10 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // the wave's 32 queries (qw) and, in pair mode, its half of the dimensions (hf)
         const int qw = PAIR ? wave >> 1 : wave, hf = PAIR ? wave & 1 : 0;
         const int r32 = lane & 31, hh = lane >> 5;
+        // (paged: formed at the group's last step or after the loop)
         Item nxt{};
-        const bool has_next = item_of(it + 1, nxt);
+        bool has_next = false;
+        if constexpr (!PAGED) has_next = item_of(it + 1, nxt);
 
         // Chunk L = LT i + gtid of a tile is the 16 bytes this thread loads
         // with its i-th instruction.  K: LDS row R = L / KCH holds key row
@@ -533,9 +600,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if constexpr (PAGED) return paged_page(a, I.seq, min(kt, I.t0 + I.nt - 1) * BN);
             else return 0;
         };
-        auto dma_page_k = [&](uint32_t kv, uint32_t page, int par, uint32_t kt) {
+        auto dma_page_k = [&](const PagedTile& p, int par, uint32_t kt) {
             if constexpr (PAGED) {
-                const PagedTile p = paged_tile<D>(a, page, kv);
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.kc)) + p.at, 0, p.bytes, 0x00020000);
                 const uint32_t at = ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
@@ -543,9 +609,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], at);
             }
         };
-        auto dma_page_v = [&](uint32_t kv, uint32_t page, int par, uint32_t kt) {
+        auto dma_page_v = [&](const PagedTile& p, int par, uint32_t kt) {
             if constexpr (PAGED) {
-                const PagedTile p = paged_tile<D>(a, page, kv);
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.vc)) + p.at, 0, p.bytes, 0x00020000);
                 const uint32_t at = ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
@@ -555,14 +620,14 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         };
         // tile kt of a K (V) resource into K (V) buffer par
         auto dma_k_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) dma_page_k(r, page_of(I, kt), par, kt);
+            if constexpr (PAGED) dma_page_k(paged_tile<D>(a, page_of(I, kt), r), par, kt);
             else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], kt * BN * D * 2);
             }
         };
         auto dma_v_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) dma_page_v(r, page_of(I, kt), par, kt);
+            if constexpr (PAGED) dma_page_v(paged_tile<D>(a, page_of(I, kt), r), par, kt);
             else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, vbuf(par) + (LT * i + 64 * wave) * 8, vgo[i], kt * BN * D * 2);
@@ -589,10 +654,11 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 item_keys<BN, SPLIT>(a, I, km, t0, nt);
             }
         };
-        auto row_in = [&](const Item& I, uint32_t r) {
-            if constexpr (PAGED) return paged_row(a, I, r);
-            else return row_of<SPLIT>(a, I, r);
+        auto row_from = [&](const A& x, const Item& I, uint32_t r) {
+            if constexpr (PAGED) return paged_row(x, I, r);
+            else return row_of<SPLIT>(x, I, r);
         };
+        auto row_in = [&](const Item& I, uint32_t r) { return row_from(a, I, r); };
         auto item_steps = [&](const Item& I, uint32_t& t0) {
             uint32_t km, nt;
             keys_of(I, km, t0, nt);
@@ -666,14 +732,18 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         auto tile_of = [&](uint32_t st) { return t0 + (uint32_t)grp + NG * st; };
 
         const auto rK = rsrc_k(kvh), rV = rsrc_v(kvh);
-        // paged: the pages of the tiles whose K and V the coming step loads
-        uint32_t page_k = page_of(cur, tile_of(NB)), page_v = page_of(cur, tile_of(NB - 1));
+        // paged: where the tiles are whose K and V the coming step loads
+        PagedTile at_k{}, at_v{};
+        if constexpr (PAGED) {
+            at_k = paged_tile<D>(a, page_of(cur, tile_of(NB)), kvh);
+            at_v = paged_tile<D>(a, page_of(cur, tile_of(NB - 1)), kvh);
+        }
         auto dma_k = [&](int par, uint32_t st) {
-            if constexpr (PAGED) dma_page_k(rK, page_k, par, tile_of(st));
+            if constexpr (PAGED) dma_page_k(at_k, par, tile_of(st));
             else dma_k_of(cur, rK, par, tile_of(st));
         };
         auto dma_v = [&](int par, uint32_t st) {
-            if constexpr (PAGED) dma_page_v(rV, page_v, par, tile_of(st));
+            if constexpr (PAGED) dma_page_v(at_v, par, tile_of(st));
             else dma_v_of(cur, rV, par, tile_of(st));
         };
 
@@ -801,7 +871,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             for (int n = 0; n < NM; ++n) {
                 if (n + 2 < NM) vf[(n + 2) % 3] = read_v(par, (n + 2) % NDB, (n + 2) / NDB);
                 o[n % NDB] = mfma32(vf[n % 3], pf[n / NDB], o[n % NDB]);
-                if constexpr (PS) o[n % NDB] = mfma32(vf[n % 3], pl[n / NDB], o[n % NDB]);
+                if constexpr (PS) o[n % NDB] = mfma32(bounded(vf[n % 3]), pl[n / NDB], o[n % NDB]);
             }
         };
         // Scores of the next tile (K buffer kpar) into Snext and P.V of this tile
@@ -826,7 +896,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 if (sch.s[t].pv) {
                     if (n + 2 < NPV) vf[(n + 2) % 3] = read_v(vpar, (n + 2) % NDB, (n + 2) / NDB);
                     o[n % NDB] = mfma32(vf[n % 3], pf[n / NDB], o[n % NDB]);
-                    if constexpr (PS) o[n % NDB] = mfma32(vf[n % 3], pl[n / NDB], o[n % NDB]);
+                    if constexpr (PS) o[n % NDB] = mfma32(bounded(vf[n % 3]), pl[n / NDB], o[n % NDB]);
                 } else {
                     if (n + KR - 1 < NQ) kf[(n + KR - 1) % KR] = read_k(kpar, (n + KR - 1) % NS, (n + KR - 1) / NS);
                     if constexpr (QL)
@@ -905,10 +975,24 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // with a successor may still need the mask.
         // the step that reads the tile holding kmax (the item's last tile, unless
         // a later split owns it), in this group's buffers
+        // paged: the first tile cut by the item's mask (~0: none), and whether this
+        // thread found an inf or NaN in such tiles
+        uint32_t cut_tile = ~0u;
+        bool odd_v = false;
+        if constexpr (PAGED) cut_tile = cut_from<BN>(cur);
+        auto clean_tile = [&](int par, uint32_t st) {
+            const uint32_t kt = tile_of(st), valid = kmax - kt * BN + 1;
+            if (st >= gsteps || !(kt >= cut_tile || valid < BN)) return;  // uniform over the group
+            for (int idx = gtid; idx < D * VCH; idx += LT) {
+                const int d = idx / VCH, c = idx % VCH;
+                odd_v |= clean_v(reinterpret_cast<f16x8*>(vbuf(par) + d * BN + ((c ^ chunk_swz<VCH>(d)) << 3)), c, valid,
+                                 kt >= cut_tile);
+            }
+        };
         const bool has_tail = ntiles > 0 && t0 + ntiles == kmax / BN + 1 && (kmax + 1) % BN != 0;
         const uint32_t tail_step = (ntiles - 1) / NG;
         const int tail_grp = (int)((ntiles - 1) % NG);
-        const bool prefetch = has_next && early;
+        bool prefetch = has_next && early;
         // the group's last step (or, for a group without tiles, the first) issues
         // the next item's loads
         const uint32_t last_st = gsteps > 0 ? gsteps - 1 : 0;
@@ -916,16 +1000,21 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             const bool lk = st + NB < gsteps, lv = st + NB - 1 < gsteps;
             if (lk) dma_k(ph, st + NB);
             if (lv) dma_v((ph + NB - 1) % NB, st + NB - 1);
-            if constexpr (PAGED) {
-                page_v = page_k;
-                page_k = page_of(cur, tile_of(st + NB + 1));
-            }
+            uint32_t page = 0;  // of the tile after those: read here, used at the step's end
+            if constexpr (PAGED) page = page_of(cur, tile_of(st + NB + 1));
+            if (PAGED && early && st == last_st) prefetch = has_next = item_of(it + 1, nxt);
             if (prefetch && st == last_st) {
                 // K buffers are free (no scores follow), V buffer 1-p too
                 issue_item_k(nxt);
                 if (ph == 1 || gsteps == 0) issue_item_v(nxt);
             }
-            if (has_tail && st == tail_step) {  // workgroup-uniform
+            if constexpr (PAGED) {
+                // workgroup-uniform: some group's tile is cut, or the last one
+                if ((has_tail && st == tail_step) || t0 + NG * st + NG - 1 >= cut_tile) {
+                    clean_tile(ph, st);
+                    lds_barrier();
+                }
+            } else if (has_tail && st == tail_step) {  // workgroup-uniform
                 if (grp == tail_grp) zero_v_tail(ph, st);
                 lds_barrier();
             }
@@ -942,6 +1031,10 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 f16x8 pf[NKC], pl[PS ? NKC : 1];
                 probs(Scur, pf, pl);
                 pv(pf, pl, ph);
+            }
+            if constexpr (PAGED) {
+                at_v = at_k;
+                at_k = paged_tile<D>(a, page, kvh);
             }
             if constexpr (NB > 2) {
                 // the previous steps' loads (this step's have two steps to land)
@@ -975,6 +1068,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             }
         }
 
+        if (PAGED && !early) has_next = item_of(it + 1, nxt);
         // the next item's first V tile when the last step still read V buffer 0,
         // and its queries
         if (prefetch) {
@@ -989,11 +1083,24 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         }
         // Thread indices for the epilogue from a fresh opaque read, so that the
         // ones of the item's start need not stay live through the key loop.
+        const A& a_e = fresh_args(args);
         int tid_e;
         asm volatile("v_mov_b32 %0, %1" : "=v"(tid_e) : "v"((int)threadIdx.x));
         const int gtid_e = NG > 1 ? tid_e % LT : tid_e, lane_e = tid_e & 63;
         const int qw_e = PAIR ? gtid_e >> 7 : gtid_e >> 6, hf_e = PAIR ? (gtid_e >> 6) & 1 : 0;
         int b_lo = 0, b_hi = NDB;  // the O blocks this thread stores
+        bool add_odd = false;      // paged: add the infs and NaNs cleared above
+        if constexpr (PAGED) {
+            if (cut_tile != ~0u) {  // workgroup-uniform; Xl (with QL the part of Qlo behind (max, sum)) is free between key loops
+                uint32_t* flags = reinterpret_cast<uint32_t*>(QL ? s_ml + 512 : s_ml + (NG > 1 ? 512 : 0));
+                const bool mine = __ballot(odd_v) != 0;
+                if (lane_e == 0) flags[tid_e >> 6] = mine;
+                lds_barrier();
+                for (int w = 0; w < LT * NG / 64; ++w) add_odd = add_odd || flags[w] != 0;
+                if (NG == 1) lds_barrier();  // read before the next item's step writes there
+            }
+        }
+        int pos_e = 0;
         if constexpr (NG > 1) {
             // The two groups' (m, l, O) meet through LDS: m, l in s_ml and O
             // through V buffer 1 of both groups (the one buffer the next item's
@@ -1049,22 +1156,39 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             b_lo = grp * HB;
             b_hi = b_lo + HB;
         }
-        const auto rw = row_in(cur, qw_e * 32 + (lane_e & 31));
+        const auto rw = row_from(a_e, cur, qw_e * 32 + (lane_e & 31));
+        if constexpr (PAGED) pos_e = cur.pos0 + (int)rw.t;
+        // four of the row's output values (unnormalised ones in a piece)
+        auto with_odd = [&](f32x4 v, uint32_t d) {
+            if constexpr (PAGED) {
+                if (add_odd)
+#pragma unroll 1
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = special_sum<D>(a_e, cur, d + e, pos_e, cut_tile * BN,
+                                                         min(cur.kmax, (cur.t0 + cur.nt) * BN - 1));
+                        v[0] += e == 0 ? x : 0.0f;
+                        v[1] += e == 1 ? x : 0.0f;
+                        v[2] += e == 2 ? x : 0.0f;
+                        v[3] += e == 3 ? x : 0.0f;
+                    }
+            }
+            return v;
+        };
         bool partial;
         if constexpr (PAGED) partial = cur.part != 0;
-        else partial = SPLIT && a.n_split > 1;
+        else partial = SPLIT && a_e.n_split > 1;
         if (rw.valid) {
             if (partial) {
                 // split partials: (max, sum) and the unnormalised O of this
                 // row over this split's keys
                 size_t pr;
                 if constexpr (PAGED) pr = (size_t)(2 * C.j + (cur.part & 1)) * BM + qw_e * 32 + (lane_e & 31);
-                else pr = ((size_t)cur.split * a.n_heads + rw.h) * a.B + rw.b;
+                else pr = ((size_t)cur.split * a_e.n_heads + rw.h) * a_e.B + rw.b;
                 // (one key group's sum: the groups round l differently, and two
                 // stores to one slot in no order would leave either)
                 if ((lane_e >> 5) == 0 && hf_e == 0 && grp == 0) {
                     typedef float f32x2 __attribute__((ext_vector_type(2)));
-                    *reinterpret_cast<f32x2*>(a.part_ml + 2 * pr) = f32x2{m, l};
+                    *reinterpret_cast<f32x2*>(a_e.part_ml + 2 * pr) = f32x2{m, l};
                 }
 #pragma unroll
                 for (int b = 0; b < NDB; ++b) {
@@ -1075,7 +1199,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                         f32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = o[b][4 * i4 + e];
-                        *reinterpret_cast<f32x4*>(a.part_o + pr * D + d) = v;
+                        *reinterpret_cast<f32x4*>(a_e.part_o + pr * D + d) = with_odd(v, d);
                     }
                 }
             } else {
@@ -1090,12 +1214,13 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                         f32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = o[b][4 * i4 + e] * inv;
-                        if (a.gate) {
-                            const float* gp = a.gate + (size_t)rw.b * a.gate_stride + (size_t)rw.h * D + d;
+                        v = with_odd(v, d);
+                        if (a_e.gate) {
+                            const float* gp = a_e.gate + (size_t)rw.b * a_e.gate_stride + (size_t)rw.h * D + d;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) v[e] *= sigmoid_ref(gp[e]);
                         }
-                        store_out4(a.out, (size_t)rw.b * a.out_stride + (size_t)rw.h * D + d, a.out_dtype, v);
+                        store_out4(a_e.out, (size_t)rw.b * a_e.out_stride + (size_t)rw.h * D + d, a_e.out_dtype, v);
                     }
                 }
             }
@@ -1103,7 +1228,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         if (!has_next) break;
         cur = nxt;
     }  // items
-    if constexpr (PAGED) paged_leave(a, C, cur);
+    if constexpr (PAGED) paged_leave(args, C, cur);
 }
 
 // head_dim 256, 16-bit queries.  Bound by the LDS: 128 bytes per
@@ -1133,7 +1258,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
 // previous item's last step.
 // A = PagedAttnArgs: paged items, as in prefill_kernel.
 template <int D, bool SPLIT, class A = PrefillArgs>
-__global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
+__global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
 {
     static_assert(D == 256, "two waves of 128 output dimensions");
     constexpr bool PAGED = std::is_same<A, PagedAttnArgs>::value;
@@ -1147,30 +1272,34 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
     __shared__ __attribute__((aligned(16))) _Float16 Kl0[BN * D], Kl1[BN * D], Vl0[D * BN], Vl1[D * BN];
     __shared__ f16x8 Pl[8][2][64];  // each wave's probabilities: k-slot, lane
     __shared__ float Ml[8][64];     // each wave's tile maxima, then its row sums
+    __shared__ uint32_t odd_flags[PAGED ? 8 : 1];
 
     PagedCursor C;
     auto item_of = [&](uint32_t it, Item& I) -> bool {
+        const A& a = fresh_args(args);
         if constexpr (PAGED) return paged_next<BN>(a, C, I);
         else if constexpr (SPLIT) return it == 0 && split_item(a, I);
         else return plain_item(a, (a.B + BM - 1) / BM, it, I);
     };
     Item cur;
     if constexpr (PAGED) {
-        if (!(paged_start<512>(a, reinterpret_cast<uint64_t*>(&Kl0[0]), C) && item_of(0, cur))) {
-            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(a.desc)[C.j].n = 0;
+        if (!(paged_start<512>(fresh_args(args), reinterpret_cast<uint64_t*>(&Kl0[0]), C) && item_of(0, cur))) {
+            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
             return;
         }
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
     for (uint32_t it = 0;; ++it) {
+        const A& a = fresh_args(args);
         int tid;  // opaque per item, as in prefill_kernel
         asm volatile("v_mov_b32 %0, %1" : "=v"(tid) : "v"((int)threadIdx.x));
         const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int qw = wave >> 1, hf = wave & 1;
         const int r32 = lane & 31, hh = lane >> 5;
-        Item nxt{};
-        const bool has_next = !SPLIT && item_of(it + 1, nxt);
+        Item nxt{};  // (paged: formed in the last step)
+        bool has_next = false;
+        if constexpr (!PAGED) has_next = !SPLIT && item_of(it + 1, nxt);
 
         auto kbuf = [&](int par) { return par == 0 ? &Kl0[0] : &Kl1[0]; };
         auto vbuf = [&](int par) { return par == 0 ? &Vl0[0] : &Vl1[0]; };
@@ -1186,9 +1315,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
             if constexpr (PAGED) return paged_page(a, I.seq, p0 + min(kt, I.nt - 1) * BN);
             else return 0;
         };
-        auto rsrc_at = [&](const uint16_t* pool, uint32_t kv, uint32_t p0, uint32_t page) {
+        auto rsrc_at = [&](const uint16_t* pool, uint32_t kv, uint32_t p0, const PagedTile& p) {
             if constexpr (PAGED) {
-                const PagedTile p = paged_tile<D>(a, page, kv);
                 return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(const_cast<uint16_t*>(pool)) + p.at, 0,
                                                          p.bytes, 0x00020000);
             } else {  // (V tiles of 32 positions take the bytes of 32 K rows)
@@ -1200,15 +1328,19 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
             if constexpr (PAGED) return ((p0 + kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
             else return kt * BN * D * 2;
         };
-        auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, uint32_t page) {
-            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.kc, kv, p0, page);
+        auto place = [&](const Item& I, uint32_t p0, uint32_t kt) {  // of tile kt
+            if constexpr (PAGED) return paged_tile<D>(a, page_of(I, p0, kt), I.kvh);
+            else return PagedTile{};
+        };
+        auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
+            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.kc, kv, p0, p);
             const uint32_t at = tile_at(p0, kt);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
                 lds_load16(r, kbuf(par) + (512 * i + 64 * wave) * 8, kgo, at + i * (16 * D * 2));
         };
-        auto dma_v = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, uint32_t page) {
-            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.vc, kv, p0, page);
+        auto dma_v = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
+            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.vc, kv, p0, p);
             const uint32_t at = tile_at(p0, kt);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
@@ -1232,21 +1364,22 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
                 return max(min(all - min(all, I.split * per), per), 1u);
             }
         };
-        auto row_in = [&](const Item& I, uint32_t r) {
-            if constexpr (PAGED) return paged_row(a, I, r);
-            else return row_of<SPLIT>(a, I, r);
+        auto row_from = [&](const A& x, const Item& I, uint32_t r) {
+            if constexpr (PAGED) return paged_row(x, I, r);
+            else return row_of<SPLIT>(x, I, r);
         };
+        auto row_in = [&](const Item& I, uint32_t r) { return row_from(a, I, r); };
         // the item's first K tiles; those of V follow into buffer 0
         auto issue_k = [&](const Item& I) {
             uint32_t km, p0;
             const uint32_t n = tiles_of(I, km, p0);
-            dma_k(I.kvh, p0, 0, 0, page_of(I, p0, 0));
-            if (n > 1) dma_k(I.kvh, p0, 1, 1, page_of(I, p0, 1));
+            dma_k(I.kvh, p0, 0, 0, place(I, p0, 0));
+            if (n > 1) dma_k(I.kvh, p0, 1, 1, place(I, p0, 1));
         };
         auto issue_v = [&](const Item& I) {
             uint32_t km, p0;
             tiles_of(I, km, p0);
-            dma_v(I.kvh, p0, 0, 0, page_of(I, p0, 0));
+            dma_v(I.kvh, p0, 0, 0, place(I, p0, 0));
         };
         const uint32_t kvh = cur.kvh;
         uint32_t kmax, p0;
@@ -1324,9 +1457,9 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
 
         // In a pair's last tile the upper 32 keys can lie past all its queries: their P is 0 but their V need not be
         // finite (an inf of a later key would reach these rows as NaN), so their products read the lower keys' V.
-        // Leaves vo like that: nothing follows that tile.
+        // Leaves vo like that: nothing follows that tile.  (Paged tiles are cleaned of what is not seen instead.)
         auto upper_v = [&](uint32_t st) {
-            if ((int)(st * BN) + 32 <= wpos_last) return;  // uniform over the wave
+            if (PAGED || (int)(st * BN) + 32 <= wpos_last) return;  // uniform over the wave
 #pragma unroll
             for (int s = 0; s < 2; ++s) vo[0][s] = vo[1][s] = hf ? vo[1][s] : vo[0][s];
         };
@@ -1374,6 +1507,25 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
             }
         };
 
+        // paged: the tiles cut by the item's mask (clean_v)
+        uint32_t cut_tile = ~0u;
+        bool odd_v = false;
+        if constexpr (PAGED) {
+            const uint32_t t = cut_from<BN>(cur);
+            if (t != ~0u) cut_tile = t - cur.t0;  // counted from p0
+        }
+        // whether tile st is cut by the mask or the last one's end (workgroup-uniform); then it is cleaned
+        auto clean_tile = [&](int par, uint32_t st) {
+            const uint32_t valid = kmax - p0 - st * BN + 1;
+            const bool cut = st >= cut_tile;
+            if (!cut && valid >= BN) return;
+            for (int idx = tid; idx < D * VCH; idx += 512) {
+                const int d = idx / VCH, c = idx % VCH;
+                odd_v |= clean_v(reinterpret_cast<f16x8*>(vbuf(par) + (d * BN + ((c ^ chunk_swz<VCH>(d)) << 3))), c, valid, cut);
+            }
+            lds_barrier();
+        };
+
         // prologue: the item's first loads are in flight
         dma_done();
         if (a.q_dtype == kBF16) {
@@ -1391,20 +1543,18 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
 
         // step st < ntiles - 1 (ph = st % 2): K(st + 2) replaces K(st), read by the previous step's scores, and
         // V(st + 1) V(st - 1)
-        uint32_t page_k = page_of(cur, p0, 2), page_v = page_of(cur, p0, 1);  // of the coming step's loads
+        PagedTile at_k = place(cur, p0, 2), at_v = place(cur, p0, 1);  // of the coming step's loads
         auto step = [&](int ph, uint32_t st, f32x16& Scur, f32x16& Snext) {
-            if (st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, page_k);
-            dma_v(kvh, p0, ph ^ 1, st + 1, page_v);
-            if constexpr (PAGED) {
-                page_v = page_k;
-                page_k = page_of(cur, p0, st + 3);
-            }
+            if (st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, at_k);
+            dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
+            const uint32_t page = page_of(cur, p0, st + 3);  // (read here, used at the step's end)
             // opaque each step, or the compiler keeps a second set of offsets for the other buffers (and spills)
 #pragma unroll
             for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(ko[j]));
 #pragma unroll
             for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(vo[j >> 1][j & 1]));
             upper_v(st);
+            if constexpr (PAGED) clean_tile(ph, st);
             f16x8 pf[2];
             if (st < wsteps) {
                 const float other = Ml[wave ^ 1][lane];
@@ -1437,17 +1587,24 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
                 pv(po, ph, 1);
                 tile_max(Snext, st + 1);
             }
+            if constexpr (PAGED) {
+                at_v = at_k;
+                at_k = paged_tile<D>(a, page, kvh);
+            }
             dma_done();
             lds_barrier();
         };
         // the item's last tile: no scores follow, so both K buffers are free and the next item's first loads go out
         auto last = [&](int ph, uint32_t st, f32x16& Scur) {
+            if constexpr (PAGED) has_next = item_of(it + 1, nxt);
             if (has_next) {
                 issue_k(nxt);
                 if (ph == 1) issue_v(nxt);
             }
             upper_v(st);
-            if (p0 / BN + ntiles == kmax / BN + 1 && (kmax + 1) % BN != 0) {  // uniform
+            if constexpr (PAGED) {
+                clean_tile(ph, st);
+            } else if (p0 / BN + ntiles == kmax / BN + 1 && (kmax + 1) % BN != 0) {  // uniform
                 zero_v_tail(ph);
                 lds_barrier();
             }
@@ -1493,36 +1650,37 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
         // each wave turns its 32 x 32 blocks of O over in 4 KB of it and then handles 8 rows of 32 dimensions per
         // instruction.  The gate's loads go out first.
         {
+            const A& a_e = fresh_args(args);
             int le;  // the lane afresh, so that nothing of this is kept through the key loop
             asm volatile("v_mov_b32 %0, %1" : "=v"(le) : "v"((int)threadIdx.x & 63));
             const int er = le >> 3, ec = le & 7;  // row within a group of 8, four dimensions
             const uint32_t col = hf * DH + 4 * ec;
             bool partial;
             if constexpr (PAGED) partial = cur.part != 0;
-            else partial = SPLIT && a.n_split > 1;
+            else partial = SPLIT && a_e.n_split > 1;
             // a partial result's row (of rw): its (max, sum), and D floats of O
             auto part_row = [&](const auto& rw, uint32_t r) -> size_t {
                 if constexpr (PAGED) return (size_t)(2 * C.j + (cur.part & 1)) * BM + r;
-                else return ((size_t)cur.split * a.n_heads + rw.h) * a.B + rw.b;
+                else return ((size_t)cur.split * a_e.n_heads + rw.h) * a_e.B + rw.b;
             };
-            const bool gated = a.gate && !partial;
+            const bool gated = a_e.gate && !partial;
             // rows 8 u + er: the first element written (and of the gate), and whether the row exists
             size_t at[4], gat[4];
             bool valid[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const auto rw = row_in(cur, qw * 32 + 8 * u + er);
+                const auto rw = row_from(a_e, cur, qw * 32 + 8 * u + er);
                 valid[u] = rw.valid;
                 at[u] = partial ? part_row(rw, qw * 32 + 8 * u + er) * D + col
-                                : (size_t)rw.b * a.out_stride + (size_t)rw.h * D + col;
-                gat[u] = (size_t)rw.b * a.gate_stride + (size_t)rw.h * D + col;
+                                : (size_t)rw.b * a_e.out_stride + (size_t)rw.h * D + col;
+                gat[u] = (size_t)rw.b * a_e.gate_stride + (size_t)rw.h * D + col;
             }
             f32x4 gt[2][4];
             auto load_gate = [&](int b) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // gate rows are float-aligned
-                    gt[b & 1][u] = *reinterpret_cast<const f32x4u*>(a.gate + gat[u] + 32 * b);
+                    gt[b & 1][u] = *reinterpret_cast<const f32x4u*>(a_e.gate + gat[u] + 32 * b);
                 }
             };
             if (gated) load_gate(0);
@@ -1531,10 +1689,20 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
             float inv = PAGED && l == 0.0f ? 0.0f : 1.0f / l;
             if (partial) {  // (max, sum) and the unnormalised O of the row over this split's keys
                 inv = 1.0f;
-                const auto rw = row_in(cur, qw * 32 + (le & 31));
+                const auto rw = row_from(a_e, cur, qw * 32 + (le & 31));
                 if (rw.valid && le < 32 && hf == 0) {
                     typedef float f32x2 __attribute__((ext_vector_type(2)));
-                    *reinterpret_cast<f32x2*>(a.part_ml + 2 * part_row(rw, qw * 32 + (le & 31))) = f32x2{m, l};
+                    *reinterpret_cast<f32x2*>(a_e.part_ml + 2 * part_row(rw, qw * 32 + (le & 31))) = f32x2{m, l};
+                }
+            }
+            bool add_odd = false;  // paged: add the infs and NaNs cleared from cut tiles
+            if constexpr (PAGED) {
+                if (cut_tile != ~0u) {  // workgroup-uniform
+                    const bool mine = __ballot(odd_v) != 0;
+                    if (le == 0) odd_flags[wave] = mine;
+                    lds_barrier();
+                    for (int w = 0; w < 8; ++w) add_odd = add_odd || odd_flags[w] != 0;
+                    lds_barrier();  // read before another item writes there
                 }
             }
             f32x4* area = reinterpret_cast<f32x4*>(&Vl1[0]) + wave * 256;  // [32 rows][8 chunks], swizzled
@@ -1552,13 +1720,27 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     f32x4 v = area[(8 * u + er) * 8 + (ec ^ er)];
+                    if constexpr (PAGED) {
+                        if (add_odd) {
+                            const int pos = cur.pos0 + (int)row_from(a_e, cur, qw * 32 + 8 * u + er).t;
+#pragma unroll 1
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = special_sum<D>(a_e, cur, col + 32 * b + e, pos, (cur.t0 + cut_tile) * BN,
+                                                                 min(cur.kmax, (cur.t0 + cur.nt) * BN - 1));
+                                v[0] += e == 0 ? x : 0.0f;
+                                v[1] += e == 1 ? x : 0.0f;
+                                v[2] += e == 2 ? x : 0.0f;
+                                v[3] += e == 3 ? x : 0.0f;
+                            }
+                        }
+                    }
                     if (gated) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] *= sigmoid_ref(gt[b & 1][u][e]);
                     }
                     if (!valid[u]) continue;
-                    if (partial) *reinterpret_cast<f32x4*>(a.part_o + at[u] + 32 * b) = v;
-                    else store_out4(a.out, at[u] + 32 * b, a.out_dtype, v);
+                    if (partial) *reinterpret_cast<f32x4*>(a_e.part_o + at[u] + 32 * b) = v;
+                    else store_out4(a_e.out, at[u] + 32 * b, a_e.out_dtype, v);
                 }
                 __builtin_amdgcn_wave_barrier();
             }
@@ -1566,7 +1748,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A a)
         if (!has_next) break;
         cur = nxt;
     }
-    if constexpr (PAGED) paged_leave(a, C, cur);
+    if constexpr (PAGED) paged_leave(args, C, cur);
 }
 
 }  // namespace

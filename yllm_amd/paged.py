@@ -19,11 +19,12 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import F32, YhipError, _gpu_of, check, lib
+from ._lib import ENOSPC, F32, OK, YhipError, check, elsewhere, lib
 from ._lib import current_stream as _stream
-from .attention import ROPE_MROPE, ROPE_NONE, LayerKV, _dtype_code, _ptr, _with_workspace
+from .attention import _DT, ROPE_MROPE, ROPE_NONE, LayerKV, _dtype_code, _with_workspace
 
 _I32 = torch.int32
+_F16 = torch.float16
 
 
 @dataclass
@@ -64,28 +65,35 @@ class PagedKV:
         return cls(k, v)
 
 
+# Small calls are bound by this module's own work (a decode step's kernels take 4 to 6 us), so the checks below ask a
+# tensor for as little as they can, and build messages only when they fail.
+
 def _pool(cache: PagedKV | LayerKV, fn: str) -> tuple[int, int, int, int]:
     """(n_blocks, n_kv, block, head_dim); a LayerKV is a pool of one page."""
     k, v = cache.k, cache.v
-    shape = (1, *k.shape) if isinstance(cache, LayerKV) else tuple(k.shape)
-    if len(shape) != 4 or k.dtype != torch.float16 or v.dtype != torch.float16 or not k.is_contiguous() \
+    shape = k.shape
+    if len(shape) == 3:
+        shape = (1, *shape)
+    if len(shape) != 4 or k.dtype is not _F16 or v.dtype is not _F16 or not k.is_contiguous() \
             or not v.is_contiguous() or v.numel() != k.numel():
         raise YhipError(-22, f"{fn}: the cache must hold contiguous f16 K and V of one size")
     return shape
 
 
-def _ints(fn: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dtype != _I32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+def _ints(fn: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         raise YhipError(-22, f"{fn}: {name} must be contiguous int32 [{n}]")
-    return t
 
 
 def _table(fn: str, t: torch.Tensor) -> tuple[int, int, int]:
     """(rows, entries per row, row stride) of a block table."""
-    if t.dtype != _I32 or t.dim() != 2 or t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise YhipError(-22, f"{fn}: block_table must be int32 [n_seq, max_blocks] with unit column stride")
-    n, w = t.shape
-    return n, w, (t.stride(0) if n > 1 else w)
+    if t.dtype is _I32 and t.dim() == 2:
+        n, w = t.shape
+        if w and t.is_contiguous():
+            return n, w, w
+        if w and (w == 1 or t.stride(1) == 1):
+            return n, w, (t.stride(0) if n > 1 else w)
+    raise YhipError(-22, f"{fn}: block_table must be int32 [n_seq, max_blocks] with unit column stride")
 
 
 @dataclass
@@ -112,33 +120,48 @@ def paged_plan(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torc
     _ints(fn, "ctx_lens", ctx_lens, n)
     _ints(fn, "new_lens", new_lens, n)
     _ints(fn, "n_free", n_free, 1)
-    _ints(fn, "free_blocks", free_blocks, free_blocks.numel())
+    n_list = free_blocks.numel()
+    _ints(fn, "free_blocks", free_blocks, n_list)
     if out is None:
-        dev = block_table.device
-        # one allocation: int32 parts of n + 1, n, n_tok, n_tok and 4
-        buf = torch.empty(2 * n + 2 * n_tok + 5, dtype=_I32, device=dev)
-        cu, lens, slots, pos, counts = buf.split([n + 1, n, n_tok, n_tok, 4])
-        out = PagedStep(block_table, cu, lens, slots, pos, counts)
+        # one allocation
+        buf = torch.empty(2 * n + 2 * n_tok + 5, dtype=_I32, device=block_table.device)
+        cu, lens, slots, pos, counts = buf.split_with_sizes([n + 1, n, n_tok, n_tok, 4])
+        there = elsewhere(fn, block_table.get_device(), ctx_lens, new_lens, free_blocks, n_free)
     else:
-        out.block_table = block_table
-        for name, t, m in (("cu_new", out.cu_new, n + 1), ("kv_lens", out.kv_lens, n), ("slots", out.slots, n_tok),
-                           ("positions", out.positions, n_tok), ("counts", out.counts, 4)):
+        cu, lens, slots, pos, counts = out.cu_new, out.kv_lens, out.slots, out.positions, out.counts
+        for name, t, m in (("cu_new", cu, n + 1), ("kv_lens", lens, n), ("slots", slots, n_tok),
+                           ("positions", pos, n_tok), ("counts", counts, 4)):
             _ints(fn, name, t, m)
-    with _gpu_of(fn, block_table, ctx_lens, new_lens, free_blocks, n_free, out.cu_new, out.kv_lens, out.slots,
-                 out.positions, out.counts):
-        check(lib().yhip_paged_plan(block_table.data_ptr(), w, stride, ctx_lens.data_ptr(), new_lens.data_ptr(),
-                                    free_blocks.data_ptr(), free_blocks.numel(), n_free.data_ptr(), n, n_tok, block,
-                                    out.cu_new.data_ptr(), out.kv_lens.data_ptr(), out.slots.data_ptr(),
-                                    out.positions.data_ptr(), out.counts.data_ptr(), _stream()))
+        there = elsewhere(fn, block_table.get_device(), ctx_lens, new_lens, free_blocks, n_free, cu, lens, slots, pos,
+                          counts)
+    args = (block_table.data_ptr(), w, stride, ctx_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), n_list,
+            n_free.data_ptr(), n, n_tok, block, cu.data_ptr(), lens.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+            counts.data_ptr())
+    _launch(lib().yhip_paged_plan, args, there)
+    if out is None:
+        return PagedStep(block_table, cu, lens, slots, pos, counts)
+    out.block_table = block_table
     return out
 
 
-def _rows(fn: str, name: str, t: torch.Tensor, width: int, dtype: torch.dtype | None = None) -> int:
-    """The row stride of a [T, >= width] matrix with unit column stride."""
-    if t.dim() != 2 or t.shape[1] < width or t.stride(1) != 1 or (dtype is not None and t.dtype != dtype):
-        raise YhipError(-22, f"{fn}: {name} must be [T, >={width}] rows with unit column stride"
-                             f"{'' if dtype is None else f' of {dtype}'}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _launch(f, args: tuple, there) -> None:
+    if there is None:
+        rc = f(*args, _stream())
+    else:
+        with there:
+            rc = f(*args, _stream())
+    if rc != OK:
+        check(rc)
+
+
+def _rows(fn: str, name: str, t: torch.Tensor, rows: int, width: int) -> int:
+    """The row stride of a [rows, >= width] matrix with unit column stride."""
+    if t.dim() == 2:
+        n, w = t.shape
+        step, one = t.stride()
+        if n == rows and w >= width and (one == 1 or w == 1):
+            return step if n > 1 else w
+    raise YhipError(-22, f"{fn}: {name} must be [{rows}, >={width}] rows with unit column stride")
 
 
 def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -158,42 +181,45 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
     None.  Rows without a slot (negative) are skipped."""
     fn = "qk_norm_rope_kv_store"
     n_blocks, n_kv, block, d = _pool(cache, fn)
+    dt = k.dtype
     T = k.shape[0]
-    ks, vs = _rows(fn, "k", k, n_kv * d), _rows(fn, "v", v, n_kv * d, k.dtype)
-    qs = qos = 0
+    ks, vs = _rows(fn, "k", k, T, n_kv * d), _rows(fn, "v", v, T, n_kv * d)
+    if v.dtype is not dt or dt not in _DT or (q is not None and q.dtype is not dt):
+        raise YhipError(-22, f"{fn}: q, k and v must have one type, f32, f16 or bf16")
+    qs = qos = qp = qop = 0
     qdt = F32
-    if v.shape[0] != T or (q is not None and q.shape[0] != T):
-        raise YhipError(-22, f"{fn}: q, k, v row counts differ")
     if q is not None:
-        qs = _rows(fn, "q", q, n_heads * d, k.dtype)
+        qs = _rows(fn, "q", q, T, n_heads * d)
         if q_out is None:
-            q_out = torch.empty((T, n_heads * d), dtype=q_out_dtype or q.dtype, device=q.device)
-        qos = _rows(fn, "q_out", q_out, n_heads * d)
-        if q_out.shape[0] != T:
-            raise YhipError(-22, f"{fn}: q_out must have the rows of q")
+            q_out = torch.empty((T, n_heads * d), dtype=q_out_dtype or dt, device=q.device)
+        qos = _rows(fn, "q_out", q_out, T, n_heads * d)
         qdt = _dtype_code(q_out)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     else:
         q_out = None
-    if slots is not None:
-        _ints(fn, "slots", slots, T)
-        if positions is None:
-            raise YhipError(-22, f"{fn}: slots come with positions")
+    pp = sp = wq = wk = None
     if positions is not None:
         _ints(fn, "positions", positions, T)
+        pp = positions.data_ptr()
+    if slots is not None:
+        if positions is None:
+            raise YhipError(-22, f"{fn}: slots come with positions")
+        _ints(fn, "slots", slots, T)
+        sp = slots.data_ptr()
     norm = F32
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.shape != (d,) or not w.is_contiguous() or w.dtype not in (torch.float32, torch.float16)):
-            raise YhipError(-22, f"{fn}: {name} must be [{d}], f32 or f16")
-    if q_norm is not None and k_norm is not None:
-        if q_norm.dtype != k_norm.dtype:
-            raise YhipError(-22, f"{fn}: q_norm and k_norm must have one type")
-        norm = _dtype_code(q_norm)
-    with _gpu_of(fn, cache.k, cache.v, q, k, v, q_out, positions, slots, q_norm, k_norm):
-        check(lib().yhip_qk_norm_rope_kv_store(
-            _ptr(q_out), qdt, qos, _ptr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _dtype_code(k), _ptr(q_norm),
-            _ptr(k_norm), norm, eps, cache.k.data_ptr(), cache.v.data_ptr(), n_blocks, block, _ptr(positions),
-            _ptr(slots), pos_start, T, n_heads, n_kv, d, rope, n_rot if rope == ROPE_MROPE else 0,
-            theta if rope != ROPE_NONE else 1.0, _stream()))
+    if q_norm is not None or k_norm is not None:
+        for w in (q_norm, k_norm):
+            if w is None or w.shape != (d,) or not w.is_contiguous() or w.dtype is not q_norm.dtype \
+                    or w.dtype not in (torch.float32, _F16):
+                raise YhipError(-22, f"{fn}: q_norm and k_norm must both be [{d}], f32 or f16")
+        norm = _DT[q_norm.dtype]
+        wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
+    kc, vc = cache.k, cache.v
+    args = (qop, qdt, qos, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DT[dt], wq, wk, norm, eps, kc.data_ptr(),
+            vc.data_ptr(), n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
+            n_rot if rope == ROPE_MROPE else 0, theta if rope != ROPE_NONE else 1.0)
+    _launch(lib().yhip_qk_norm_rope_kv_store, args,
+            elsewhere(fn, k.get_device(), kc, vc, q, v, q_out, positions, slots, q_norm, k_norm))
     return q_out
 
 
@@ -225,22 +251,39 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, kv_le
     _ints(fn, "kv_lens", kv_lens, n)
     _ints(fn, "cu_new", cu_new, n + 1)
     width = n_heads * d
-    qs = _rows(fn, "q", q, width)
     T = q.shape[0]
-    if q.shape[1] != width:
+    if q.shape[-1] != width:
         raise YhipError(-22, f"{fn}: q must be [T, n_heads*head_dim]")
+    qs = _rows(fn, "q", q, T, width)
     if max_len is None:
         max_len = min(w * block, 0x7fffffff)
     if out is None:
         out = torch.empty((T, width), dtype=out_dtype or q.dtype, device=q.device)
-    os_ = _rows(fn, "out", out, width)
-    if out.shape[0] != T or (gate is not None and gate.shape[0] != T):
-        raise YhipError(-22, f"{fn}: out and gate must have the rows of q")
-    gs = _rows(fn, "gate", gate, width, torch.float32) if gate is not None else 0
-    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, cache.k.data_ptr(),
-            cache.v.data_ptr(), n_blocks, block, block_table.data_ptr(), w, stride, kv_lens.data_ptr(),
-            cu_new.data_ptr(), n, T, max_new, max_len, n_heads, n_kv, d, _ptr(gate), gs)
-    with _gpu_of(fn, q, cache.k, cache.v, block_table, kv_lens, cu_new, out, gate):
-        _with_workspace(lib().yhip_paged_attn, args, workspace,
-                        lambda: paged_attn_workspace_bytes(T, n, max_new, max_len, n_heads, n_kv, d), q.device)
+    os_ = _rows(fn, "out", out, T, width)
+    gp, gs = None, 0
+    if gate is not None:
+        gs = _rows(fn, "gate", gate, T, width)
+        gp = gate.data_ptr()
+        if gate.dtype is not torch.float32:
+            raise YhipError(-22, f"{fn}: gate must be fp32")
+    kc, vc = cache.k, cache.v
+    dev = q.get_device()
+    there = elsewhere(fn, dev, kc, vc, block_table, kv_lens, cu_new, out, gate)
+    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, kc.data_ptr(), vc.data_ptr(),
+            n_blocks, block, block_table.data_ptr(), w, stride, kv_lens.data_ptr(), cu_new.data_ptr(), n, T, max_new,
+            max_len, n_heads, n_kv, d, gp, gs)
+    f = lib().yhip_paged_attn
+    if there is None and workspace is not None and workspace.get_device() == dev:
+        rc = f(*args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+        if rc == OK:
+            return out
+        if rc != ENOSPC:
+            check(rc)
+        workspace = None  # too short: allocated below
+    need = lambda: paged_attn_workspace_bytes(T, n, max_new, max_len, n_heads, n_kv, d)  # noqa: E731
+    if there is None:
+        _with_workspace(f, args, workspace, need, q.device)
+    else:
+        with there:
+            _with_workspace(f, args, workspace, need, q.device)
     return out
