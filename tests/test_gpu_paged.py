@@ -451,11 +451,12 @@ def test_attn_output_types_strides_and_rows_behind(cuda, out_dtype):
 @pytest.mark.parametrize("seqs", [[(200, 1)] * 3, [(200, 5), (90, 1)], [(400, 150), (64, 64)]])
 def test_attn_table_entries_outside_the_pool(cuda, seqs):
     """They read as zeros: keys that score 0 with a value of 0."""
-    b = Batch(seqs, 8, 2, 128, seed=9)
-    b.table[0, 0], b.table[1, 0] = 1 << 30, -9
-    for i in (0, 1):
-        b.K[i][:, :64], b.V[i][:, :64] = 0, 0
-    b.check()
+    for block, nkv, d in ((64, 2, 128), (128, 2, 256), (256, 4, 64)):
+        b = Batch(seqs, 8, nkv, d, block=block, seed=9)
+        b.table[0, 0], b.table[1, 0] = 1 << 30, -9
+        for i in (0, 1):
+            b.K[i][:, :block], b.V[i][:, :block] = 0, 0
+        b.check()
 
 
 @pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128), (16, 2, 256)])

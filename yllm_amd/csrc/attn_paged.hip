@@ -149,14 +149,18 @@ void launch_tiles(const PagedAttnArgs& a, hipStream_t st)
 
 }  // namespace
 
-size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t, uint32_t max_len, uint32_t n_heads, uint32_t n_kv,
-                            uint32_t D)
+size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                            uint32_t n_kv, uint32_t D)
 {
-    return paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1), D);
+    // (the decode kernel's, where it serves every call within the bounds; else also large enough for its calls)
+    const size_t decode = paged_decode_workspace(n_seq, max_len, n_kv, D);
+    if (paged_decode_fits(n_heads, n_kv, max_new)) return decode;
+    return std::max(decode, paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1), D));
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
 {
+    if (paged_decode_fits(in.n_heads, in.n_kv, in.max_new)) return launch_paged_decode(in, st);
     PagedAttnArgs a = in;
     const bool qs = a.q_dtype == kF32;
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;

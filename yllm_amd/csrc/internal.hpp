@@ -197,6 +197,12 @@ size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, ui
                             uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t st);
 
+// ---- paged_decode.hip ----
+// whether every sequence's new tokens fit the decode kernel's rows, and its part of launch_paged_attn
+bool paged_decode_fits(uint32_t n_heads, uint32_t n_kv, uint32_t max_new);
+size_t paged_decode_workspace(uint32_t n_seq, uint32_t max_len, uint32_t n_kv, uint32_t D);
+hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t st);
+
 // ---- o_proj.hip ----
 struct OProjArgs {
     float* x;               // [B] rows x_stride apart, residual in / out

@@ -77,6 +77,11 @@ __device__ inline uint64_t seq_units(const PagedAttnArgs& a, const PagedSeq& s)
     return (uint64_t)a.n_kv * a.gmax * (plain_before(nb - 1, c) + plain_last(s));
 }
 
+// How the line of units is made up (paged_decode.hip has another)
+struct PagedLine {
+    static __device__ uint64_t units(const PagedAttnArgs& a, const PagedSeq& s) { return seq_units(a, s); }
+};
+
 // A piece of an item: `n` key tiles from t0 on.  part: 0 the whole item, 1 its
 // first piece, 2 a later one.  idle: no key of it is seen (its tile is loaded
 // and not used).
@@ -120,7 +125,7 @@ __device__ inline const PagedAttnArgs& fresh_args(const PagedAttnArgs&)
 // are spread over the XCDs (consecutive workgroups go to the 8 XCDs in turn),
 // neighbours on one XCD, whose L2 then holds the keys they share.  `scratch`:
 // 24 words of LDS, free again after the call's last barrier.
-template <int NT>
+template <int NT, class Line = PagedLine>
 __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C)
 {
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
@@ -128,7 +133,7 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
     const uint32_t per = small ? 1u : (a.n_seq + NT - 1) / NT;
     const uint32_t lo = min((small ? lane : t) * per, a.n_seq), hi = min(lo + per, a.n_seq);
     uint64_t sum = 0;
-    for (uint32_t i = lo; i < hi; ++i) sum += seq_units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
+    for (uint32_t i = lo; i < hi; ++i) sum += Line::units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
     uint64_t inc = sum;
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
@@ -167,7 +172,7 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
         if (mine) {
             uint32_t i = lo;
             for (;; ++i) {
-                const uint64_t n = seq_units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
+                const uint64_t n = Line::units(a, paged_seq(a, a.cu_new[i], a.cu_new[i + 1], a.kv_lens[i]));
                 if (begin < before + n) break;
                 before += n;
             }
@@ -179,6 +184,36 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
         C.off = uni((uint32_t)scratch[17]);
         __syncthreads();
     }
+    return true;
+}
+
+// An item of T units, the cursor at its unit t: moves the cursor past the
+// chunk's piece of it, units t .. t + n - 1; false if the chunk ends before
+// it.  Cuts inside items of at most snap_units + fixed units, and at or before
+// unit `start`, move to the item's start (the chunk that begins with such a
+// cut takes the item whole, t becomes 0).  last: the chunk that ends the item.
+__device__ inline bool paged_cut(const PagedAttnArgs& a, PagedCursor& C, uint32_t T, uint32_t& t, uint32_t fixed,
+                                 uint32_t start, uint32_t& n, uint32_t& last)
+{
+    auto at_start = [&](uint32_t cut) { return T <= a.snap_units + fixed || cut <= start; };
+    if (C.fresh && t > 0 && at_start(t)) {
+        C.off -= t;
+        C.done -= (int)t;
+        t = 0;
+    }
+    C.fresh = false;
+    const int to_end = C.done + (int)(T - t);  // of the chunk, at the item's end
+    n = T - t;
+    if (to_end > C.len) {  // the chunk ends inside the item
+        n = (uint32_t)(C.len - C.done);
+        if (at_start(t + n)) {
+            C.done = C.len;
+            return false;
+        }
+    }
+    last = C.j + (uint32_t)(to_end - 1) / C.chunk;
+    C.off += n;
+    C.done += (int)n;
     return true;
 }
 
@@ -227,26 +262,8 @@ __device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedI
             none = I.h >= h1;
             seen = s.pos0 + (int)min(s.nq, (b + 1) * kItemRows);
         }
-        // cuts inside short items, and near an item's start, move to its start
-        auto at_start = [&](uint32_t cut) { return T <= a.snap_units + kItemUnits || cut <= kItemUnits + 1; };
-        if (C.fresh && t > 0 && at_start(t)) {
-            C.off -= t;
-            C.done -= (int)t;
-            t = 0;
-        }
-        C.fresh = false;
-        const int to_end = C.done + (int)(T - t);  // of the chunk, at the item's end
-        uint32_t n = T - t;
-        if (to_end > C.len) {  // the chunk ends inside the item
-            n = (uint32_t)(C.len - C.done);
-            if (at_start(t + n)) {
-                C.done = C.len;
-                return false;
-            }
-        }
-        I.last = C.j + (uint32_t)(to_end - 1) / C.chunk;  // the chunk that ends the item
-        C.off += n;
-        C.done += (int)n;
+        uint32_t n;
+        if (!paged_cut(a, C, T, t, kItemUnits, kItemUnits + 1, n, I.last)) return false;
         if (none) continue;
         I.part = n == T ? 0u : t == 0 ? 1u : 2u;
         const uint32_t tile0 = t ? t - kItemUnits : 0u;  // the piece's tiles of 64 keys
@@ -298,5 +315,62 @@ __device__ inline uint32_t paged_page(const PagedAttnArgs& a, uint32_t seq, uint
     return (uint32_t)const_ints(a.table + (size_t)seq * a.table_stride)[key >> a.shift];
 }
 
+// ---- shared by the kernels ----
+
+__device__ inline float sigmoid_ref(float g) { return 1.0f / (1.0f + expf(-g)); }
+
+__device__ inline void store_out4(void* out, size_t off, uint32_t dt, f32x4 v)
+{
+    if (dt == kF32) {
+        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + off) = v;
+    } else if (dt == kF16) {
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        f16x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = (_Float16)v[j];
+        *reinterpret_cast<f16x4*>(reinterpret_cast<uint16_t*>(out) + off) = h;
+    } else {
+        // round to nearest even; each element goes through a scalar float
+        // (bit-casting an ext-vector element directly reads element 0)
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = v[j];
+            const uint32_t x = __builtin_bit_cast(uint32_t, f);
+            h[j] = (x + 0x7fffu + ((x >> 16) & 1u)) >> 16;
+        }
+        u32x2 w;
+        w[0] = h[0] | (h[1] << 16);
+        w[1] = h[2] | (h[3] << 16);
+        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(out) + off) = w;
+    }
+}
+
+// Values for the product with the probabilities' lo parts: an inf or NaN as a
+// finite value.  The hi parts bring it in; with a lo part, 0 or negative
+// beside a positive hi, the same inf would make NaN.
+__device__ inline f16x8 bounded(const f16x8& v)
+{
+    const f16x8 top = {65504, 65504, 65504, 65504, 65504, 65504, 65504, 65504};
+    return __builtin_elementwise_max(__builtin_elementwise_min(v, top), -top);
+}
+// The sum of the infs and NaNs among the values of dimension d that a query at
+// position pos sees of keys lo .. end - 1.
+template <int D>
+__device__ float special_sum(const PagedAttnArgs& a, uint32_t seq, uint32_t kvh, uint32_t d, int pos, uint32_t lo, int end)
+{
+    float s = 0.0f;
+#pragma unroll 1
+    for (uint32_t k = lo; (int)k < end && (int)k <= pos; ++k) {
+        const PagedTile t = paged_tile<D>(a, (uint32_t)a.table[(size_t)seq * a.table_stride + (k >> a.shift)], kvh);
+        if (t.bytes == 0) continue;
+        const uint32_t off = k & ((1u << a.shift) - 1u);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc) + t.at);
+        const uint16_t b = p[(size_t)(off & ~31u) * D + d * kVTile + (off & 31u)];
+        if ((b & 0x7fff) >= 0x7c00) s += f16_bits_to_f32(b);
+    }
+    return s;
+}
 }  // namespace
 }  // namespace yhip

@@ -52,8 +52,6 @@ __device__ inline f32x16 mfma32(const f16x8& a, const f16x8& b, const f32x16& c)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ inline float sigmoid_ref(float g) { return 1.0f / (1.0f + expf(-g)); }
-
 // key row r of a tile lives in LDS row perm(r): rows 4..7 <-> 8..11 of each 16
 __device__ inline int lds_row_of_key(int r)
 {
@@ -85,34 +83,6 @@ __device__ inline void split_q8(f16x8& hi, f16x8& lo, const f32x4& a, const f32x
         lo[j] = (_Float16)(a[j] - (float)hi[j]);
         hi[j + 4] = (_Float16)b[j];
         lo[j + 4] = (_Float16)(b[j] - (float)hi[j + 4]);
-    }
-}
-
-__device__ inline void store_out4(void* out, size_t off, uint32_t dt, f32x4 v)
-{
-    if (dt == kF32) {
-        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + off) = v;
-    } else if (dt == kF16) {
-        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-        f16x4 h;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = (_Float16)v[j];
-        *reinterpret_cast<f16x4*>(reinterpret_cast<uint16_t*>(out) + off) = h;
-    } else {
-        // round to nearest even; each element goes through a scalar float
-        // (bit-casting an ext-vector element directly reads element 0)
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float f = v[j];
-            const uint32_t x = __builtin_bit_cast(uint32_t, f);
-            h[j] = (x + 0x7fffu + ((x >> 16) & 1u)) >> 16;
-        }
-        u32x2 w;
-        w[0] = h[0] | (h[1] << 16);
-        w[1] = h[2] | (h[3] << 16);
-        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(out) + off) = w;
     }
 }
 
@@ -169,31 +139,6 @@ __device__ inline bool clean_v(f16x8* ch, int c, uint32_t valid, bool cut)
     }
     *reinterpret_cast<u16x8*>(ch) = v;
     return odd && cut;
-}
-// Values for the product with the probabilities' lo parts: an inf or NaN as a
-// finite value.  The hi parts bring it in; with a lo part, 0 or negative
-// beside a positive hi, the same inf would make NaN.
-__device__ inline f16x8 bounded(const f16x8& v)
-{
-    const f16x8 top = {65504, 65504, 65504, 65504, 65504, 65504, 65504, 65504};
-    return __builtin_elementwise_max(__builtin_elementwise_min(v, top), -top);
-}
-// The sum of the infs and NaNs among the values of dimension d that a query at
-// position pos sees of keys lo .. hi of the item.
-template <int D>
-__device__ float special_sum(const PagedAttnArgs& a, const PagedItem& I, uint32_t d, int pos, uint32_t lo, uint32_t hi)
-{
-    float s = 0.0f;
-#pragma unroll 1
-    for (uint32_t k = lo; k <= hi && (int)k <= pos; ++k) {
-        const PagedTile t = paged_tile<D>(a, (uint32_t)a.table[(size_t)I.seq * a.table_stride + (k >> a.shift)], I.kvh);
-        if (t.bytes == 0) continue;
-        const uint32_t off = k & ((1u << a.shift) - 1u);
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc) + t.at);
-        const uint16_t b = p[(size_t)(off & ~31u) * D + d * kVTile + (off & 31u)];
-        if ((b & 0x7fff) >= 0x7c00) s += f16_bits_to_f32(b);
-    }
-    return s;
 }
 // the first tile of BN keys that an item's mask cuts; ~0 if its piece has none
 template <int BN>
@@ -604,7 +549,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if constexpr (PAGED) {
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.kc)) + p.at, 0, p.bytes, 0x00020000);
-                const uint32_t at = ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
+                const uint32_t at = p.bytes ? ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2 : 0u;
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], at);
             }
@@ -613,7 +558,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if constexpr (PAGED) {
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.vc)) + p.at, 0, p.bytes, 0x00020000);
-                const uint32_t at = ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
+                const uint32_t at = p.bytes ? ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2 : 0u;
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, vbuf(par) + (LT * i + 64 * wave) * 8, vgo[i], at);
             }
@@ -1164,8 +1109,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 if (add_odd)
 #pragma unroll 1
                     for (int e = 0; e < 4; ++e) {
-                        const float x = special_sum<D>(a_e, cur, d + e, pos_e, cut_tile * BN,
-                                                         min(cur.kmax, (cur.t0 + cur.nt) * BN - 1));
+                        const float x = special_sum<D>(a_e, cur.seq, cur.kvh, d + e, pos_e, cut_tile * BN,
+                                                         (int)min(cur.kmax + 1, (cur.t0 + cur.nt) * BN));
                         v[0] += e == 0 ? x : 0.0f;
                         v[1] += e == 1 ? x : 0.0f;
                         v[2] += e == 2 ? x : 0.0f;
@@ -1324,8 +1269,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                                                          0, (a.kv_stride - p0) * D * 2, 0x00020000);
             }
         };
-        auto tile_at = [&](uint32_t p0, uint32_t kt) -> uint32_t {
-            if constexpr (PAGED) return ((p0 + kt * BN) & ((1u << a.shift) - 1u)) * D * 2;
+        auto tile_at = [&](uint32_t p0, uint32_t kt, const PagedTile& p) -> uint32_t {
+            if constexpr (PAGED) return p.bytes ? ((p0 + kt * BN) & ((1u << a.shift) - 1u)) * D * 2 : 0u;
             else return kt * BN * D * 2;
         };
         auto place = [&](const Item& I, uint32_t p0, uint32_t kt) {  // of tile kt
@@ -1334,14 +1279,14 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
         };
         auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
             const __amdgpu_buffer_rsrc_t r = rsrc_at(a.kc, kv, p0, p);
-            const uint32_t at = tile_at(p0, kt);
+            const uint32_t at = tile_at(p0, kt, p);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
                 lds_load16(r, kbuf(par) + (512 * i + 64 * wave) * 8, kgo, at + i * (16 * D * 2));
         };
         auto dma_v = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
             const __amdgpu_buffer_rsrc_t r = rsrc_at(a.vc, kv, p0, p);
-            const uint32_t at = tile_at(p0, kt);
+            const uint32_t at = tile_at(p0, kt, p);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
                 lds_load16(r, vbuf(par) + (512 * i + 64 * wave) * 8, vgo, at + i * (64 * (int)kVTile * 2));
@@ -1725,8 +1670,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                             const int pos = cur.pos0 + (int)row_from(a_e, cur, qw * 32 + 8 * u + er).t;
 #pragma unroll 1
                             for (int e = 0; e < 4; ++e) {
-                                const float x = special_sum<D>(a_e, cur, col + 32 * b + e, pos, (cur.t0 + cut_tile) * BN,
-                                                                 min(cur.kmax, (cur.t0 + cur.nt) * BN - 1));
+                                const float x = special_sum<D>(a_e, cur.seq, cur.kvh, col + 32 * b + e, pos, (cur.t0 + cut_tile) * BN,
+                                                                 (int)min(cur.kmax + 1, (cur.t0 + cur.nt) * BN));
                                 v[0] += e == 0 ? x : 0.0f;
                                 v[1] += e == 1 ? x : 0.0f;
                                 v[2] += e == 2 ? x : 0.0f;
