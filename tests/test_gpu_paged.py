@@ -298,6 +298,34 @@ def test_qk_norm_rope_into_a_contiguous_cache(cuda):
         assert torch.equal(qa, qb) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
 
 
+@pytest.mark.parametrize("T", [4, 160])
+def test_qk_norm_rope_stores_the_bits_that_kv_store_stores(cuda, T):
+    """Ties, f16 subnormals, results at the ends of the range, inf and NaN, of every type that can hold them."""
+    from yllm_amd.attention import ROPE_NONE, LayerKV, kv_store
+    from yllm_amd.paged import qk_norm_rope_kv_store
+
+    g = _gen(3)
+    e = torch.randint(-30, 18, (T, 2 * 64), generator=g, device="cuda").float()
+    m = 1.0 + torch.randint(0, 2048, e.shape, generator=g, device="cuda") / 2048.0  # ties at 11 bits
+    x = m * torch.exp2(e) * torch.where(torch.rand(e.shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    x[:, ::5] = torch.nextafter(x[:, ::5], torch.zeros_like(x[:, ::5]))
+    x[:, 1::7] = torch.nextafter(x[:, 1::7], torch.full_like(x[:, 1::7], math.inf))
+    special = [0.0, -0.0, math.inf, -math.inf, math.nan, 65504.0, 65519.99, 65520.0, -65520.0, 65536.0, 3e38, 1e-45, -1e-40,
+               2.0 ** -14, 2.0 ** -14 - 2.0 ** -38, 2.0 ** -14 - 2.0 ** -25, 2.0 ** -24, 2.0 ** -25, 2.0 ** -25 - 2.0 ** -49,
+               3 * 2.0 ** -25, 1.5 * 2.0 ** -15]
+    x[0, :len(special)] = torch.tensor(special, device="cuda")
+    for dtype in (F32, BF16, F16):
+        y = x.to(dtype)
+        a, b = LayerKV.empty(2, 64, 192), LayerKV.empty(2, 64, 192)
+        kv_store(a, y, y.flip(0).contiguous(), 3)
+        qk_norm_rope_kv_store(b, None, y, y.flip(0).contiguous(), 2, ROPE_NONE, 1.0, pos_start=3)
+        for s, t in ((a.k, b.k), (a.v, b.v)):
+            nan = s.isnan()
+            assert torch.equal(nan, t.isnan())
+            s, t = s.view(torch.int16).masked_fill(nan, 0), t.view(torch.int16).masked_fill(nan, 0)
+            assert torch.equal(s, t), (dtype, int((s != t).sum()))
+
+
 # ---- paged_attn --------------------------------------------------------------------------------------
 
 class Batch:

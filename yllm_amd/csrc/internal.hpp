@@ -163,8 +163,8 @@ struct QkNormRopeArgs {
     uint32_t dtype, q_out_dtype, q_stride, k_stride, v_stride, q_out_stride, norm_f16;
     uint32_t n_tok, n_heads, n_kv, D, block, n_slots, pos_start, kind, n_rot;
     float eps;
-    // set by the launcher: waves per token, heads per wave, workgroups of each role
-    uint32_t groups, heads_per_wave, rope_blocks, v_blocks;
+    // set by the launcher: waves per token, passes per wave, workgroups of each role
+    uint32_t groups, passes, rope_blocks, v_blocks;
     // turns[j] = theta^(-2j / span) / 2 pi for the rotated pairs j < span / 2
     double turns[128];
 };

@@ -14,14 +14,14 @@
 // The row's slot says where K and V go: page slot / block, row slot % block.
 // Rows without a slot (negative, or past the pool) are skipped.
 //
-// Bound by HBM: each row is read once and written once.  A lane holds eight
-// elements of a head as two runs of four (for pairs half a span apart one run
-// of the first and one of the second elements, so a pair never leaves the
-// lane; otherwise eight consecutive ones), so a head is D / 8 lanes, a wave
-// takes 64 / (D / 8) heads a pass, and the sum of squares is a few DPP steps.
-// The lane's four sines and cosines serve all its passes.  V is stored
-// d-major, in 16-byte groups of eight positions, by workgroups of their own
-// (a few rows: by the same waves, 2 bytes at a time).
+// Bound by HBM and, half as much, by its arithmetic: each row is read once and
+// written once.  A lane holds eight elements of a head as two runs of four, with
+// neighbouring lanes' runs next to each other (eight in one run left every load
+// and store with holes), and the pairs of every rope kind within one lane; so a
+// head is D / 8 lanes, a wave takes 64 / (D / 8) heads a pass, and the sum of
+// squares is a few DPP steps.  The lane's four sines and cosines serve all its
+// passes.  V is stored d-major, in 16-byte groups of eight positions, by
+// workgroups of their own (a few rows: by the same waves, 2 bytes at a time).
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -47,26 +47,60 @@ __device__ inline f32x4 load4(const void* p, size_t i)
     }
 }
 
-__device__ inline uint16_t bf16_bits(float x)
+// The value whose truncation to f16 is f32_to_f16_ref(x), without branches:
+// half a step of the result is added (to the magnitude's bits where it is
+// normal in f16; 2^-25 below, exactly), what rounds past the largest becomes
+// inf.  (The general form is some twenty instructions and six branches for each
+// element; waves that spent them were bound by them, not by HBM.)
+__device__ inline float half_away(float x)
 {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);  // NaN stays NaN
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+    const float a = fabsf(x);
+    float t = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) + 0x1000u);
+    const float half = 2.98023223876953125e-08f;  // below it, zero (and the sum would round up to the first step)
+    t = a < 6.103515625e-05f ? x + copysignf(a < half ? 0.0f : half, x) : t;
+    t = a >= 65520.0f ? copysignf(INFINITY, x) : t;
+    return x == x ? t : x;
+}
+__device__ inline u16x4 to_cache4(const f32x4& x)
+{
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(half_away(x[0]), half_away(x[1]))),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(half_away(x[2]), half_away(x[3])))};
+    return __builtin_bit_cast(u16x4, w);
 }
 
+// (the conversions to bf16 and f16 are gfx950's own, to nearest even)
 __device__ inline void store4(void* p, size_t i, uint32_t dt, const f32x4& x)
 {
     if (dt == kF32) {
         *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i) = x;
-    } else {
-        u16x4 w;
+    } else if (dt == kF16) {
+        f16x4 w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float f = x[e];
-            w[e] = dt == kF16 ? __builtin_bit_cast(uint16_t, (_Float16)f) : bf16_bits(f);
-        }
-        *reinterpret_cast<u16x4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
+        for (int e = 0; e < 4; ++e) w[e] = (_Float16)x[e];
+        *reinterpret_cast<f16x4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
+    } else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        bf16x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (__bf16)x[e];
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
     }
+}
+
+// sine and cosine of u turns: whole turns and then quarters are taken off in
+// 64 bits, and the Taylor series over an eighth of a turn to either side follow
+// (what they leave out is below 2.5e-8)
+__device__ inline void sincos_turns(double u, float* sn, float* cs)
+{
+    const double q4 = 4.0 * (u - __builtin_rint(u)), whole = __builtin_rint(q4);
+    const float x = 1.5707963267948966f * (float)(q4 - whole), z = x * x;
+    const int q = (int)whole;
+    const float s = x + x * z * (-1.6666667e-1f + z * (8.3333333e-3f + z * (-1.9841270e-4f + z * 2.7557319e-6f)));
+    const float c = 1.0f + z * (-0.5f + z * (4.1666667e-2f + z * (-1.3888889e-3f + z * 2.4801587e-5f)));
+    const float a = q & 1 ? c : s, b = q & 1 ? s : c;
+    *sn = q & 2 ? -a : a;
+    *cs = (q + 1) & 2 ? -b : b;
 }
 
 // the sum over each aligned group of N lanes, by DPP moves: within quads, the
@@ -131,14 +165,17 @@ __device__ void v_block(const QkNormRopeArgs& a, uint32_t vb)
         slots[t] = b >= 0 && (uint32_t)b < a.n_tok ? slot_of(a, (uint32_t)b) : -1;
     }
 #pragma unroll
-    for (uint32_t u = 0; u < R / 16; ++u)
+    for (uint32_t u = 0; u < R / 16; ++u) {
+        u16x4 w;
+        if constexpr (DT == kF16) {  // f16 rows keep their bits (the widened value is converted back; a NaN's payload apart)
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-            const float f = x[u][e];
-            // f16 rows keep their bits (the widened value rounds back to them; a NaN's payload apart)
-            tile[(c4 + e) * TP + rr + 16u * u] =
-                DT == kF16 ? __builtin_bit_cast(uint16_t, (_Float16)f) : f32_to_f16_ref(f);
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_bit_cast(uint16_t, (_Float16)x[u][e]);
+        } else {
+            w = to_cache4(x[u]);
         }
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) tile[(c4 + e) * TP + rr + 16u * u] = w[e];
+    }
     __syncthreads();
     if (t < 64u) {
         // leads(i): rows i .. i + 7 of slots[] are one group
@@ -210,70 +247,81 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
         }
     }
     constexpr uint32_t LPH = D / 8, HPP = 64 / LPH;  // lanes per head, heads per pass
-    constexpr uint32_t U = 4;                        // passes whose loads are issued together
+    constexpr uint32_t U = 3;                        // passes whose loads are issued together
     const uint32_t lane = threadIdx.x & 63u, i = lane % LPH, sub = lane / LPH;
-    const uint32_t w = blk * 4u + (threadIdx.x >> 6);
-    const uint32_t b = w / a.groups, g = w % a.groups;
+    const uint32_t w = blk * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t b = w / a.groups, g = w - b * a.groups;
     if (b >= a.n_tok) return;  // wave-uniform; no barrier follows in this role
+    // (the row's slot and position are waited for behind its first loads)
     const int slot = slot_of(a, b);
-    if (slot < 0) return;
     const int pos = a.positions ? a.positions[b] : (int)(a.pos_start + b);
 
-    // the lane's two runs of four elements, and whether its pairs turn
-    const uint32_t half = (KIND == kRopeMrope ? a.n_rot : (uint32_t)D) / 2;
-    const bool far = KIND == kRopeHalf || (KIND == kRopeMrope && 4u * i < half);
-    const bool turn = KIND == kRopePairs || far;
-    const uint32_t e0 = far ? 4u * i : 8u * i, e1 = far ? half + 4u * i : 8u * i + 4u;
+    // The lane's two runs of four elements: one of the lower and one of the upper half of the dimensions, or (MROPE)
+    // of the rotated ones or the rest.  Neighbouring lanes' runs are neighbours, and the pairs of every kind lie
+    // within a lane: two in each run, or one element in each.
+    const uint32_t span = KIND == kRopeMrope ? a.n_rot : (uint32_t)D;
+    const bool head = 8u * i < span;  // whether they are among the first `span` dimensions, which turn
+    const uint32_t e0 = head ? 4u * i : span / 2 + 4u * i, e1 = e0 + (head ? span : (uint32_t)D - span) / 2;
+    const bool turn = KIND != kRopeNone && head;
+    auto pair_of = [&](uint32_t e) -> uint32_t {  // the pair index of the lane's e-th pair
+        return KIND == kRopePairs ? (e < 2 ? 2u * i + e : D / 4 + 2u * i + (e - 2)) : 4u * i + e;
+    };
+
+    // This wave's passes: HPP heads each, those of q (none without q_out), then those of k.  A pass is of one kind,
+    // so that everything but the lane's offsets is wave-uniform.
+    const uint32_t pq = a.q_out ? (a.n_heads + HPP - 1) / HPP : 0u, passes = pq + (a.n_kv + HPP - 1) / HPP;
+    const uint32_t p_lo = g * a.passes, p_hi = min(passes, p_lo + a.passes);
+    const size_t esz = DT == kF32 ? 4 : 2;
+    const char* const qrow = reinterpret_cast<const char*>(a.q) + (size_t)b * a.q_stride * esz;
+    const char* const krow = reinterpret_cast<const char*>(a.k) + (size_t)b * a.k_stride * esz;
+    const size_t kstep = (size_t)a.block * D;  // between a page's heads
+    size_t kpage = 0;
     float c[4], s[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        c[e] = 1.0f;
-        s[e] = 0.0f;
-        if (turn) {
-            const double u = a.turns[4u * i + e] * (double)pos;
-            sincospif(2.0f * (float)(u - __builtin_rint(u)), &s[e], &c[e]);
-        }
-    }
     f32x4 qw[2], kw[2];
     const bool norm = a.q_norm != nullptr;
-    if (norm) {
-        if (a.norm_f16) {
-            qw[0] = load4<kF16>(a.q_norm, e0);
-            qw[1] = load4<kF16>(a.q_norm, e1);
-            kw[0] = load4<kF16>(a.k_norm, e0);
-            kw[1] = load4<kF16>(a.k_norm, e1);
-        } else {
-            qw[0] = load4<kF32>(a.q_norm, e0);
-            qw[1] = load4<kF32>(a.q_norm, e1);
-            kw[0] = load4<kF32>(a.k_norm, e0);
-            kw[1] = load4<kF32>(a.k_norm, e1);
-        }
-    }
-
-    // this wave's heads: [h_lo, h_hi) of q heads then kv heads (kv heads only without q_out)
-    const uint32_t heads = a.n_heads + a.n_kv;
-    const uint32_t h_lo = (a.q_out ? 0u : a.n_heads) + g * a.heads_per_wave;
-    const uint32_t h_hi = min(heads, h_lo + a.heads_per_wave);
-    const size_t krow = k_page_row<D>(a, 0, (uint32_t)slot), kstep = (size_t)a.block * D;  // + h * kstep
-    for (uint32_t h0 = h_lo; h0 < h_hi; h0 += HPP * U) {
+    for (uint32_t p0 = p_lo; p0 < p_hi; p0 += U) {
         // loads of U passes first, then their stores (q_out may be q: every lane reads its own elements before
-        // it writes them); past the end a valid head's are loaded again
+        // it writes them); heads past the last load it again
         f32x4 x[U][2];
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t h = min(h0 + u * HPP + sub, h_hi - 1u);
-            const bool is_q = h < a.n_heads;
-            const void* src = is_q ? a.q : a.k;
-            const size_t at = is_q ? (size_t)b * a.q_stride + (size_t)h * D
-                                   : (size_t)b * a.k_stride + (size_t)(h - a.n_heads) * D;
-            x[u][0] = load4<DT>(src, at + e0);
-            x[u][1] = load4<DT>(src, at + e1);
+            const uint32_t p = min(p0 + u, p_hi - 1u);
+            const bool is_q = p < pq;
+            const uint32_t h = min((is_q ? p : p - pq) * HPP + sub, (is_q ? a.n_heads : a.n_kv) - 1u);
+            const char* src = is_q ? qrow : krow;
+            x[u][0] = load4<DT>(src, h * D + e0);
+            x[u][1] = load4<DT>(src, h * D + e1);
+        }
+        if (p0 == p_lo) {  // once, behind the first loads
+            __builtin_amdgcn_sched_barrier(0);
+            if (slot < 0) return;  // wave-uniform
+            kpage = k_page_row<D>(a, 0, (uint32_t)slot);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[e] = 1.0f;
+                s[e] = 0.0f;
+                if (turn) sincos_turns(a.turns[pair_of(e)] * (double)pos, &s[e], &c[e]);
+            }
+            if (norm) {
+                if (a.norm_f16) {
+                    qw[0] = load4<kF16>(a.q_norm, e0);
+                    qw[1] = load4<kF16>(a.q_norm, e1);
+                    kw[0] = load4<kF16>(a.k_norm, e0);
+                    kw[1] = load4<kF16>(a.k_norm, e1);
+                } else {
+                    qw[0] = load4<kF32>(a.q_norm, e0);
+                    qw[1] = load4<kF32>(a.q_norm, e1);
+                    kw[0] = load4<kF32>(a.k_norm, e0);
+                    kw[1] = load4<kF32>(a.k_norm, e1);
+                }
+            }
         }
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t h = h0 + u * HPP + sub;
-            if (h0 + u * HPP >= h_hi) break;  // wave-uniform
-            const bool is_q = h < a.n_heads;
+            const uint32_t p = p0 + u;
+            if (p >= p_hi) break;  // wave-uniform
+            const bool is_q = p < pq;
+            const uint32_t h = (is_q ? p : p - pq) * HPP + sub;
             f32x4 y0 = x[u][0], y1 = x[u][1];
             if (norm) {
                 float ss = 0.0f;
@@ -281,45 +329,37 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
                 for (int e = 0; e < 4; ++e) ss = fmaf(y0[e], y0[e], fmaf(y1[e], y1[e], ss));
                 ss = group_sum<LPH>(ss);
                 const float inv = __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / D, a.eps));
+                y0 *= inv;
+                y1 *= inv;
+                y0 *= is_q ? qw[0] : kw[0];
+                y1 *= is_q ? qw[1] : kw[1];
+            }
+            if (KIND == kRopePairs) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    y0[e] *= inv * (is_q ? qw[0][e] : kw[0][e]);
-                    y1[e] *= inv * (is_q ? qw[1][e] : kw[1][e]);
+                    f32x4& y = e < 2 ? y0 : y1;
+                    const float v = y[2 * (e & 1)], r = y[2 * (e & 1) + 1];
+                    y[2 * (e & 1)] = v * c[e] - r * s[e];
+                    y[2 * (e & 1) + 1] = v * s[e] + r * c[e];
+                }
+            } else if (KIND != kRopeNone) {  // (lanes that do not turn have cosine 1 and sine 0)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = y0[e], r = y1[e];
+                    y0[e] = KIND == kRopeHalf || turn ? v * c[e] - r * s[e] : v;
+                    y1[e] = KIND == kRopeHalf || turn ? v * s[e] + r * c[e] : r;
                 }
             }
-            if (turn) {
-                if (KIND == kRopePairs) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f32x4& y = e < 2 ? y0 : y1;
-                        const float p = y[2 * (e & 1)], r = y[2 * (e & 1) + 1];
-                        y[2 * (e & 1)] = p * c[e] - r * s[e];
-                        y[2 * (e & 1) + 1] = p * s[e] + r * c[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float p = y0[e], r = y1[e];
-                        y0[e] = p * c[e] - r * s[e];
-                        y1[e] = p * s[e] + r * c[e];
-                    }
-                }
-            }
-            if (h >= h_hi) continue;
             if (is_q) {
-                const size_t at = (size_t)b * a.q_out_stride + (size_t)h * D;
-                store4(a.q_out, at + e0, a.q_out_dtype, y0);
-                store4(a.q_out, at + e1, a.q_out_dtype, y1);
-            } else {
-                uint16_t* row = a.kc + krow + (h - a.n_heads) * kstep;
-                u16x4 k0, k1;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    k0[e] = f32_to_f16_ref(y0[e]);
-                    k1[e] = f32_to_f16_ref(y1[e]);
+                if (h < a.n_heads) {
+                    const size_t at = (size_t)b * a.q_out_stride + h * D;
+                    store4(a.q_out, at + e0, a.q_out_dtype, y0);
+                    store4(a.q_out, at + e1, a.q_out_dtype, y1);
                 }
-                *reinterpret_cast<u16x4*>(row + e0) = k0;
-                *reinterpret_cast<u16x4*>(row + e1) = k1;
+            } else if (h < a.n_kv) {
+                uint16_t* row = a.kc + kpage + h * kstep;
+                *reinterpret_cast<u16x4*>(row + e0) = to_cache4(y0);
+                *reinterpret_cast<u16x4*>(row + e1) = to_cache4(y1);
             }
         }
     }
@@ -361,13 +401,11 @@ hipError_t launch_kind(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
 hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st)
 {
     const uint32_t hpp = 64u / (a.D / 8u);
-    const uint32_t active = a.q_out ? a.n_heads + a.n_kv : a.n_kv;
-    const uint32_t passes = (active + hpp - 1) / hpp;
-    const uint32_t per0 = a.n_tok <= kScatterRows ? 1u : 4u;
+    const uint32_t passes = (a.q_out ? (a.n_heads + hpp - 1) / hpp : 0u) + (a.n_kv + hpp - 1) / hpp;
+    const uint32_t per0 = a.n_tok <= kScatterRows ? 1u : 3u;
     const uint32_t groups = (passes + per0 - 1) / per0;
-    const uint32_t per = (passes + groups - 1) / groups;  // passes per wave, evenly
-    a.heads_per_wave = per * hpp;
-    a.groups = (passes + per - 1) / per;
+    a.passes = (passes + groups - 1) / groups;  // per wave, evenly
+    a.groups = (passes + a.passes - 1) / a.passes;
     a.rope_blocks = (uint32_t)(((uint64_t)a.n_tok * a.groups + 3u) / 4u);
     a.v_blocks = a.n_tok > kScatterRows ? a.n_kv * a.D / 64u * ((a.n_tok + 63u) / 64u) : 0u;
     const dim3 grid(a.rope_blocks + a.v_blocks);
