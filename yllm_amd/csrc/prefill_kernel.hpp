@@ -469,6 +469,10 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // then wait behind these loads; such items issue their loads at their
     // own start.
     const bool early = args.gate == nullptr && !PAIR;
+    // paged, 16-bit queries: an item waits for the next one's first loads before
+    // its output stores instead of behind them, so the stores drain during the
+    // next item's first step
+    constexpr bool AHEAD = PAGED && !QS && NB == 2;
     Item cur;
     if constexpr (PAGED) {
         const bool any = paged_start<256 * NG * (PAIR ? 2 : 1)>(fresh_args(args), reinterpret_cast<uint64_t*>(&Kl0[0][0]), C) &&
@@ -644,6 +648,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             issue_item_v(cur);
             issue_item_q(cur);
             if constexpr (NB > 2) deep_loads = issue_item_deep(cur);
+            if constexpr (AHEAD) dma_done();
         }
 
         const uint32_t kvh = cur.kvh;
@@ -882,7 +887,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // -> 79 us).  All loads are complete before the key loop, whose waits then
         // count only tile loads (in pair mode K(2) and V(1) may still be in
         // flight; the first step waits for them).
-        dma_wait_but(deep_loads);
+        if constexpr (!AHEAD) dma_wait_but(deep_loads);
         if (QL && it > 0) lds_barrier();  // the merge has read (max, sum)
         if constexpr (QS) {
             const float* qp = reinterpret_cast<const float*>(a.q) + (size_t)myrow.b * a.q_stride + (size_t)myrow.h * D +
@@ -900,7 +905,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
 #pragma unroll
             for (int kk = 0; kk < NKK; ++kk) bf16_to_f16(qf[kk]);
         }
-        if constexpr (NB > 2) lds_barrier();
+        if constexpr (NB > 2 || AHEAD) lds_barrier();
         else __syncthreads();
         f32x16 Sa[NS], Sb[NS];
         if (wsteps > 0) {
@@ -908,7 +913,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             xwrite(Sa, 0);
         }
         // step 0 loads K(NB) over K(0), whose last readers are the scores above
-        if constexpr (NB > 2) lds_barrier();
+        if constexpr (NB > 2 || AHEAD) lds_barrier();
         else __syncthreads();
 
         // step st (buffer phase ph = st % NB, score parity sp = st % 2): loads
@@ -1122,6 +1127,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         bool partial;
         if constexpr (PAGED) partial = cur.part != 0;
         else partial = SPLIT && a_e.n_split > 1;
+        if constexpr (AHEAD) dma_done();
         if (rw.valid) {
             if (partial) {
                 // split partials: (max, sum) and the unnormalised O of this
