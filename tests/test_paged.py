@@ -82,7 +82,7 @@ def attn_args(**kw):
     ({"lens": None}, "null"), ({"cu": None}, "null"), ({"odt": 3}, "dtype"), ({"qdt": 4}, "dtype"), ({"block": 16}, "block"),
     ({"block": 192}, "block"), ({"d": 80}, "head_dim"), ({"nkv": 0}, "n_kv_heads"), ({"nh": 34, "os": 4352, "qs": 4352}, "16 query heads"),
     ({"w": 0}, "max_blocks"), ({"stride": 3}, "max_blocks"), ({"max_len": 0}, "max_len"), ({"max_len": 257}, "max_len"),
-    ({"n": 65536}, "n_seq"), ({"max_new": 6}, "max_new"), ({"qs": 1000}, "stride"), ({"os": 1028}, "stride"),
+    ({"n": 65536}, "n_seq"), ({"nb": 1 << 31}, "too many blocks"), ({"w": 1 << 22, "stride": 1 << 22, "max_len": 1 << 27, "T": 1 << 20, "max_new": 1 << 20, "q": _at(1 << 40)}, "in chunks"), ({"max_new": 6}, "max_new"), ({"qs": 1000}, "stride"), ({"os": 1028}, "stride"),
     ({"gate": _at(0x8000000), "gs": 1000}, "gate_stride"), ({"q": _at(0x2000008)}, "aligned"), ({"out": _at(0x1000004)}, "aligned"),
     ({"kp": _at(0x6000008)}, "aligned"), ({"out": _at(0x2000000)}, "overlaps"), ({"gate": _at(0x1000000 + 4096), "gs": 1024}, "overlaps"),
 ])

@@ -865,7 +865,8 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
         return fail(YHIP_EINVAL, "%s: max_len %u must be in 1..max_blocks * block", fn, max_len);
     if (n_seq > 65535 || n_tok > 0x7fffffffu || max_new > n_tok)
         return fail(YHIP_EINVAL, "%s: n_seq %u, n_tok %u, max_new %u out of range", fn, n_seq, n_tok, max_new);
-    if ((uint64_t)n_blocks * n_kv_heads > 0xffffffffull) return fail(YHIP_EINVAL, "%s: too many blocks", fn);
+    if ((uint64_t)n_blocks * n_kv_heads > 0xffffffffull || (uint64_t)n_seq * n_kv_heads > 0x7fffffffull)
+        return fail(YHIP_EINVAL, "%s: too many blocks or sequences", fn);
     const uint64_t row = (uint64_t)n_heads * head_dim;
     if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8)
         return fail(YHIP_EINVAL, "%s: q_stride/out_stride must be >= n_heads*head_dim and a multiple of 8", fn);

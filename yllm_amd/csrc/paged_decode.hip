@@ -81,6 +81,23 @@ __device__ inline bool decode_next(const PagedAttnArgs& a, PagedCursor& C, Decod
     return true;
 }
 
+// The item of this workgroup where none is cut (short contexts): one each, by
+// its number, without the line; false where the sequence brings no token.
+__device__ inline bool decode_whole(const PagedAttnArgs& a, DecodePiece& I)
+{
+    I.seq = blockIdx.x / a.n_kv;
+    I.kvh = blockIdx.x - I.seq * a.n_kv;
+    const PagedSeq s = cursor_seq(a, I.seq);
+    I.row0 = s.row0;
+    I.nq = s.nq;
+    I.pos0 = s.pos0;
+    I.L = s.L;
+    I.kbeg = 0;
+    I.kend = (uint32_t)s.L;
+    I.part = I.last = 0;
+    return s.nq != 0;
+}
+
 // one 32-key block of K and V as MFMA operands of one lane
 template <int D>
 struct Frag {
@@ -98,9 +115,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
     __shared__ uint32_t s_odd[kWaves];
     _Float16* const s_q = reinterpret_cast<_Float16*>(&s_o[0][0][0]);
 
-    PagedCursor C;
+    PagedCursor C{};
     DecodePiece I;
-    if (!(paged_start<256, DecodeLine>(fresh_args(args), reinterpret_cast<uint64_t*>(&s_o[0][0][0]), C) &&
+    if (args.n_wg == 0) {
+        if (!decode_whole(fresh_args(args), I)) return;  // workgroup-uniform
+    } else if (!(paged_start<256, DecodeLine>(fresh_args(args), reinterpret_cast<uint64_t*>(&s_o[0][0][0]), C) &&
           decode_next(fresh_args(args), C, I))) {
         if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
         return;
@@ -328,6 +347,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
                 }
             }
         }
+        if (fresh_args(args).n_wg == 0) return;
         const uint32_t part = I.part;
         const PagedDesc desc{I.last - C.j + 1, I.row0, I.nq, I.kvh, 0, 0, 0, 0};
         if (!decode_next(fresh_args(args), C, I)) {
@@ -426,17 +446,20 @@ uint32_t snap_units(uint32_t D) { return kWholeBytes / (4 * D * kUnit); }
 
 size_t align256d(size_t x) { return (x + 255) / 256 * 256; }
 
-// workgroups of a launch: what the GPU holds at once, or all that the bounds can fill
+// Chunks of a launch: what the GPU holds at once, or all that the bounds can
+// fill; 0: none is cut.
 uint32_t decode_wgs(uint32_t n_seq, uint32_t max_len, uint32_t n_kv, uint32_t D)
 {
-    const uint64_t items = (uint64_t)n_seq * n_kv, per = (max_len + kUnit - 1) / kUnit + kDecodeItemUnits;
-    const uint64_t most = (max_len + kUnit - 1) / kUnit <= snap_units(D) ? items : items * per;
+    const uint32_t units = (max_len + kUnit - 1) / kUnit;
+    if (units <= snap_units(D)) return 0;  // no item is cut: a workgroup each
+    const uint64_t most = (uint64_t)n_seq * n_kv * (units + kDecodeItemUnits);
     const uint64_t full = (uint64_t)(D <= 128 ? 2 : 1) * (uint64_t)n_cus();
     return (uint32_t)(((most < full ? most : full) + 7) / 8 * 8);
 }
 
 size_t decode_bytes(uint32_t wgs, uint32_t D)
 {
+    if (wgs == 0) return 0;
     const size_t rows = (size_t)2 * wgs * kRows;
     return align256d((size_t)wgs * sizeof(PagedDesc)) + align256d(rows * 2 * sizeof(float)) + rows * D * sizeof(float);
 }
@@ -444,10 +467,11 @@ size_t decode_bytes(uint32_t wgs, uint32_t D)
 template <int D, bool PREC>
 void launch_decode_pieces(const PagedAttnArgs& a, bool stream, hipStream_t st)
 {
+    const dim3 grid(a.n_wg ? a.n_wg : a.n_seq * a.n_kv);
     if (stream)
-        hipLaunchKernelGGL((paged_decode_kernel<D, PREC, 2>), dim3(a.n_wg), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_decode_kernel<D, PREC, 2>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((paged_decode_kernel<D, PREC, 0>), dim3(a.n_wg), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_decode_kernel<D, PREC, 0>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -468,7 +492,6 @@ hipError_t launch_paged_decode(const PagedAttnArgs& in, hipStream_t st)
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
     a.n_wg = decode_wgs(a.n_seq, a.max_len, a.n_kv, a.D);
     a.snap_units = snap_units(a.D);
-    const bool whole = (a.max_len + kUnit - 1) / kUnit <= a.snap_units;  // no item is cut
     a.min_units = 1 + kDecodeItemUnits;
     char* p = reinterpret_cast<char*>(a.ws);
     a.desc = p;
@@ -484,7 +507,7 @@ hipError_t launch_paged_decode(const PagedAttnArgs& in, hipStream_t st)
     case 256: prec ? launch_decode_pieces<256, true>(a, stream, st) : launch_decode_pieces<256, false>(a, stream, st); break;
     default: return hipErrorInvalidValue;
     }
-    if (!whole) {
+    if (a.n_wg) {
         const dim3 grid(a.n_wg, a.gmax * a.max_new);
         switch (a.D) {
         case 64: hipLaunchKernelGGL(paged_decode_merge_kernel<64>, grid, dim3(256), 0, st, a); break;

@@ -156,11 +156,9 @@ def _launch(f, args: tuple, there) -> None:
 
 def _rows(fn: str, name: str, t: torch.Tensor, rows: int, width: int) -> int:
     """The row stride of a [rows, >= width] matrix with unit column stride."""
-    if t.dim() == 2:
-        n, w = t.shape
-        step, one = t.stride()
-        if n == rows and w >= width and (one == 1 or w == 1):
-            return step if n > 1 else w
+    shape, step = t.shape, t.stride()
+    if len(step) == 2 and shape[0] == rows and shape[1] >= width and (step[1] == 1 or shape[1] == 1):
+        return step[0] if rows > 1 else shape[1]
     raise YhipError(-22, f"{fn}: {name} must be [{rows}, >={width}] rows with unit column stride")
 
 
@@ -208,10 +206,10 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
         sp = slots.data_ptr()
     norm = F32
     if q_norm is not None or k_norm is not None:
-        for w in (q_norm, k_norm):
-            if w is None or w.shape != (d,) or not w.is_contiguous() or w.dtype is not q_norm.dtype \
-                    or w.dtype not in (torch.float32, _F16):
-                raise YhipError(-22, f"{fn}: q_norm and k_norm must both be [{d}], f32 or f16")
+        if q_norm is None or k_norm is None or q_norm.shape != (d,) or k_norm.shape != (d,) \
+                or not q_norm.is_contiguous() or not k_norm.is_contiguous() or k_norm.dtype is not q_norm.dtype \
+                or q_norm.dtype not in (torch.float32, _F16):
+            raise YhipError(-22, f"{fn}: q_norm and k_norm must both be [{d}], f32 or f16")
         norm = _DT[q_norm.dtype]
         wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
     kc, vc = cache.k, cache.v
