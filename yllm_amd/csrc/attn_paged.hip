@@ -22,9 +22,10 @@ namespace {
 
 constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
 
-// Workgroup (j, y): the y-th kMergeRows * 256 / (D / 4) rows of the split item
-// that chunk j begins, if any.  Pieces are joined in their order; a thread
-// holds four dimensions of its rows.  Nearly all split items have two pieces:
+// Workgroup (j, y): the y-th 256 / (D / 4) rows of the split item that chunk j
+// begins, if any.  Pieces are joined in their order; a thread holds four
+// dimensions of a row.  Nearly all split items of a full launch have two
+// pieces: there every kMergeRows-th workgroup takes the rows of as many, and
 // their loads, and the gate's, go out together (one row after the other, 16
 // dependent round trips: a gated chunk of 2048 tokens, 16 / 2 heads of 256,
 // merged in 22 us; so, in 19, 6 TB/s).
@@ -36,7 +37,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
     const uint32_t j = blockIdx.x;
     const PagedDesc d = reinterpret_cast<const PagedDesc*>(a.desc)[j];
     if (d.n == 0) return;
-    const uint32_t dim = threadIdx.x % C4 * 4u, r0 = blockIdx.y * (kMergeRows * RP) + threadIdx.x / C4;
+    const uint32_t dim = threadIdx.x % C4 * 4u, r0 = blockIdx.y * RP + threadIdx.x / C4;
+    if (d.n == 2 && blockIdx.y % kMergeRows != 0) return;
     auto finish = [&](const PagedRow& rw, f32x4 O, float L, const f32x4& g) {
         f32x4 v = O * (L == 0.0f ? 0.0f : 1.0f / L);
         if (a.gate) {
@@ -73,8 +75,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
         }
         return;
     }
-    for (uint32_t i = 0; i < kMergeRows; ++i) {
-        const uint32_t r = r0 + i * RP;
+    {
+        const uint32_t r = r0;
         const PagedRow rw = paged_row(a, d, r);
         if (!rw.valid) return;
         float M = -1e30f, L = 0.0f;
@@ -116,8 +118,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
 
 namespace {
 
-// The shortest chunk, and the longest item that is not cut, in units of 64 keys.
-constexpr uint32_t kMinUnits = 4, kSnapUnits = 4;
+// The shortest chunk, and the longest item that is not cut (without its fixed
+// units), in units of 64 keys.
+constexpr uint32_t kMinUnits = kItemUnits + 1, kSnapUnits = 4;
 
 uint32_t round8(uint64_t x) { return (uint32_t)((x + 7) / 8 * 8); }
 
@@ -127,7 +130,8 @@ uint32_t paged_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_
 {
     const uint64_t gmax = (n_heads + n_kv - 1) / n_kv;
     const uint64_t items = (uint64_t)n_kv * gmax * ((uint64_t)n_tok / kItemRows + n_seq);
-    const uint64_t most = items * ((max_len + kUnitKeys - 1) / kUnitKeys) / kMinUnits + 1;
+    const uint64_t units = ((uint64_t)max_len + kUnitKeys - 1) / kUnitKeys + kItemUnits;
+    const uint64_t most = (items * units + kMinUnits - 1) / kMinUnits;
     const uint64_t full = (uint64_t)per_cu * (uint64_t)n_cus();
     return round8(most < full ? most : full);
 }
@@ -182,7 +186,7 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
     default: return hipErrorInvalidValue;
     }
     if ((a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
-        const uint32_t rp = kMergeRows * 1024u / a.D;  // rows of a merge workgroup
+        const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
         const dim3 grid(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
         switch (a.D) {
         case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, st, a); break;

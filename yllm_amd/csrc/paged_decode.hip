@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
 #pragma unroll
         for (int r = 0; r < D / 64; ++r) {
             const uint32_t idx = threadIdx.x + r * 256u, hn = idx / D4, d = idx % D4 * 4u, hr = hn < rows ? hn : 0u;
-            const uint32_t t = hr / G;
+            const uint32_t t = div_small(hr, G);
             const size_t at = (size_t)(I.row0 + t) * a.q_stride + (size_t)(h0 + hr - t * G) * D + d;
             if (PREC) {
                 qv[r] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.q) + at);
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
         }
 
         // row n sees keys below lim; keys from `cut` on are not seen by every row
-        const int lim = min(I.pos0 + (int)((uint32_t)n < rows ? (uint32_t)n / G : 0u) + 1, I.L);
+        const int lim = min(I.pos0 + (int)((uint32_t)n < rows ? div_small((uint32_t)n, G) : 0u) + 1, I.L);
         const int cut = min(I.pos0 + 1, I.L);
         float m = -1e30f, l = 0.0f;
         bool odd = false;  // an inf or NaN was cleared
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
                 O += ow[w] * c;
                 L += lw[w] * c;
             }
-            const uint32_t t = hn / G, h = h0 + hn - t * G;
+            const uint32_t t = div_small(hn, G), h = h0 + hn - t * G;
             if (I.part == 0) O *= L == 0.0f ? 0.0f : 1.0f / L;
             if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) {
 #pragma unroll 1

@@ -30,8 +30,19 @@ __device__ inline uint64_t uni64(uint64_t x) { return (uint64_t)uni((uint32_t)(x
 typedef const int __attribute__((address_space(4))) * ConstInts;
 __device__ inline ConstInts const_ints(const int* p) { return (ConstInts)(uintptr_t)p; }
 
+// a / b for a below 2^21: the quotient with a + 1/2 is at least 1/(2 b) off
+// every whole number, more than the reciprocal's error makes (five
+// instructions for some thirty-five)
+__device__ inline uint32_t div_small(uint32_t a, uint32_t b)
+{
+    return (uint32_t)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b));
+}
+
 // first query head of kv head g (common mapping h * n_kv / n_heads)
-__device__ inline uint32_t head0(const PagedAttnArgs& a, uint32_t g) { return (g * a.n_heads + a.n_kv - 1) / a.n_kv; }
+__device__ inline uint32_t head0(const PagedAttnArgs& a, uint32_t g)
+{
+    return a.gmax * a.n_kv == a.n_heads ? g * a.gmax : (g * a.n_heads + a.n_kv - 1) / a.n_kv;
+}
 
 // A sequence's rows and keys: rows row0 .. row0 + nq - 1, token t at position
 // pos0 + t (negative: sees nothing), L keys.
@@ -121,13 +132,37 @@ __device__ inline const PagedAttnArgs& fresh_args(const PagedAttnArgs&)
     return *(const PagedAttnArgs*)p;
 }
 
-// This workgroup's place in the line; false if it has no chunk.  Active chunks
-// are spread over the XCDs (consecutive workgroups go to the 8 XCDs in turn),
-// neighbours on one XCD, whose L2 then holds the keys they share.  `scratch`:
-// 24 words of LDS, free again after the call's last barrier.
+// This workgroup's chunk, units begin .. of a line of `total`; false if it has
+// none.  Active chunks are spread over the XCDs (consecutive workgroups go to
+// the 8 XCDs in turn), neighbours on one XCD, whose L2 then holds the keys they
+// share.
+__device__ inline bool paged_chunk(const PagedAttnArgs& a, PagedCursor& C, uint64_t total, uint64_t& begin)
+{
+    const uint64_t even = (total >> 32) ? (total + a.n_wg - 1) / a.n_wg : ((uint32_t)total + a.n_wg - 1) / a.n_wg;
+    C.chunk = (uint32_t)max(even, (uint64_t)a.min_units);
+    const uint32_t active = (total >> 32) ? (uint32_t)((total + C.chunk - 1) / C.chunk)
+                                          : ((uint32_t)total + C.chunk - 1) / C.chunk;
+    const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
+    C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
+    begin = (uint64_t)C.j * C.chunk;
+    C.done = 0;
+    C.len = (int)min((uint64_t)C.chunk, total - begin);
+    C.fresh = true;
+    return C.j < active;
+}
+
+// This workgroup's place in the line; false if it has no chunk.  `scratch`: 24
+// words of LDS, free again after the call's last barrier.
 template <int NT, class Line = PagedLine>
 __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C)
 {
+    if (a.n_seq == 1) {  // nothing to scan
+        C.seq = 0;
+        uint64_t begin;
+        const bool any = paged_chunk(a, C, Line::units(a, cursor_seq(a, 0)), begin);
+        C.off = (uint32_t)begin;
+        return any;
+    }
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const bool small = a.n_seq <= 64u;  // every wave scans for itself
     const uint32_t per = small ? 1u : (a.n_seq + NT - 1) / NT;
@@ -152,17 +187,8 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
         }
         total = uni64(total);
     }
-    const uint64_t even = (total >> 32) ? (total + a.n_wg - 1) / a.n_wg : ((uint32_t)total + a.n_wg - 1) / a.n_wg;
-    C.chunk = (uint32_t)max(even, (uint64_t)a.min_units);
-    const uint32_t active = (total >> 32) ? (uint32_t)((total + C.chunk - 1) / C.chunk)
-                                          : ((uint32_t)total + C.chunk - 1) / C.chunk;
-    const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
-    C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
-    const uint64_t begin = (uint64_t)C.j * C.chunk;
-    if (C.j >= active) return false;  // workgroup-uniform
-    C.done = 0;
-    C.len = (int)min((uint64_t)C.chunk, total - begin);
-    C.fresh = true;
+    uint64_t begin;
+    if (!paged_chunk(a, C, total, begin)) return false;  // workgroup-uniform
     const bool mine = before <= begin && begin < before + sum;
     if (small) {
         const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(mine));

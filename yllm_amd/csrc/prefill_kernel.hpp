@@ -275,7 +275,7 @@ __device__ inline PagedRow paged_row(const PagedAttnArgs& a, const I& it, uint32
         return PagedRow{it.row0 + t, it.h, t, rr < it.nq};
     }
     const uint32_t h0 = head0(a, it.kvh), nrows = (head0(a, it.kvh + 1) - h0) * it.nq;
-    const uint32_t rc = min(rr, nrows - 1), g = rc / it.nq, t = rc - g * it.nq;
+    const uint32_t rc = min(rr, nrows - 1), g = div_small(rc, it.nq), t = rc - g * it.nq;
     return PagedRow{it.row0 + t, h0 + g, t, rr < nrows};
 }
 __device__ inline bool paged_span(const PagedAttnArgs& a, const PagedItem& I, int wave, uint32_t& first, uint32_t& last)
@@ -286,12 +286,15 @@ __device__ inline bool paged_span(const PagedAttnArgs& a, const PagedItem& I, in
     if (!I.pack) {
         first = r0;
         last = rl;
-    } else if (r0 / I.nq == rl / I.nq) {
-        first = r0 % I.nq;
-        last = rl % I.nq;
-    } else {  // the rows cross into the next head
-        first = 0;
-        last = I.nq - 1;
+    } else {
+        const uint32_t g = div_small(r0, I.nq);
+        if (g == div_small(rl, I.nq)) {
+            first = r0 - g * I.nq;
+            last = rl - g * I.nq;
+        } else {  // the rows cross into the next head
+            first = 0;
+            last = I.nq - 1;
+        }
     }
     return r0 < nrows && !I.idle;
 }
