@@ -248,11 +248,12 @@ int yhip_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride,
  *                blocks missing
  * A sequence that does not get all it needs is not served: none of its table
  * entries is set, its kv_lens is 0 and its rows have slot -1 (so nothing of it
- * is stored and its attention rows are zero).  That is one whose blocks,
- * counted after those of all earlier sequences, pass the free ones or its
- * table row, whose rows pass n_tok, or with a negative length.  The caller
- * takes counts[0] as the next *n_free (outputs must not overlap inputs).  A
- * value past 31 bits is reported as 2^31 - 1.
+ * is stored and its attention rows are zero).  That is one with a negative
+ * length or more blocks than its table row has entries (of these no blocks are
+ * counted), whose blocks, counted after those of all earlier sequences, pass
+ * the free ones, or whose rows pass n_tok.  The caller takes counts[0] as the
+ * next *n_free (outputs must not overlap inputs).  A value past 31 bits is
+ * reported as 2^31 - 1.
  * block is a power of two in 64..65536, n_seq at most 8192. */
 int yhip_paged_plan(int32_t* block_table, uint32_t max_blocks, uint32_t table_stride, const int32_t* ctx_lens,
                     const int32_t* new_lens, const int32_t* free_blocks, uint32_t free_cap, const int32_t* n_free,

@@ -35,8 +35,9 @@ def plan_oracle(table, ctx, new, free, n_free, block, n_tok):
         rows, ok = max(new[i], 0), ctx[i] >= 0 and new[i] >= 0
         c = max(ctx[i], 0)
         held = -(-c // block)
+        ok = ok and -(-(c + rows) // block) <= width  # (of those that can never be served no blocks are counted)
         need = -(-(c + rows) // block) - held if ok else 0
-        ok = ok and held + need <= width and (need == 0 or taken + need <= nf) and cu[-1] + rows <= n_tok
+        ok = ok and (need == 0 or taken + need <= nf) and cu[-1] + rows <= n_tok
         if ok:
             for t in range(need):
                 table[i][held + t] = free[nf - 1 - taken - t]
@@ -116,6 +117,28 @@ def test_plan_narrow_table_bad_lengths_and_few_rows(cuda):
     _check_plan([7, 9], [0, 0], 64, 2, 9, n_tok=0)
     _check_plan([0x7fffffff, 3], [0x7fffffff, 2], 64, 2, 9, n_tok=4)
     _check_plan([], [], 64, 2, 2, n_tok=3)
+
+
+@pytest.mark.parametrize("width", [2, 3, 5])
+@pytest.mark.parametrize("n_free", [0, 5, 40, 90])
+def test_plan_hands_out_no_block_twice(cuda, width, n_free):
+    """What is left on the free list is no one's, whichever sequences were refused: a step's blocks are its last."""
+    g = torch.Generator().manual_seed(width * 100 + n_free)
+    n = 70
+    ctx = [int(x) for x in torch.randint(-20, 200, (n,), generator=g)]
+    new = [int(x) for x in torch.randint(-2, 260, (n,), generator=g)]
+    ctx = [min(c, width * 64) for c in ctx]
+    table, free, T = _plan_case(ctx, new, 64, width, n_free, seed=n_free)
+    for n_tok in (T, T // 2):
+        from yllm_amd.paged import paged_plan
+
+        dev = _i32(table)
+        step = paged_plan(dev, _i32(ctx), _i32(new), _i32(free), _i32([n_free]), 64, n_tok)
+        left = set(free[:int(step.counts[0])])
+        held = [e for r, L in zip(dev.tolist(), step.kv_lens.tolist()) for e in r[:-(-L // 64)]]
+        assert len(held) == len(set(held)) and not left & set(held)
+        new_ones = sum(a != b for r, s in zip(dev.tolist(), table) for a, b in zip(r, s))
+        assert len(left) + new_ones == n_free
 
 
 def test_plan_many_sequences(cuda):

@@ -28,7 +28,10 @@ constexpr uint32_t kTop = 0x7fffffffu;
 __device__ inline uint32_t blocks_of(uint32_t n, uint32_t shift) { return (n >> shift) + ((n & ((1u << shift) - 1u)) != 0); }
 
 // One sequence's lengths as the plan takes them: a negative new length is
-// zero rows, and a negative context (never served) counts no blocks.
+// zero rows, and one that cannot be served whatever comes before it (a negative
+// length, more blocks than its table row has entries) counts no blocks.  So the
+// blocks of those served are the free list's last: behind the first that is
+// refused for blocks or rows none is served that needs any.
 struct SeqLen {
     uint32_t ctx, rows, held, need;
     bool ok;
@@ -41,7 +44,9 @@ __device__ inline SeqLen seq_len(const PagedPlanArgs& a, uint32_t i)
     s.ctx = c > 0 ? (uint32_t)c : 0u;
     s.rows = n > 0 ? (uint32_t)n : 0u;
     s.held = blocks_of(s.ctx, a.shift);
-    s.need = s.ok ? blocks_of(s.ctx + s.rows, a.shift) - s.held : 0u;
+    const uint32_t all = blocks_of(s.ctx + s.rows, a.shift);
+    s.ok = s.ok && all <= a.width;
+    s.need = s.ok ? all - s.held : 0u;
     return s;
 }
 
@@ -49,8 +54,7 @@ __device__ inline SeqLen seq_len(const PagedPlanArgs& a, uint32_t i)
 __device__ inline bool served(const PagedPlanArgs& a, const SeqLen& s, uint64_t need_before, uint64_t rows_before,
                               uint32_t n_free)
 {
-    return s.ok && (uint64_t)s.held + s.need <= a.width && (s.need == 0 || need_before + s.need <= n_free) &&
-           rows_before + s.rows <= a.n_tok;
+    return s.ok && (s.need == 0 || need_before + s.need <= n_free) && rows_before + s.rows <= a.n_tok;
 }
 
 __device__ inline uint32_t clamp31(uint64_t x) { return x < kTop ? (uint32_t)x : kTop; }
