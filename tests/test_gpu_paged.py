@@ -610,6 +610,104 @@ def test_attn_on_another_stream(cuda):
     torch.cuda.current_stream().wait_stream(st)
 
 
+def test_attn_more_new_tokens_than_the_bound(cuda):
+    """A sequence with more than max_new new tokens: the first max_new rows are computed, the rest left as they were."""
+    for seqs, cut in (([(90, 5), (200, 2)], 2), ([(300, 200), (64, 3)], 150), ([(300, 200), (64, 3)], 60)):
+        b = Batch(seqs, 8, 2, 128, seed=21)
+        whole, out = b.check(), torch.full((b.T, 8 * 128), 5.0, dtype=F16, device="cuda")
+        b.run(max_new=cut, out=out)
+        want, tol = b.exact()
+        for i, (_, n) in enumerate(seqs):
+            at = slice(b.cu[i], b.cu[i] + min(n, cut))
+            assert ((out[at].double() - want[at]).abs() <= tol[at] + U[F16] * want[at].abs() + 2.0 ** -24).all()
+            assert (out[b.cu[i] + min(n, cut):b.cu[i + 1]] == 5).all()
+        assert torch.equal(b.run(), whole)
+
+
+def test_attn_captured_chunks_replay_with_new_lengths(cuda):
+    """A captured call with prompt chunks follows the lengths, offsets and tables that it finds when it runs."""
+    from yllm_amd.paged import paged_attn, paged_attn_workspace
+
+    steps = [Batch(s, 28, 4, 128, seed=30 + i) for i, s in enumerate(
+        ([(700, 200), (90, 1), (3000, 33)], [(1, 1), (0, 0), (233, 233)], [(5000, 1), (64, 64), (129, 128)],
+         [(2, 2), (1, 1), (1, 1)], [(400, 100), (2000, 130), (77, 4)]))]
+    T, w, nb = max(b.T for b in steps), max(b.table.shape[1] for b in steps), max(b.cache.n_blocks for b in steps)
+    k, v = (torch.zeros((nb, *x.shape[1:]), dtype=F16, device="cuda") for x in (steps[0].cache.k, steps[0].cache.v))
+    pool = type(steps[0].cache)(k, v)
+    q, out = torch.zeros((T, 28 * 128), dtype=F16, device="cuda"), torch.empty((T, 28 * 128), dtype=F16, device="cuda")
+    table, lens, cu = torch.zeros((3, w), dtype=torch.int32, device="cuda"), _i32([1, 1, 1]), _i32([0, 1, 2, 3])
+    ws = paged_attn_workspace(T, 3, 233, 5000, 28, 4, 128)
+    paged_attn(q, pool, table, lens, cu, 28, 233, 5000, out=out, workspace=ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_attn(q, pool, table, lens, cu, 28, 233, 5000, out=out, workspace=ws)
+    for b in steps * 2:
+        q[:b.T], out[:] = b.q, 5.0
+        pool.k[:b.cache.n_blocks], pool.v[:b.cache.n_blocks] = b.cache.k, b.cache.v
+        table[:, :b.table.shape[1]] = b.table
+        lens.copy_(_i32([L for L, _ in b.seqs])), cu.copy_(_i32(b.cu))
+        graph.replay()
+        want, tol = b.exact()
+        err = (out[:b.T].double() - want).abs()
+        assert (err <= tol + U[F16] * want.abs() + 2.0 ** -24).all() and (out[b.T:] == 5).all()
+
+
+def test_attn_calls_on_two_streams_at_once(cuda):
+    """Each with its own workspace."""
+    from yllm_amd.paged import paged_attn_workspace
+
+    batches = [Batch([(3000, 1), (700, 200)], 28, 4, 128, seed=40), Batch([(9000, 1), (50, 1)], 16, 2, 256, seed=41)]
+    want = [b.check() for b in batches]
+    spaces = [paged_attn_workspace(b.T, 2, b.max_new, b.max_len, b.nh, b.nkv, b.d) for b in batches]
+    streams, got = [torch.cuda.Stream() for _ in batches], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for st, b, ws, o in zip(streams, batches, spaces, got):
+            with torch.cuda.stream(st):
+                o.append(b.run(workspace=ws))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+def test_store_into_a_pool_past_4_gib(cuda):
+    from yllm_amd.attention import ROPE_NONE
+    from yllm_amd.paged import PagedKV, qk_norm_rope_kv_store
+
+    nkv, d, block = 8, 128, 256
+    nb = (5 << 30) // (nkv * d * block * 2)  # 5 GiB of K
+    big = PagedKV(torch.empty((nb, nkv, block, d), dtype=F16, device="cuda"),
+                  torch.empty((nb, nkv, block // 32, d, 32), dtype=F16, device="cuda"))
+    for T in (3, 200):  # single rows, and groups of rows
+        first = (nb - 2) * block + 17
+        big.k[-2:], big.v[-2:] = 3.0, 3.0
+        kv = torch.randn((2, T, nkv * d), generator=_gen(T), device="cuda").half()
+        qk_norm_rope_kv_store(big, None, kv[0], kv[1], nkv, ROPE_NONE, 1.0, positions=_i32(list(range(T))),
+                              slots=_i32(list(range(first, first + T))))
+        K = big.k[-2:].transpose(1, 2).reshape(-1, nkv * d)
+        V = big.v[-2:].permute(0, 2, 4, 1, 3).reshape(-1, nkv * d)
+        for got, want in ((K, kv[0]), (V, kv[1])):
+            assert torch.equal(got[17:17 + T], want) and (got[:17] == 3).all() and (got[17 + T:] == 3).all()
+
+
+def test_calls_without_rows_and_single_rows_of_odd_strides(cuda):
+    from yllm_amd.paged import paged_attn, qk_norm_rope_kv_store
+
+    b = Batch([(70, 1)], 8, 2, 128, seed=50)
+    none = torch.empty((0, 256), dtype=F16, device="cuda")
+    empty = _i32([])
+    assert qk_norm_rope_kv_store(b.cache, torch.empty((0, 1024), dtype=F16, device="cuda"), none, none, 8, 2, 1e6,
+                                 positions=empty, slots=empty).shape == (0, 1024)
+    q = torch.empty((0, 1024), dtype=F16, device="cuda")
+    assert paged_attn(q, b.cache, b.table, _i32([70]), _i32([0, 0]), 8, 1, 70).shape == (0, 1024)
+    assert paged_attn(q, b.cache, b.table[:0], empty, _i32([0]), 8, 1, 70).shape == (0, 1024)
+    wide = torch.zeros((1, 1024 + 13), dtype=F16, device="cuda")  # the next row would not be aligned
+    wide[:, :1024] = b.q
+    want = b.check()
+    b.q = wide[:, :1024]
+    assert torch.equal(b.run(), want)
+
+
 # ---- a step, and steps in a row ------------------------------------------------------------------------
 
 class Serve:

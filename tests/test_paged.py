@@ -67,6 +67,19 @@ def test_store_refusals(hiplib, kw, msg):
 
 def test_store_of_nothing(hiplib):
     assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(T=0)) == 0
+    assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(T=0, qo=None, q=None, k=None, v=None, pos=None, slots=None)) == 0
+
+
+def test_positions_past_31_bits(hiplib):
+    """Rows with slots and no positions count from pos_start."""
+    assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(pos=None, start=0x7ffffffc)) == -22 and "31 bits" in _err(hiplib)
+    assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(pos=None, start=0xffffffff)) == -22 and "31 bits" in _err(hiplib)
+
+
+def test_attn_of_too_much_in_all(hiplib):
+    """Each sequence fits a call, all of them do not."""
+    big = dict(n=65535, T=65535, max_new=1, max_len=0x7fffffff, w=32768, stride=32768, block=65536, q=_at(1 << 40))
+    assert hiplib.yhip_paged_attn(*attn_args(**big)) == -22 and "in chunks" in _err(hiplib)
 
 
 def attn_args(**kw):
@@ -91,7 +104,8 @@ def test_attn_refusals(hiplib, kw, msg):
 
 
 def test_attn_of_nothing(hiplib):
-    for kw in ({"T": 0, "max_new": 0}, {"n": 0}, {"max_new": 0}):
+    null = dict(out=None, q=None, kp=None, vp=None, table=None, lens=None)
+    for kw in ({"T": 0, "max_new": 0}, {"n": 0}, {"max_new": 0}, {"T": 0, "max_new": 0, **null}, {"n": 0, **null}):
         assert hiplib.yhip_paged_attn(*attn_args(**kw)) == 0
 
 
@@ -110,7 +124,11 @@ def test_python_refusals():
     i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
     kv = PG.PagedKV.empty(4, 2, 128, device="cpu")
     assert (kv.n_blocks, kv.n_kv, kv.block, kv.head_dim) == (4, 2, 64, 128)
+    flat = PG.PagedKV(kv.k, kv.k.clone())  # V in rows, as K
     bad = [lambda: PG.PagedKV.empty(4, 2, 128, block=48, device="cpu"),
+           lambda: PG.PagedKV.empty(1, 1, 64, block=1 << 17, device="cpu"),
+           lambda: PG.paged_attn(torch.zeros(5, 1024), flat, i(3, 4), i(3), i(4), 8, 2),
+           lambda: PG.qk_norm_rope_kv_store(flat, None, torch.zeros(5, 256), torch.zeros(5, 256), 8, 2, 1e6),
            lambda: PG.paged_plan(i(3, 4), i(3), i(3), i(9), i(1), 64, 9),                   # on the CPU
            lambda: PG.paged_plan(i(3, 4).t(), i(4), i(4), i(9), i(1), 64, 9),
            lambda: PG.paged_plan(i(3, 4).long(), i(3), i(3), i(9), i(1), 64, 9),

@@ -759,7 +759,7 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
     // (one kv head's page takes the place of its contiguous cache)
     if (block == 0 || block % 64) return fail(YHIP_EINVAL, "%s: block %u must be a positive multiple of 64", fn, block);
     if (int rc = check_heads(fn, n_heads, n_kv_heads, head_dim, block)) return rc;
-    if (!k || !v || !kpool || !vpool || (q_out && !q)) return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    if (n_tok && (!k || !v || !kpool || !vpool || (q_out && !q))) return fail(YHIP_EINVAL, "%s: null pointer", fn);
     if (!q_norm != !k_norm) return fail(YHIP_EINVAL, "%s: q_norm and k_norm come together", fn);
     if (!valid_dtype(dtype) || (q_out && !valid_dtype(q_out_dtype))) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
     if (q_norm && norm_dtype != YHIP_F32 && norm_dtype != YHIP_F16)
@@ -776,6 +776,8 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
         return fail(YHIP_EINVAL, "%s: %u blocks of %u positions pass 31 bits", fn, n_blocks, block);
     if (!slots && (positions || (uint64_t)pos_start + n_tok > (uint64_t)n_blocks * block))
         return fail(YHIP_EINVAL, "%s: without slots, rows are the positions %u.. and must fit the pool", fn, pos_start);
+    if (!positions && (uint64_t)pos_start + n_tok > 0x80000000ull)
+        return fail(YHIP_EINVAL, "%s: positions %u.. pass 31 bits", fn, pos_start);
     if (n_tok > 0x7fffffffu || (uint64_t)n_tok * n_heads > 0x7fffffffull)
         return fail(YHIP_EINVAL, "%s: too many rows", fn);
     // runs of four elements move as one access
@@ -853,7 +855,7 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
                     uint32_t gate_stride, void* workspace, size_t workspace_bytes, void* stream)
 {
     const char* fn = "yhip_paged_attn";
-    if (!att_out || !q || !kpool || !vpool || !block_table || !kv_lens || !cu_new)
+    if (n_tok && n_seq && (!att_out || !q || !kpool || !vpool || !block_table || !kv_lens || !cu_new))
         return fail(YHIP_EINVAL, "%s: null pointer", fn);
     if (!valid_dtype(out_dtype) || !valid_dtype(q_dtype)) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
     uint32_t shift;
@@ -863,7 +865,7 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
         return fail(YHIP_EINVAL, "%s: need 1 <= max_blocks (%u) <= table_stride (%u)", fn, max_blocks, table_stride);
     if (max_len == 0 || max_len > (uint64_t)max_blocks * block || max_len > 0x7fffffffu)
         return fail(YHIP_EINVAL, "%s: max_len %u must be in 1..max_blocks * block", fn, max_len);
-    if (n_seq > 65535 || n_tok > 0x7fffffffu || max_new > n_tok)
+    if (n_seq > 65535 || n_tok > 0x7fffffffu || (n_tok && max_new > n_tok))
         return fail(YHIP_EINVAL, "%s: n_seq %u, n_tok %u, max_new %u out of range", fn, n_seq, n_tok, max_new);
     if ((uint64_t)n_blocks * n_kv_heads > 0xffffffffull || (uint64_t)n_seq * n_kv_heads > 0x7fffffffull)
         return fail(YHIP_EINVAL, "%s: too many blocks or sequences", fn);
@@ -880,7 +882,9 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
         return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
     // tiles of 64 keys that the largest sequence's 128-row items walk
     const uint64_t nb = (max_new + 127) / 128, tiles = max_len / 64 + 1, gmax = (n_heads + n_kv_heads - 1) / n_kv_heads;
-    if ((nb * (tiles + nb + 8) + tiles) * gmax * n_kv_heads >= 1ull << 31)
+    // (and all of them: a workgroup's chunk of the line stays below 2^31 units)
+    const uint64_t items = (n_tok / 128 + (uint64_t)n_seq) * gmax * n_kv_heads;
+    if ((nb * (tiles + nb + 8) + tiles) * gmax * n_kv_heads >= 1ull << 31 || items * (tiles + 8) >= 1ull << 38)
         return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
                     max_new, max_len);
     const size_t need = yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);

@@ -57,8 +57,8 @@ class PagedKV:
     @classmethod
     def empty(cls, n_blocks: int, n_kv: int, head_dim: int, block: int = 64, device: str | torch.device = "cuda",
               zero: bool = True) -> "PagedKV":
-        if block < 64 or block & (block - 1):
-            raise YhipError(-22, f"PagedKV: block {block} must be a power of two of at least 64")
+        if not 64 <= block <= 65536 or block & (block - 1):
+            raise YhipError(-22, f"PagedKV: block {block} must be a power of two in 64..65536")
         alloc = torch.zeros if zero else torch.empty
         k = alloc((n_blocks, n_kv, block, head_dim), dtype=torch.float16, device=device)
         v = alloc((n_blocks, n_kv, block // 32, head_dim, 32), dtype=torch.float16, device=device)
@@ -75,8 +75,8 @@ def _pool(cache: PagedKV | LayerKV, fn: str) -> tuple[int, int, int, int]:
     if len(shape) == 3:
         shape = (1, *shape)
     if len(shape) != 4 or k.dtype is not _F16 or v.dtype is not _F16 or not k.is_contiguous() \
-            or not v.is_contiguous() or v.numel() != k.numel():
-        raise YhipError(-22, f"{fn}: the cache must hold contiguous f16 K and V of one size")
+            or not v.is_contiguous() or v.numel() != k.numel() or v.shape[-2:] != (shape[3], 32):
+        raise YhipError(-22, f"{fn}: the cache must hold contiguous f16 K and V of one size, V in tiles of 32 positions")
     return shape
 
 
@@ -158,7 +158,7 @@ def _rows(fn: str, name: str, t: torch.Tensor, rows: int, width: int) -> int:
     """The row stride of a [rows, >= width] matrix with unit column stride."""
     shape, step = t.shape, t.stride()
     if len(step) == 2 and shape[0] == rows and shape[1] >= width and (step[1] == 1 or shape[1] == 1):
-        return step[0] if rows > 1 else shape[1]
+        return step[0] if rows > 1 else width
     raise YhipError(-22, f"{fn}: {name} must be [{rows}, >={width}] rows with unit column stride")
 
 
