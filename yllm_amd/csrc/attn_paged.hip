@@ -118,20 +118,31 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
 
 namespace {
 
-// The shortest chunk, and the longest item that is not cut (without its fixed
-// units), in units of 64 keys.
-constexpr uint32_t kMinUnits = kItemUnits + 1, kSnapUnits = 4;
+// The longest item that is not cut (without its fixed units), and the shortest
+// chunk, in units of 64 keys.  Where a line does not fill the GPU, a piece more
+// of an item of T units costs its merge 0.4 us, and a unit more of a piece its
+// walk 1.2: pieces of sqrt(T / 3) units (28 / 4 heads of 128, 16 tokens at 1000:
+// 19 us, 25 with pieces of nine; 14 / 2 heads of 64, 64 tokens at 16000: 26, 34
+// with pieces of four).
+constexpr uint32_t kSnapUnits = 4, kMinUnits = 4;
+uint32_t min_units(uint32_t max_len)
+{
+    const uint32_t T = (max_len - 1) / kUnitKeys + 1 + kItemUnits;
+    return std::max(kMinUnits, (uint32_t)lroundf(sqrtf((float)T / 3.0f)));
+}
 
 uint32_t round8(uint64_t x) { return (uint32_t)((x + 7) / 8 * 8); }
 
 // Workgroups of a launch: what the GPU holds at once (per_cu a CU), or all that
-// the bounds on the batch can fill.
-uint32_t paged_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t per_cu)
+// the bounds on the batch can fill with chunks of `shortest` units.  (A workspace
+// is sized for the shortest there are: larger bounds never need less.)
+uint32_t paged_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t per_cu,
+                   uint32_t shortest)
 {
     const uint64_t gmax = (n_heads + n_kv - 1) / n_kv;
     const uint64_t items = (uint64_t)n_kv * gmax * ((uint64_t)n_tok / kItemRows + n_seq);
     const uint64_t units = ((uint64_t)max_len + kUnitKeys - 1) / kUnitKeys + kItemUnits;
-    const uint64_t most = (items * units + kMinUnits - 1) / kMinUnits;
+    const uint64_t most = (items * units + shortest - 1) / shortest;
     const uint64_t full = (uint64_t)per_cu * (uint64_t)n_cus();
     return round8(most < full ? most : full);
 }
@@ -159,7 +170,7 @@ size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, ui
     // (the decode kernel's, where it serves every call within the bounds; else also large enough for its calls)
     const size_t decode = paged_decode_workspace(n_seq, max_len, n_kv, D);
     if (paged_decode_fits(n_heads, n_kv, max_new)) return decode;
-    return std::max(decode, paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1), D));
+    return std::max(decode, paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1, kMinUnits), D));
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
@@ -168,8 +179,8 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
     PagedAttnArgs a = in;
     const bool qs = a.q_dtype == kF32;
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
-    a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, a.D <= 128 && !qs ? 2 : 1);
-    a.min_units = kMinUnits;
+    a.min_units = min_units(a.max_len);
+    a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, a.D <= 128 && !qs ? 2 : 1, a.min_units);
     a.snap_units = kSnapUnits;
     char* p = reinterpret_cast<char*>(a.ws);
     a.desc = p;
