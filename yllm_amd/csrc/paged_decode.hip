@@ -22,6 +22,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace yhip {
 namespace {
 
@@ -54,6 +56,9 @@ struct DecodePiece {
     int pos0, L;
 };
 
+// the keys that the sequence's last row sees (all, but for tokens left out past max_new)
+__device__ inline int seen_keys(const PagedSeq& s) { return max(min(s.L, s.pos0 + (int)s.nq), 0); }
+
 __device__ inline bool decode_next(const PagedAttnArgs& a, PagedCursor& C, DecodePiece& I)
 {
     if (C.done >= C.len) return false;
@@ -74,10 +79,10 @@ __device__ inline bool decode_next(const PagedAttnArgs& a, PagedCursor& C, Decod
     I.nq = s.nq;
     I.kvh = kvh;
     I.pos0 = s.pos0;
-    I.L = s.L;
+    I.L = seen_keys(s);
     const uint32_t u0 = t ? t - kDecodeItemUnits : 0u, u1 = t + n - kDecodeItemUnits;
-    I.kbeg = min(u0 * kUnit, (uint32_t)s.L);
-    I.kend = min(u1 * kUnit, (uint32_t)s.L);
+    I.kbeg = min(u0 * kUnit, (uint32_t)I.L);
+    I.kend = min(u1 * kUnit, (uint32_t)I.L);
     return true;
 }
 
@@ -91,9 +96,9 @@ __device__ inline bool decode_whole(const PagedAttnArgs& a, DecodePiece& I)
     I.row0 = s.row0;
     I.nq = s.nq;
     I.pos0 = s.pos0;
-    I.L = s.L;
+    I.L = seen_keys(s);
     I.kbeg = 0;
-    I.kend = (uint32_t)s.L;
+    I.kend = (uint32_t)I.L;
     I.part = I.last = 0;
     return s.nq != 0;
 }
@@ -213,7 +218,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        auto compute = [&](Frag<D>& f, uint32_t i) {
+        // (only a wave's last block can hold keys that some row does not see: there are less than 16)
+        auto compute = [&](Frag<D>& f, uint32_t i, auto last) {
             const int key0 = (int)key_of(i);
             f32x4 s[2];
 #pragma unroll
@@ -229,22 +235,40 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
             float x[8];  // row n, key key0 + 8 g + j
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3];
-            const bool cuts = key0 + 32 > cut;  // wave-uniform
-            if (cuts) {
+            if (last && key0 + 32 > cut) {  // wave-uniform
+                // a value that some row does not see must be finite (0 * inf); those that a row sees are added
+                // at the end.  Keys past the last were never stored.  (Two values a register: element by element
+                // this took a wave 4 us at head_dim 256, with every other waiting for it.)
+                const int key = key0 + 8 * g;
+                uint32_t keep[4], hid[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int key = key0 + 8 * g + j;
-                    if (key >= lim) x[j] = -INFINITY;
-                    // a value that some row does not see must be finite (0 * inf); those that a row sees are added
-                    // at the end.  Keys past the last were never stored.
-                    if (key >= cut) {
+                for (int w = 0; w < 4; ++w) {
+                    const int k0 = key + 2 * w, k1 = k0 + 1;
+                    if (k0 >= lim) x[2 * w] = -INFINITY;
+                    if (k1 >= lim) x[2 * w + 1] = -INFINITY;
+                    keep[w] = (k0 < I.L ? 0xffffu : 0u) | (k1 < I.L ? 0xffff0000u : 0u);
+                    hid[w] = (k0 >= cut ? 0x8000u : 0u) | (k1 >= cut ? 0x80000000u : 0u);
+                }
+                auto each = [&](auto&& fn) {
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const bool special = (__builtin_bit_cast(uint16_t, (_Float16)f.v[b][j]) & 0x7fff) >= 0x7c00;
-                            odd = odd || (special && key < I.L);
-                            if (special || key >= I.L) f.v[b][j] = (_Float16)0.0f;
-                        }
+                    for (int b = 0; b < NB; ++b) {
+                        u32x4 v = __builtin_bit_cast(u32x4, f.v[b]);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v[w] = fn(v[w] & keep[w], w);
+                        f.v[b] = __builtin_bit_cast(f16x8, v);
                     }
+                };
+                if (cut < I.L) {  // wave-uniform
+                    uint32_t any = 0;
+                    each([&](uint32_t v, int w) {
+                        // the top bit of each half where the exponent is all ones (it carries no further)
+                        const uint32_t s = ((v & 0x7c007c00u) + 0x04000400u) & hid[w];
+                        any |= s;
+                        return v & ~(s | (s - (s >> 15)));
+                    });
+                    odd = odd || any != 0;
+                } else {
+                    each([](uint32_t v, int) { return v; });
                 }
             }
             float mx = x[0];
@@ -275,15 +299,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
         };
         uint32_t i = 0;
         for (; i + 2 < nbw; i += 2) {
-            compute(f0, i);
+            compute(f0, i, std::false_type{});
             load(f0, i + 2, page0);
             page0 = page_of(i + 4);
-            compute(f1, i + 1);
+            compute(f1, i + 1, std::false_type{});
             load(f1, i + 3, page1);  // (past the wave's last block: page ~0, zeros without a read)
             page1 = page_of(i + 5);
         }
-        if (i < nbw) compute(f0, i);
-        if (i + 1 < nbw) compute(f1, i + 1);
+        if (i < nbw) compute(f0, i, std::true_type{});
+        if (i + 1 < nbw) compute(f1, i + 1, std::true_type{});
 
         l = sum_xor32(sum_xor16(l));
         lds_barrier();  // every wave has read its queries
