@@ -22,6 +22,12 @@
 // squares is a few DPP steps.  The lane's four sines and cosines serve all its
 // passes.  V is stored d-major, in 16-byte groups of eight positions, by
 // workgroups of their own (a few rows: by the same waves, 2 bytes at a time).
+//
+// Measured: 8193 tokens of three prompts, 16 / 2 heads of 256 (M-RoPE over 64),
+// bf16: 43.7 us, 3.8 TB/s, where a large copy reaches 5.4; 480 VALU instructions
+// a wave (some of them 64 bits wide) are 22 us of that time.  Three passes a wave
+// and four waves a SIMD: one pass 54 us, two 46, five 45; six waves a SIMD spill,
+// 50.  One decode token or 64: 5 us of GPU time, the launch and two round trips.
 #include "common.hpp"
 #include "internal.hpp"
 
