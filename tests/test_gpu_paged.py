@@ -652,6 +652,19 @@ def test_attn_captured_chunks_replay_with_new_lengths(cuda):
         assert (err <= tol + U[F16] * want.abs() + 2.0 ** -24).all() and (out[b.T:] == 5).all()
 
 
+@pytest.mark.parametrize("nh,nkv,d", [(3, 2, 64), (28, 4, 128), (5, 3, 128), (16, 2, 256)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("L,new", [(0, 0), (50, 10), (300, 1), (130, 130), (129, 129), (700, 127), (640, 200), (90, 150)])
+def test_attn_one_sequence_below_its_bounds(cuda, nh, nkv, d, dtype, L, new):
+    """A launch sized for 200 tokens and 700 keys, as a captured one is, with fewer of either."""
+    b = Batch([(L, new)], nh, nkv, d, dtype=dtype, seed=60, behind=200 - new)
+    out = torch.full((200, nh * d), 5.0, dtype=dtype, device="cuda")
+    if b.table.shape[1] * 64 < 700:
+        b.table = torch.cat([b.table, torch.full((1, 11 - b.table.shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+    b.check(max_new=200, max_len=700, out=out)
+    assert (out[new:] == 5).all()
+
+
 def test_attn_calls_on_two_streams_at_once(cuda):
     """Each with its own workspace."""
     from yllm_amd.paged import paged_attn_workspace

@@ -14,7 +14,7 @@
 // Measured: a prompt of 8192 tokens, 32 / 8 heads of 128, 595 to 612 us by box,
 // 900 to 924 TFLOP/s (a contiguous cache: 553 to 600), of them 14 for the merge
 // and as much for the partial results it reads; a gated chunk of 2048 tokens at
-// 2048, 16 / 2 heads of 256, 150 us (merge 19).  A short call is a chain: 1.7 us
+// 2048, 16 / 2 heads of 256, 140 us, 735 TFLOP/s.  A short call is a chain: 1.7 us
 // to the piece, 3.3 to its first tiles, 1.2 a tile, 2 to 3 out.
 #include "common.hpp"
 #include "internal.hpp"
@@ -33,8 +33,8 @@ constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
 // dimensions of a row.  Nearly all split items of a full launch have two
 // pieces: there every kMergeRows-th workgroup takes the rows of as many, and
 // their loads, and the gate's, go out together (one row after the other, 16
-// dependent round trips: a gated chunk of 2048 tokens, 16 / 2 heads of 256,
-// merged in 22 us; so, in 19, 6 TB/s).
+// dependent round trips: 2048 tokens of 16 / 2 heads of 256 with a gate merged
+// in 22 us; so, in 19, 6 TB/s).
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
 {
@@ -153,6 +153,29 @@ uint32_t paged_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_
     return round8(most < full ? most : full);
 }
 
+// Workgroups of a launch that gives each a whole item of its one sequence,
+// without the merge; 0: it does not.  Where a whole item's walk takes no longer than a piece's with what cutting
+// costs, the merge's launch and its partial results (28 / 4 heads of 128, 1000
+// tokens: 31 us, 39 cut; 2048: 55, 66; 16 / 2 heads of 256, 2048 at 2048: 142,
+// 149; 14 / 2 heads of 64, 2048, where cutting is better: 38, 35).  In
+// microseconds, a tile 1 to 2 by head_dim, more with two workgroups on a CU.
+uint32_t paged_whole_wgs(const PagedAttnArgs& a, uint32_t per_cu, bool qs)
+{
+    if (a.n_seq != 1) return 0;
+    const uint64_t cus = (uint64_t)n_cus(), tiles = ((uint64_t)a.max_len + kUnitKeys - 1) / kUnitKeys;
+    const bool pack = a.max_new < kItemRows;
+    const uint64_t items = pack ? (uint64_t)a.n_kv * ((a.gmax * a.max_new + kItemRows - 1) / kItemRows)
+                                : (uint64_t)a.n_kv * a.gmax * ((a.max_new + kItemRows - 1) / kItemRows);
+    if (items > cus * per_cu) return 0;
+    const double mean = (double)tiles - (pack ? 0.0 : std::min(a.max_new, a.max_len) / (2.0 * kUnitKeys));
+    const double piece = std::max(((double)items * (mean + kItemUnits)) / a.n_wg, (double)a.min_units);
+    const double pieces = (double)items * (mean + kItemUnits) / piece;
+    const double tile = (a.D == 64 ? 1.0 : a.D == 128 ? 1.2 : 2.0) * (qs ? 1.5 : 1.0);
+    const double whole = tile * std::max((double)tiles, items > cus ? 1.5 * mean : 0.0);
+    const double cut = tile * piece * (pieces > (double)cus ? 1.25 : 1.0) + 5.0 + pieces * a.D * 2e-4;
+    return whole <= cut ? (uint32_t)items : 0;
+}
+
 size_t align256a(size_t x) { return (x + 255) / 256 * 256; }
 
 size_t paged_bytes(uint32_t wgs, uint32_t D)
@@ -162,10 +185,10 @@ size_t paged_bytes(uint32_t wgs, uint32_t D)
 }
 
 template <int D, int NG, bool QS>
-void launch_tiles(const PagedAttnArgs& a, hipStream_t st)
+void launch_tiles(const PagedAttnArgs& a, uint32_t grid, hipStream_t st)
 {
     constexpr int threads = 256 * NG * (D > 128 ? 2 : 1);
-    hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, PagedAttnArgs>), dim3(a.n_wg), dim3(threads), 0, st, a);
+    hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, PagedAttnArgs>), dim3(grid), dim3(threads), 0, st, a);
 }
 
 }  // namespace
@@ -186,29 +209,32 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
     const bool qs = a.q_dtype == kF32;
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
     a.min_units = min_units(a.max_len);
-    a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, a.D <= 128 && !qs ? 2 : 1, a.min_units);
+    const uint32_t per_cu = a.D <= 128 && !qs ? 2 : 1;
+    a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, per_cu, a.min_units);
     a.snap_units = kSnapUnits;
     char* p = reinterpret_cast<char*>(a.ws);
     a.desc = p;
     p += align256a((size_t)a.n_wg * sizeof(PagedDesc));
     a.part_ml = reinterpret_cast<float*>(p);
     a.part_o = reinterpret_cast<float*>(p + align256a((size_t)2 * a.n_wg * kItemRows * 2 * sizeof(float)));
+    const uint32_t whole = paged_whole_wgs(a, per_cu, qs), grid = whole ? whole : a.n_wg;
+    if (whole) a.n_wg = 0;
     switch (a.D) {
-    case 64: qs ? launch_tiles<64, 1, true>(a, st) : launch_tiles<64, 1, false>(a, st); break;
-    case 128: qs ? launch_tiles<128, 2, true>(a, st) : launch_tiles<128, 1, false>(a, st); break;
+    case 64: qs ? launch_tiles<64, 1, true>(a, grid, st) : launch_tiles<64, 1, false>(a, grid, st); break;
+    case 128: qs ? launch_tiles<128, 2, true>(a, grid, st) : launch_tiles<128, 1, false>(a, grid, st); break;
     case 256:
-        if (qs) launch_tiles<256, 1, true>(a, st);
-        else hipLaunchKernelGGL((prefill_halves_kernel<256, false, PagedAttnArgs>), dim3(a.n_wg), dim3(512), 0, st, a);
+        if (qs) launch_tiles<256, 1, true>(a, grid, st);
+        else hipLaunchKernelGGL((prefill_halves_kernel<256, false, PagedAttnArgs>), dim3(grid), dim3(512), 0, st, a);
         break;
     default: return hipErrorInvalidValue;
     }
-    if ((a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
+    if (!whole && (a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
         const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
-        const dim3 grid(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
+        const dim3 merge(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
         switch (a.D) {
-        case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, st, a); break;
+        case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, merge, dim3(256), 0, st, a); break;
+        case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, merge, dim3(256), 0, st, a); break;
+        default: hipLaunchKernelGGL(paged_merge_kernel<256>, merge, dim3(256), 0, st, a); break;
         }
     }
     return hipGetLastError();

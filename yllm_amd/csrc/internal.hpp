@@ -186,8 +186,8 @@ struct PagedAttnArgs {
     uint32_t table_stride, n_seq, n_tok, max_new, max_len, n_heads, n_kv, D, shift, n_blocks;
     float c;                // log2(e) / sqrt(D)
     void* ws;
-    // set by the launcher: the largest group of query heads per kv head; workgroups, smallest chunk and longest
-    // item left uncut (paged_items.hpp); where partial results go
+    // set by the launcher: the largest group of query heads per kv head; workgroups of the line (0: a whole item
+    // each), smallest chunk and longest item left uncut (paged_items.hpp); where partial results go
     uint32_t gmax, n_wg, min_units, snap_units;
     void* desc;             // [n_wg] PagedDesc
     float* part_ml;         // [2 n_wg][rows][2]

@@ -9,8 +9,9 @@
 // number of units.  A cut inside an item leaves partial results (running
 // maximum, sum and unnormalised output), at most one at each end of a chunk,
 // which a merge kernel joins in order; cuts inside short items move to the
-// item's start, which costs less than joining them.  Lengths are read on the
-// device, so a captured launch replays with new ones.
+// item's start, which costs less than joining them.  (One sequence may go item
+// by item instead, paged_whole.)  Lengths are read on the device, so a captured
+// launch replays with new ones.
 #pragma once
 
 #include "common.hpp"
@@ -313,11 +314,58 @@ __device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedI
     }
 }
 
+// The item of this workgroup where each takes a whole one of the only sequence
+// (n_wg 0: paged_whole_wgs, attn_paged.hip), those of the last tokens, the
+// longest, first; false if there is none.
+template <int BN>
+__device__ inline bool paged_whole(const PagedAttnArgs& a, PagedItem& I)
+{
+    const PagedSeq s = cursor_seq(a, 0);
+    const uint32_t w = blockIdx.x;
+    int seen;
+    I.pack = s.nq < kItemRows;
+    if (I.pack) {
+        I.qb = w / a.n_kv;
+        I.kvh = w - I.qb * a.n_kv;
+        I.h = head0(a, I.kvh);
+        if (I.qb * kItemRows >= (head0(a, I.kvh + 1) - I.h) * s.nq) return false;
+        seen = s.L;
+    } else {
+        const uint32_t nb = (s.nq + kItemRows - 1) / kItemRows, i = w / a.n_heads;
+        if (i >= nb) return false;
+        I.qb = nb - 1 - i;
+        I.h = w - i * a.n_heads;
+        I.kvh = I.h * a.n_kv / a.n_heads;
+        seen = s.pos0 + (int)min(s.nq, (I.qb + 1) * kItemRows);
+    }
+    I.part = I.last = I.seq = I.t0 = 0;
+    I.row0 = s.row0;
+    I.nq = s.nq;
+    I.pos0 = s.pos0;
+    I.kmax = (uint32_t)max(seen - 1, 0);
+    I.idle = seen <= 0;
+    I.nt = I.kmax / BN + 1;
+    return true;
+}
+
+// The workgroup's first piece; false if it has none.
+template <int NT, int BN>
+__device__ inline bool paged_first(const PagedAttnArgs& args, uint64_t* scratch, PagedCursor& C, PagedItem& I)
+{
+    if (args.n_wg == 0) {
+        C = PagedCursor{};  // an empty chunk: nothing comes after the item
+        return paged_whole<BN>(fresh_args(args), I);
+    }
+    if (paged_start<NT>(fresh_args(args), scratch, C) && paged_next<BN>(fresh_args(args), C, I)) return true;
+    if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
+    return false;
+}
+
 // The workgroup's last piece, which may begin a split item: what the merge
 // needs to know of it.
 __device__ inline void paged_leave(const PagedAttnArgs& a, const PagedCursor& C, const PagedItem& I)
 {
-    if (threadIdx.x != 0) return;
+    if (threadIdx.x != 0 || a.n_wg == 0) return;
     PagedDesc* d = reinterpret_cast<PagedDesc*>(a.desc) + C.j;
     if (I.part == 1) *d = PagedDesc{I.last - C.j + 1, I.row0, I.nq, I.kvh, I.h, I.qb, I.pack, 0};
     else d->n = 0;

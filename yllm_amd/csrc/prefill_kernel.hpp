@@ -478,12 +478,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     constexpr bool AHEAD = PAGED && !QS && NB == 2;
     Item cur;
     if constexpr (PAGED) {
-        const bool any = paged_start<256 * NG * (PAIR ? 2 : 1)>(fresh_args(args), reinterpret_cast<uint64_t*>(&Kl0[0][0]), C) &&
-                         item_of(0, cur);
-        if (!any) {
-            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
-            return;
-        }
+        if (!paged_first<256 * NG * (PAIR ? 2 : 1), BN>(args, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C, cur)) return;
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
@@ -1237,10 +1232,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
     };
     Item cur;
     if constexpr (PAGED) {
-        if (!(paged_start<512>(fresh_args(args), reinterpret_cast<uint64_t*>(&Kl0[0]), C) && item_of(0, cur))) {
-            if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
-            return;
-        }
+        if (!paged_first<512, BN>(args, reinterpret_cast<uint64_t*>(&Kl0[0]), C, cur)) return;
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
