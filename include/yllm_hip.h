@@ -294,14 +294,15 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
  * with kv_lens 0).  Rows from cu_new[n_seq] on are left as they were.  dtypes,
  * strides (multiples of 8; q, att_out and pools 16-byte aligned) and gate as in
  * yhip_attn_prefill; att_out must not overlap q or gate.  16-bit queries:
- * scores and P.V from f16 products with fp32 sums; fp32 queries: both at
- * fp32-level error.  Queries must lie within the f16 range (65504).
+ * scores and P.V from f16 products with fp32 sums (P in f16, or better);
+ * fp32 queries: both at fp32-level error.  Queries must lie within the f16
+ * range (65504).
  *
  * max_new (at most n_tok) and max_len bound the new tokens and the length of
  * every sequence: longer ones are cut to them (rows past a sequence's max_new
  * are left as they were).  max_new 1 (with n_tok = n_seq) is a decode step.
- * cu_new does not decrease.  Table entries outside the pool read as keys and values of zero.
- * Needs yhip_paged_attn_workspace bytes (16-byte aligned, no initialisation)
+ * cu_new does not decrease.  Table entries outside the pool read as keys and
+ * values of zero.  Needs yhip_paged_attn_workspace bytes (16-byte aligned, no initialisation)
  * for the bounds given; a workspace sized for larger n_tok, n_seq, max_new and
  * max_len serves smaller ones.  Calls that share a workspace must not run
  * concurrently. */

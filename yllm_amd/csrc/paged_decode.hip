@@ -13,13 +13,14 @@
 // lengths cost no idle time; items cut by a chunk's end are joined by the
 // merge kernel.  Page numbers are read a round ahead of the loads they place.
 //
-// 16-bit queries are exact as f16; fp32 ones are split into f16 hi + lo parts,
-// and so are their probabilities (PREC), which the matrix cores do in the
-// shadow of the loads.
+// 16-bit queries are exact as f16; fp32 ones are split into f16 hi + lo parts
+// (PREC).  So are the probabilities of either: rounded to f16 alone they double
+// the variance of an f16 output's error, and the second product is in the shadow
+// of the loads (64 sequences of 1024 .. 32768 keys 357 us with it or without).
 //
 // Measured: 64 sequences of 1024 .. 32768 keys, 32 / 8 heads of 128, 357 us, 6.67
 // TB/s; one token over 131072 keys 83 us and a merge of 5, over 300 keys of 28 /
-// 4 heads of 128 9.4, of 16 / 2 heads of 256 13.4.  A short call is a chain: 1.6 us to the piece, 2
+// 4 heads of 128 9.9, of 16 / 2 heads of 256 14.3.  A short call is a chain: 1.6 us to the piece, 2
 // to issue two blocks' loads (64 of them at head_dim 256: 4 to 6), 1 to 2 for a
 // block and 1.5 to join the waves.
 #include "common.hpp"
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 o[b] = mfma16(f.v[b], pf, o[b]);
-                if constexpr (PREC) o[b] = mfma16(bounded(f.v[b]), pl, o[b]);
+                o[b] = mfma16(bounded(f.v[b]), pl, o[b]);
             }
         };
         uint32_t i = 0;
