@@ -860,3 +860,37 @@ def test_serving_step_captured_and_replayed(cuda):
             rows = s.rows(40)
             for o, (want, tol) in zip(s.step(_i32([0, 39, 1]), rows, 40, 39, 384), s.exact([0, 39, 1], rows)):
                 _hold(o, want, tol)
+
+
+# ---- calls that the documentation allows at the ends of its ranges ---------------------------------------
+
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (32, 8, 128), (16, 2, 256)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("seqs", [[(0, 600), (0, 600)], [(100, 600), (0, 700), (256, 1)], [(0, 3000)], [(256, 900), (5, 400)]])
+def test_attn_many_more_tokens_than_positions(cuda, nh, nkv, d, dtype, seqs):
+    """Bounds of at most 256 keys, and prompts of more tokens than that, as the plan leaves a prompt that its table row
+    cannot hold: every row is written."""
+    b = Batch(seqs, nh, nkv, d, dtype=dtype, seed=70)
+    out = torch.full((b.T, nh * d), math.nan, dtype=dtype, device="cuda")
+    b.check(max_len=256 if b.table.shape[1] >= 4 else b.max_len, out=out)
+    for (L, n), at in zip(seqs, b.cu):
+        assert (out[at:at + max(0, n - L)] == 0).all()
+
+
+def test_serving_prompts_that_their_table_rows_cannot_hold(cuda):
+    """Refused by the plan, their attention rows are zero, whatever the output held."""
+    from yllm_amd import paged as P
+
+    new, width, (nh, nkv, d) = [600, 1, 500, 300], 4, (32, 8, 128)
+    table = torch.full((4, width), -1, dtype=torch.int32, device="cuda")
+    pool, T = P.PagedKV.empty(20, nkv, d), sum(new)
+    step = P.paged_plan(table, _i32([0, 0, 0, 0]), _i32(new), _i32(list(range(20))), _i32([20]), 64, T)
+    assert step.kv_lens.tolist() == [0, 1, 0, 0] and step.counts.tolist() == [19, T, 3, 0]
+    x = torch.randn(T, (nh + 2 * nkv) * d, generator=_gen(71), device="cuda").half()
+    q, k, v = x[:, :nh * d], x[:, nh * d:(nh + nkv) * d], x[:, (nh + nkv) * d:]
+    P.qk_norm_rope_kv_store(pool, q, k, v, nh, KINDS["half"], 1e6, positions=step.positions, slots=step.slots)
+    out = torch.full((T, nh * d), math.nan, dtype=F16, device="cuda")
+    P.paged_attn(q, pool, step.block_table, step.kv_lens, step.cu_new, nh, max(new), width * 64, out=out)
+    want = torch.zeros_like(out)
+    want[600] = v[600].view(nkv, 1, d).expand(nkv, nh // nkv, d).reshape(-1)  # its only key
+    assert torch.equal(out, want)

@@ -228,7 +228,9 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
         break;
     default: return hipErrorInvalidValue;
     }
-    if (!whole && (a.max_len + kUnitKeys - 1) / kUnitKeys > a.snap_units) {  // an item may be split
+    // an item may be split (with more new tokens than keys its units go by its tokens, paged_items.hpp)
+    const uint32_t longest = std::max(a.max_len, a.max_new);
+    if (!whole && longest > a.snap_units * kUnitKeys) {
         const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
         const dim3 merge(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
         switch (a.D) {
