@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 
@@ -150,3 +152,22 @@ def test_python_refusals():
     for f in bad:
         with pytest.raises(YhipError):
             f()
+
+
+def test_chunks_of_a_line_of_any_length(tmp_path):
+    """The line's cuts (csrc/paged_chunks.hpp, compiled for the host): equal chunks, one per workgroup at most, that cover
+    it, also where a sum comes near 2^32."""
+    csrc = Path(__file__).resolve().parent.parent / "yllm_amd" / "csrc"
+    src, exe = tmp_path / "chunks.cpp", tmp_path / "chunks"
+    src.write_text('#include "paged_chunks.hpp"\n#include <stdio.h>\n#include <inttypes.h>\nint main() {\n'
+                   'uint64_t t; uint32_t w, m;\nwhile (scanf("%" SCNu64 " %" SCNu32 " %" SCNu32, &t, &w, &m) == 3) {\n'
+                   'const auto c = yhip::paged_chunks(t, w, m);\nprintf("%u %u\\n", c.units, c.n); } }\n')
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", f"-I{csrc}", str(src), "-o", str(exe)], check=True)
+    near = [(1 << b) + k for b in (31, 32, 33) for k in (-(1 << 24), -(1 << 23), -(1 << 23) - 512, -(1 << 22), -513, -511, -1, 0, 1, 511)]
+    cases = [(t, w, m) for t in [0, 1, 9, 100, 4096, 10 ** 6, (1 << 38) - 1, *near] for w in (8, 256, 512, 520) for m in (2, 4, 26, 3344)]
+    run = subprocess.run([str(exe)], input="".join(f"{t} {w} {m}\n" for t, w, m in cases), capture_output=True, text=True, check=True)
+    got = [tuple(map(int, line.split())) for line in run.stdout.splitlines()]
+    assert len(got) == len(cases)
+    for (t, w, m), (units, n) in zip(cases, got):
+        want = max(min(-(-t // w), 0x7fffffff), m)
+        assert (units, n) == (want, -(-t // want)), (t, w, m)

@@ -16,6 +16,7 @@
 
 #include "common.hpp"
 #include "internal.hpp"
+#include "paged_chunks.hpp"
 
 namespace yhip {
 namespace {
@@ -139,10 +140,9 @@ __device__ inline const PagedAttnArgs& fresh_args(const PagedAttnArgs&)
 // share.
 __device__ inline bool paged_chunk(const PagedAttnArgs& a, PagedCursor& C, uint64_t total, uint64_t& begin)
 {
-    const uint64_t even = (total >> 32) ? (total + a.n_wg - 1) / a.n_wg : ((uint32_t)total + a.n_wg - 1) / a.n_wg;
-    C.chunk = max((uint32_t)min(even, (uint64_t)0x7fffffff), a.min_units);
-    const uint32_t all = (total >> 32) ? (uint32_t)((total + C.chunk - 1) / C.chunk) : ((uint32_t)total + C.chunk - 1) / C.chunk;
-    const uint32_t active = min(all, a.n_wg);  // (more only if offsets that overlap pass the bounds checked on the host)
+    const PagedChunks cut = paged_chunks(total, a.n_wg, a.min_units);
+    C.chunk = cut.units;
+    const uint32_t active = min(cut.n, a.n_wg);  // (more only if offsets that overlap pass the bounds checked on the host)
     const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
     C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
     begin = (uint64_t)C.j * C.chunk;
