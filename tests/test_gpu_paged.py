@@ -894,3 +894,22 @@ def test_serving_prompts_that_their_table_rows_cannot_hold(cuda):
     want = torch.zeros_like(out)
     want[600] = v[600].view(nkv, 1, d).expand(nkv, nh // nkv, d).reshape(-1)  # its only key
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("L,new", [(70, 1), (70, 6), (900, 2), (400, 40), (400, 300)])
+def test_attn_nan_of_any_bits_stays_nan(cuda, nh, nkv, d, dtype, out_dtype, L, new):
+    """Values of all ones, as a page filled with 0xff bytes holds, are NaN in every output type, of the rows that see them."""
+    for at in (L - 1, 0):  # seen by the last row alone, by all
+        b = Batch([(L, new), (129, 2)], nh, nkv, d, dtype=dtype, seed=72)
+        page, off = int(b.table[0, at // 64]), at % 64
+        bits = torch.tensor([0x7fff, -1, 0x7c01, -0x3ff], dtype=torch.int16, device="cuda").repeat(d // 4)
+        b.cache.v.view(torch.int16)[page, :, off // 32, :, off % 32] = bits
+        got = b.run(out_dtype=out_dtype)
+        assert got[new - 1].isnan().all()
+        rest = got[new:] if at == 0 else torch.cat([got[:new - 1], got[new:]])
+        assert rest.isfinite().all()
+        if at == 0:
+            assert got[:new].isnan().all()

@@ -404,20 +404,12 @@ __device__ inline void store_out4(void* out, size_t off, uint32_t dt, f32x4 v)
         for (int j = 0; j < 4; ++j) h[j] = (_Float16)v[j];
         *reinterpret_cast<f16x4*>(reinterpret_cast<uint16_t*>(out) + off) = h;
     } else {
-        // round to nearest even; each element goes through a scalar float
-        // (bit-casting an ext-vector element directly reads element 0)
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        uint32_t h[4];
+        // gfx950's own conversion, to nearest even (an addition to the bits would carry a NaN of all ones to zero)
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        bf16x4 h;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float f = v[j];
-            const uint32_t x = __builtin_bit_cast(uint32_t, f);
-            h[j] = (x + 0x7fffu + ((x >> 16) & 1u)) >> 16;
-        }
-        u32x2 w;
-        w[0] = h[0] | (h[1] << 16);
-        w[1] = h[2] | (h[3] << 16);
-        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(out) + off) = w;
+        for (int j = 0; j < 4; ++j) h[j] = (__bf16)v[j];
+        *reinterpret_cast<bf16x4*>(reinterpret_cast<uint16_t*>(out) + off) = h;
     }
 }
 
