@@ -295,8 +295,10 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
  * strides (multiples of 8; q, att_out and pools 16-byte aligned) and gate as in
  * yhip_attn_prefill; att_out must not overlap q or gate.  16-bit queries:
  * scores and P.V from f16 products with fp32 sums (P in f16, or better);
- * fp32 queries: both at fp32-level error.  Queries must lie within the f16
- * range (65504).
+ * fp32 queries: both at fp32-level error, from f16 hi + lo pairs.  f16's
+ * smallest step shows where values are far apart: a query element is off by up
+ * to 2^-25, a probability by up to 2^-32 of the row's largest.  Queries must
+ * lie within the f16 range (65504).
  *
  * max_new (at most n_tok) and max_len bound the new tokens and the length of
  * every sequence: longer ones are cut to them (rows past a sequence's max_new

@@ -913,3 +913,32 @@ def test_attn_nan_of_any_bits_stays_nan(cuda, nh, nkv, d, dtype, out_dtype, L, n
         assert rest.isfinite().all()
         if at == 0:
             assert got[:new].isnan().all()
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n_seq,L,new", [(1, 131072, 2048), (72, 32768, 1)])
+def test_attn_many_small_probabilities(cuda, nh, nkv, d, dtype, n_seq, L, new):
+    """One key far above all others, which are so many that they count all the same: with a score of s the first key, of
+    value 0, and of 0 the others, of value 1, the row at position p is p e^-s / (1 + p e^-s)."""
+    from yllm_amd.paged import PagedKV, paged_attn
+
+    c = 19.0 / math.sqrt(d)  # e^-19 = 2^-27.4
+    c = float(torch.tensor(c).half())
+    s = c * math.sqrt(d)
+    pages = L // 1024
+    pool = PagedKV(torch.zeros((pages, nkv, 1024, d), dtype=F16, device="cuda"),
+                   torch.ones((pages, nkv, 32, d, 32), dtype=F16, device="cuda"))
+    pool.k[0, :, 0], pool.v[0, :, 0, :, 0] = c, 0.0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(n_seq, pages).contiguous()
+    q = torch.ones((n_seq * new, nh * d), dtype=dtype, device="cuda")
+    got = paged_attn(q, pool, table, _i32([L] * n_seq), _i32([i * new for i in range(n_seq + 1)]), nh, new, L, out_dtype=F32)
+    p = torch.arange(L - new, L, device="cuda").double().repeat(n_seq)
+    w = p * math.exp(-s)
+    want = (w / (1 + w))[:, None]
+    # a probability: half a step of f16 (of a hi and lo pair, 2^-22), or, below the f16 normals, half of 2^-24 times the
+    # 2^-7 by which the largest is scaled up; the score's sum and exp2: 2^-24 of s = 19 three times, its sums 2^-20
+    u = 2.0 ** -22 if dtype == F32 else 2.0 ** -11
+    tol = want * (u + 2.0 ** -20 + 3 * 19 * 2.0 ** -24) + p[:, None] * 2.0 ** -32 + want * 2.0 ** -24
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), (float(err.max()), float((err / tol).max()), float(want.max()))

@@ -282,8 +282,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode_kernel(Pag
 #pragma unroll
             for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
             mx = max_xor32(max_xor16(mx)) * a.c;
-            if (__ballot(mx > m + 8.0f)) {  // (p stays below 2^8)
-                const float mn = mx > m + 8.0f ? mx : m;
+            if (__ballot(mx > m + (kLift + kSlack))) {
+                const float mn = mx > m + (kLift + kSlack) ? mx - kLift : m;
                 const float alpha = fast_exp2(m - mn);
                 m = mn;
                 l *= alpha;

@@ -413,6 +413,15 @@ __device__ inline void store_out4(void* out, size_t off, uint32_t dt, f32x4 v)
     }
 }
 
+// Probabilities enter the products scaled by 2^kLift: the running maximum that
+// they are formed against stays kLift below the true one, in powers of two, as
+// it is up to kSlack behind it (so that it seldom moves), and 2^(kLift + kSlack)
+// is below f16's largest.  f16 has nothing below 2^-25: without the scale, keys
+// below 2^-25 of the largest counted as nothing, and 100,000 of them are 2^-8 of
+// a row (a key that draws nearly all the attention, over a long context).  Sums
+// and partial results carry the scale; the division takes it out.
+constexpr float kSlack = 8.0f, kLift = 7.0f;
+
 // Values for the product with the probabilities' lo parts: an inf or NaN as a
 // finite value.  The hi parts bring it in; with a lo part, 0 or negative
 // beside a positive hi, the same inf would make NaN.

@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     constexpr int CH = BN * D / (8 * LT);  // 16-byte chunks per thread per tile (K and V each)
     constexpr int KCH = D / 8;    // 16-byte chunks per K row
     constexpr int VCH = BN / 8;   // 16-byte chunks per V row
-    constexpr float kSlack = 8.0f;
+    constexpr float LIFT = PAGED ? kLift : 0.0f;
     // NG key groups of 4 waves share the workgroup's 128 queries: group g
     // walks key tiles g, g+NG, g+2NG, ... with its own LDS buffers, and the
     // groups' partial results are merged at the end, so the longest chain
@@ -789,8 +789,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
                                                              __builtin_bit_cast(uint32_t, mx), false, false);
             mx = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1])) * a.c;
-            if (__ballot(mx > m + kSlack)) {  // wave-uniform: some query's max moved
-                const float mn = mx > m + kSlack ? mx : m;
+            if (__ballot(mx > m + (LIFT + kSlack))) {  // wave-uniform: some query's max moved
+                const float mn = mx > m + (LIFT + kSlack) ? mx - LIFT : m;
                 const float alpha = fast_exp2(m - mn);
                 m = mn;
                 l *= alpha;
@@ -1217,7 +1217,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
     constexpr int NKK = D / 16, NDB = DH / 32;
     constexpr int KCH = D / 8, VCH = BN / 8;
     constexpr int CH = BN * D / (8 * 512);  // 16-byte chunks per thread per tile (K and V each)
-    constexpr float kSlack = 8.0f;
+    constexpr float LIFT = PAGED ? kLift : 0.0f;
     __shared__ __attribute__((aligned(16))) _Float16 Kl0[BN * D], Kl1[BN * D], Vl0[D * BN], Vl1[D * BN];
     __shared__ f16x8 Pl[8][2][64];  // each wave's probabilities: k-slot, lane
     __shared__ float Ml[8][64];     // each wave's tile maxima, then its row sums
@@ -1426,8 +1426,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
         };
         auto rescale = [&](float other) {
             const float t = fmaxf(mx, other) * a.c;
-            if (__ballot(t > m + kSlack)) {  // wave-uniform, and the same for both waves of the pair
-                const float mn = t > m + kSlack ? t : m;
+            if (__ballot(t > m + (LIFT + kSlack))) {  // wave-uniform, and the same for both waves of the pair
+                const float mn = t > m + (LIFT + kSlack) ? t - LIFT : m;
                 const float alpha = fast_exp2(m - mn);
                 m = mn;
                 l *= alpha;
