@@ -275,7 +275,8 @@ int yhip_paged_plan(int32_t* block_table, uint32_t max_blocks, uint32_t table_st
  * to pos * 6e-8 rad).
  * q, k, v: rows of `dtype` (YHIP_F32 / F16 / BF16), strides in elements, so
  * they may be slices of one projection row; q_out NULL skips q, and may be q
- * itself with the same type and stride.  Pointers aligned to four elements
+ * itself with the same type and stride; but for that, q_out and the pools must
+ * overlap neither an input nor each other.  Pointers aligned to four elements
  * (pools to 16 bytes), strides multiples of 4, block a multiple of 64, an
  * MROPE n_rot a multiple of 8. */
 int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
@@ -293,12 +294,12 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
  * all stored (a negative position sees nothing: a zero row, as has a sequence
  * with kv_lens 0).  Rows from cu_new[n_seq] on are left as they were.  dtypes,
  * strides (multiples of 8; q, att_out and pools 16-byte aligned) and gate as in
- * yhip_attn_prefill; att_out must not overlap q or gate.  16-bit queries:
- * scores and P.V from f16 products with fp32 sums (P in f16, or better);
- * fp32 queries: both at fp32-level error, from f16 hi + lo pairs.  f16's
- * smallest step shows where values are far apart: a query element is off by up
- * to 2^-25, a probability by up to 2^-32 of the row's largest.  Queries must
- * lie within the f16 range (65504).
+ * yhip_attn_prefill; att_out and the workspace must overlap neither an input
+ * nor each other.  16-bit queries: scores and P.V from f16 products with fp32
+ * sums (P in f16, or better); fp32 queries: both at fp32-level error, from f16
+ * hi + lo pairs.  f16's smallest step shows where values are far apart: a bf16
+ * or fp32 query element is off by up to 2^-25, a probability by up to 2^-32 of
+ * the row's largest.  Queries must lie within the f16 range (65504).
  *
  * max_new (at most n_tok) and max_len bound the new tokens and the length of
  * every sequence: longer ones are cut to them (rows past a sequence's max_new

@@ -171,3 +171,27 @@ def test_chunks_of_a_line_of_any_length(tmp_path):
     for (t, w, m), (units, n) in zip(cases, got):
         want = max(min(-(-t // w), 0x7fffffff), m)
         assert (units, n) == (want, -(-t // want)), (t, w, m)
+
+
+# (addresses of attn_args and store_args: the pools take 0x20000 bytes each)
+@pytest.mark.parametrize("kw", [
+    {"out": _at(0x6000000 + 0x1fff0)}, {"out": _at(0x7000000 - 4096)}, {"out": _at(0x5000000)}, {"out": _at(0x5100000 - 4096)},
+    {"out": _at(0x5200000 - 10224)}, {"kp": _at(0x1000000 - 0x1fff0)}, {"vp": _at(0x1000000 + 10224)},
+    {"ws": _at(0x1000000 + 10224)}, {"ws": _at(0x2000000 - 16)}, {"ws": _at(0x6000000 + 0x1fff0)}, {"ws": _at(0x7000000)},
+    {"ws": _at(0x5000020)}, {"ws": _at(0x5100000)}, {"ws": _at(0x5200000)}, {"gate": _at(0x9000000), "gs": 1024, "ws": _at(0x9000000 + 5 * 4096 - 16)},
+])
+def test_attn_overlaps(hiplib, kw):
+    """What the call writes (the rows, the workspace) is neither what it reads nor each other."""
+    kw = dict(w=64, stride=64, max_len=4096, wsb=1 << 30, **{"ws": _at(1 << 40), **kw})
+    assert hiplib.yhip_paged_attn(*attn_args(**kw)) == -22 and "overlaps" in _err(hiplib)
+
+
+@pytest.mark.parametrize("kw", [
+    {"qo": _at(0x6000000 + 0x1fff0)}, {"qo": _at(0x7000000 - 4096)}, {"qo": _at(0x5000000)}, {"qo": _at(0x5100000 - 4096)},
+    {"qo": _at(0x5200000)}, {"qo": _at(0x5300000 - 10224)}, {"vp": _at(0x6000000 + 0x1fff0)}, {"kp": _at(0x2000000)},
+    {"kp": _at(0x3000000 - 0x1fff0)}, {"vp": _at(0x4000000)}, {"vp": _at(0x3000000)}, {"kp": _at(0x5000000)}, {"kp": _at(0x5100000)},
+    {"vp": _at(0x5200000)}, {"vp": _at(0x5300000)}, {"kp": _at(0x4000000), "qo": None, "q": None},
+])
+def test_store_overlaps(hiplib, kw):
+    """What the call writes (the queries, the pools) is neither what it reads (q_out may be q) nor each other."""
+    assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(**kw)) == -22 and "overlap" in _err(hiplib)

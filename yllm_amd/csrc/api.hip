@@ -688,6 +688,9 @@ yhip::Rows rows_of(const void* p, uint32_t dt, uint32_t stride, uint64_t width, 
     return yhip::Rows{p, stride * e, width * e, n};
 }
 
+// some row of r has a byte of [p, p + n)
+bool hits(const yhip::Rows& r, const void* p, uint64_t n) { return p && n && rows_overlap(r, yhip::Rows{p, n, n, 1}); }
+
 // log2 of the positions of a block, or an error
 int block_shift(const char* fn, uint32_t block, uint32_t& shift)
 {
@@ -788,14 +791,24 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
         (q_norm && ((uintptr_t)q_norm % w_al || (uintptr_t)k_norm % w_al)))
         return fail(YHIP_EINVAL, "%s: rows, weights and pools must be aligned to four elements (pools to 16 bytes)", fn);
     if (n_tok == 0) return done(hipSuccess, "");
+    // nothing that the call writes is read by it (q_out may be q itself) or written twice
+    const yhip::Rows rk = rows_of(k, dtype, k_stride, kv_dim, n_tok), rv = rows_of(v, dtype, v_stride, kv_dim, n_tok);
+    const uint64_t pool = 2ull * n_blocks * block * kv_dim, w_bytes = q_norm ? (norm_dtype == YHIP_F32 ? 4ull : 2ull) * head_dim : 0,
+                   row_ints = 4ull * n_tok;
     if (q_out) {
-        const yhip::Rows ro = rows_of(q_out, q_out_dtype, q_out_stride, qd, n_tok);
+        const yhip::Rows ro = rows_of(q_out, q_out_dtype, q_out_stride, qd, n_tok), rq = rows_of(q, dtype, q_stride, qd, n_tok);
         const bool same = q_out == q && q_out_dtype == dtype && q_out_stride == q_stride;
-        if ((!same && rows_overlap(ro, rows_of(q, dtype, q_stride, qd, n_tok))) ||
-            rows_overlap(ro, rows_of(k, dtype, k_stride, kv_dim, n_tok)) ||
-            rows_overlap(ro, rows_of(v, dtype, v_stride, kv_dim, n_tok)))
+        if ((!same && rows_overlap(ro, rq)) || rows_overlap(ro, rk) || rows_overlap(ro, rv) || hits(ro, q_norm, w_bytes) ||
+            hits(ro, k_norm, w_bytes) || hits(ro, positions, row_ints) || hits(ro, slots, row_ints))
             return fail(YHIP_EINVAL, "%s: q_out overlaps its inputs (it may be q itself, of the same type and stride)", fn);
+        if (hits(ro, kpool, pool) || hits(ro, vpool, pool) || hits(rq, kpool, pool) || hits(rq, vpool, pool))
+            return fail(YHIP_EINVAL, "%s: a pool overlaps q or q_out", fn);
     }
+    if (overlap(kpool, pool, vpool, pool)) return fail(YHIP_EINVAL, "%s: the pools overlap", fn);
+    for (const uint16_t* p : {kpool, vpool})
+        if (hits(rk, p, pool) || hits(rv, p, pool) || overlap(p, pool, q_norm, w_bytes) || overlap(p, pool, k_norm, w_bytes) ||
+            overlap(p, pool, positions, positions ? row_ints : 0) || overlap(p, pool, slots, slots ? row_ints : 0))
+            return fail(YHIP_EINVAL, "%s: a pool overlaps the call's inputs", fn);
     yhip::QkNormRopeArgs a = {};
     a.q_out = q_out;
     a.q = q;
@@ -876,9 +889,9 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     if (((uintptr_t)q | (uintptr_t)att_out | (uintptr_t)kpool | (uintptr_t)vpool) % 16)
         return fail(YHIP_EINVAL, "%s: q, att_out and the pools must be 16-byte aligned", fn);
     if (n_tok == 0 || n_seq == 0 || max_new == 0) return done(hipSuccess, "");
-    const yhip::Rows ro = rows_of(att_out, out_dtype, out_stride, row, n_tok);
-    if (rows_overlap(ro, rows_of(q, q_dtype, q_stride, row, n_tok)) ||
-        (gate && rows_overlap(ro, rows_of(gate, YHIP_F32, gate_stride, row, n_tok))))
+    const yhip::Rows ro = rows_of(att_out, out_dtype, out_stride, row, n_tok), rq = rows_of(q, q_dtype, q_stride, row, n_tok),
+                     rg = rows_of(gate, YHIP_F32, gate_stride, row, n_tok);
+    if (rows_overlap(ro, rq) || (gate && rows_overlap(ro, rg)))
         return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
     // tiles of 64 keys that the largest sequence's 128-row items walk
     const uint64_t nb = (max_new + 127) / 128, tiles = max_len / 64 + 1, gmax = (n_heads + n_kv_heads - 1) / n_kv_heads;
@@ -887,10 +900,21 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     if ((nb * (tiles + nb + 8) + tiles) * gmax * n_kv_heads >= 1ull << 31 || items * (tiles + 8) >= 1ull << 38)
         return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
                     max_new, max_len);
+    const struct { const void* p; uint64_t n; } in[] = {
+        {kpool, 2ull * n_blocks * n_kv_heads * block * head_dim}, {vpool, 2ull * n_blocks * n_kv_heads * block * head_dim},
+        {block_table, 4ull * ((n_seq - 1ull) * table_stride + max_blocks)}, {kv_lens, 4ull * n_seq}, {cu_new, 4ull * n_seq + 4}};
+    bool clash = false;
+    for (const auto& i : in) clash = clash || hits(ro, i.p, i.n);
+    if (clash) return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
     const size_t need = yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(YHIP_ENOSPC, "%s: %zu bytes of workspace (16-byte aligned) needed, %zu given", fn, need,
                     workspace_bytes);
+    if (need) {
+        clash = hits(ro, workspace, need) || hits(rq, workspace, need) || (gate && hits(rg, workspace, need));
+        for (const auto& i : in) clash = clash || overlap(workspace, need, i.p, i.n);
+        if (clash) return fail(YHIP_EINVAL, "%s: the workspace overlaps the call's tensors", fn);
+    }
     yhip::PagedAttnArgs a = {};
     a.q = q;
     a.q_dtype = q_dtype;
