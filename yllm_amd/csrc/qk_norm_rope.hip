@@ -205,7 +205,6 @@ __device__ void v_block(const QkNormRopeArgs& a, uint32_t vb)
     }
     __syncthreads();
     // first rows of groups are at least 8 apart: at most one in each 8 rows
-    const bool wide = ((uintptr_t)a.vc & 15u) == 0;
 #pragma unroll
     for (uint32_t it = 0; it < 2; ++it) {
         const uint32_t g = (t + 256u * it) & 7u, c = (t + 256u * it) >> 3;
@@ -214,15 +213,10 @@ __device__ void v_block(const QkNormRopeArgs& a, uint32_t vb)
         const uint32_t r = 8u * g + (uint32_t)__builtin_ctz(m);
         const uint16_t* src = &tile[c * TP + r];
         uint16_t* dst = a.vc + v_page_at<D>(a, h, (uint32_t)slots[7 + r], d0 + c);
-        if (wide) {
-            u32x4 w;
+        u32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-            *reinterpret_cast<u32x4*>(dst) = w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = src[e];
-        }
+        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
+        *reinterpret_cast<u32x4*>(dst) = w;  // (pools are aligned to 16 bytes, checked on the host)
     }
     uint64_t left = (uint64_t)lone[1] << 32 | lone[0];
     for (uint32_t n = 0; left; ++n, left &= left - 1) {  // uniform: each wave takes every fourth
