@@ -942,3 +942,14 @@ def test_attn_many_small_probabilities(cuda, nh, nkv, d, dtype, n_seq, L, new):
     tol = want * (u + 2.0 ** -20 + 3 * 19 * 2.0 ** -24) + p[:, None] * 2.0 ** -32 + want * 2.0 ** -24
     err = (got.double() - want).abs()
     assert (err <= tol).all(), (float(err.max()), float((err / tol).max()), float(want.max()))
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("n_seq", [1, 9])
+@pytest.mark.parametrize("new", [1, 2])
+def test_attn_contexts_about_the_longest_that_is_not_cut(cuda, nh, nkv, d, n_seq, new):
+    for L in (65536 // d - 128, 65536 // d - 1, 65536 // d, 65536 // d + 1, 65536 // d + 129):
+        b = Batch([(max(new, L - 37 * i), new) for i in range(n_seq)], nh, nkv, d, dtype=(F16, F32)[L % 2], seed=L)
+        b.check()
+        # under another bound, on either side of that length, the same rows
+        b.check(max_len=b.table.shape[1] * 64)

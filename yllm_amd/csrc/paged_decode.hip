@@ -13,16 +13,17 @@
 // lengths cost no idle time; items cut by a chunk's end are joined by the
 // merge kernel.  Page numbers are read a round ahead of the loads they place.
 //
-// 16-bit queries are exact as f16; fp32 ones are split into f16 hi + lo parts
-// (PREC).  So are the probabilities of either: rounded to f16 alone they double
-// the variance of an f16 output's error, and the second product is in the shadow
-// of the loads (64 sequences of 1024 .. 32768 keys 357 us with it or without).
+// f16 queries are taken as they are, bf16 ones as f16 (exact from 2^-17 up to
+// 65504, off by at most 2^-25 below), fp32 ones as f16 hi + lo parts (PREC).  The
+// probabilities of all are hi + lo parts: rounded to f16 alone they double the
+// variance of an f16 output's error, and the second product is in the shadow of
+// the loads (64 sequences of 1024 .. 32768 keys 357 us with it or without).
 //
 // Measured: 64 sequences of 1024 .. 32768 keys, 32 / 8 heads of 128, 357 us, 6.67
-// TB/s; one token over 131072 keys 83 us and a merge of 5, over 300 keys of 28 /
-// 4 heads of 128 9.9, of 16 / 2 heads of 256 14.3.  A short call is a chain: 1.6 us to the piece, 2
-// to issue two blocks' loads (64 of them at head_dim 256: 4 to 6), 1 to 2 for a
-// block and 1.5 to join the waves.
+// TB/s; one token over 131072 keys 83 us and a merge of 5, over 320 keys of 28 /
+// 4 heads of 128 7.4, of 16 / 2 heads of 256 14.1.  A short call is a chain: 1.6
+// us to the piece, 2 to issue two blocks' loads (64 of them at head_dim 256: 4 to
+// 6), 1 to 2 for a block and 1.5 to join the waves.
 #include "common.hpp"
 #include "internal.hpp"
 #include "paged_items.hpp"
@@ -469,11 +470,20 @@ __global__ __launch_bounds__(256) void paged_decode_merge_kernel(PagedAttnArgs a
     store_out4(a.out, row * a.out_stride + col, a.out_dtype, v);
 }
 
-// Cutting an item costs two partial results and the merge's launch (4 us): one
-// whose K and V take at most this many bytes per kv head is not cut.
-constexpr uint32_t kWholeBytes = 160 * 1024;
+// Cutting an item costs two partial results and the merge's launch (4 us).
+// Where no item's K and V take more than this many bytes per kv head, none is
+// cut: whole and cut, us for one sequence: 14 / 2 heads of 64, 768 keys 7.3 and
+// 8.6, 1024 8.6 and 8.7; 28 / 4 of 128, 512 keys 9.1 and 10.3, 640 10.8 and
+// 10.4; 16 / 2 of 256, 256 keys 11.7 and 15.0, 384 15.6 and 14.9.  (64 sequences:
+// 512 keys at 128 12.7 and 23.8, 256 at 256 13.3 and 19.6.)
+constexpr uint32_t kWholeBytes = 256 * 1024;
+// On the line, beside longer ones, fewer: there the merge comes anyway and items
+// that are not cut make chunks uneven (200 sequences of up to 3000 keys, 14 / 2
+// heads of 64: 31.1 us, 37.6 with the bytes above; 64 of up to 2000, 28 / 4 of
+// 128: 32.6 and 37.2).
+constexpr uint32_t kSnapBytes = 160 * 1024;
 
-uint32_t snap_units(uint32_t D) { return kWholeBytes / (4 * D * kUnit); }
+uint32_t units_of_bytes(uint32_t bytes, uint32_t D) { return bytes / (4 * D * kUnit); }
 
 size_t align256d(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -482,7 +492,7 @@ size_t align256d(size_t x) { return (x + 255) / 256 * 256; }
 uint32_t decode_wgs(uint32_t n_seq, uint32_t max_len, uint32_t n_kv, uint32_t D)
 {
     const uint32_t units = (max_len + kUnit - 1) / kUnit;
-    if (units <= snap_units(D)) return 0;  // no item is cut: a workgroup each
+    if (units <= units_of_bytes(kWholeBytes, D)) return 0;  // no item is cut: a workgroup each
     const uint64_t most = (uint64_t)n_seq * n_kv * (units + kDecodeItemUnits);
     const uint64_t full = (uint64_t)(D <= 128 ? 2 : 1) * (uint64_t)n_cus();
     return (uint32_t)(((most < full ? most : full) + 7) / 8 * 8);
@@ -522,7 +532,7 @@ hipError_t launch_paged_decode(const PagedAttnArgs& in, hipStream_t st)
     PagedAttnArgs a = in;
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
     a.n_wg = decode_wgs(a.n_seq, a.max_len, a.n_kv, a.D);
-    a.snap_units = snap_units(a.D);
+    a.snap_units = units_of_bytes(kSnapBytes, a.D);
     a.min_units = 1 + kDecodeItemUnits;
     char* p = reinterpret_cast<char*>(a.ws);
     a.desc = p;
