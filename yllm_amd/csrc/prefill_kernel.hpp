@@ -379,7 +379,11 @@ __device__ inline bool split_item(const PrefillArgs& a, PItem& I)
 // A = PagedAttnArgs: the items and key pages of paged attention
 // (paged_items.hpp); a workgroup walks its chunk's pieces of items as the
 // plain mode walks items.  fp32 queries then also take their probabilities as
-// f16 hi + lo parts (PS), so that the output keeps fp32-level error.
+// f16 hi + lo parts (PS), so that the output keeps fp32-level error.  16-bit ones
+// take f16 alone, half a step (2^-11) for each: the lo parts' products cost 604
+// -> 972 us for a prompt of 8192 tokens of 32 / 8 heads of 128 and 83 -> 110 for a
+// mixed step, and gain 2.6e-4 -> 2.0e-4 of relative error in f16, 1.67e-3 ->
+// 1.66e-3 in bf16, whose outputs' own rounding is 2.0e-4 and 1.65e-3 of it.
 template <int D, int NG, bool SPLIT, bool QS = false, class A = PrefillArgs>
 __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 && !QS) ? 2 : 1) void prefill_kernel(A args)
 {
@@ -1195,7 +1199,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
 // 4096 tokens, 16 / 2 heads, bf16, gated: 215 -> 170 us (808 TFLOP/s), ungated
 // 188 -> 153.  (The gate is the fp32 sigmoid of the other kernels; by the
 // approximate reciprocal of 1 + exp2 it took 6 us less and was up to 3.5e-6
-// off at gates of -60, 2.3e-7 now.)
+// off at gates of -60, 2.3e-7 now.)  The probabilities are f16, as there; their
+// lo parts would need 16 KB of LDS more than is left (150 KB of 160 are taken).
 //
 // Step t starts with the raw scores of tile t in registers and their maxima
 // in LDS.  The next tile's score MFMAs begin; the pair's common maximum is

@@ -14,8 +14,10 @@
 // The row's slot says where K and V go: page slot / block, row slot % block.
 // Rows without a slot (negative, or past the pool) are skipped.
 //
-// Bound by HBM and, half as much, by its arithmetic: each row is read once and
-// written once.  A lane holds eight elements of a head as two runs of four, with
+// Each row is read once and written once; few rows are bound by the launch and
+// two round trips, many by the latency of their loads: a wave loads its passes,
+// waits, computes, stores and ends, and nothing of another row is in flight
+// meanwhile.  A lane holds eight elements of a head as two runs of four, with
 // neighbouring lanes' runs next to each other (eight in one run left every load
 // and store with holes), and the pairs of every rope kind within one lane; so a
 // head is D / 8 lanes, a wave takes 64 / (D / 8) heads a pass, and the sum of
@@ -24,10 +26,11 @@
 // workgroups of their own (a few rows: by the same waves, 2 bytes at a time).
 //
 // Measured: 8193 tokens of three prompts, 16 / 2 heads of 256 (M-RoPE over 64),
-// bf16: 43.7 us, 3.8 TB/s, where a large copy reaches 5.4; 480 VALU instructions
-// a wave (some of them 64 bits wide) are 22 us of that time.  Three passes a wave
-// and four waves a SIMD: one pass 54 us, two 46, five 45; six waves a SIMD spill,
-// 50.  One decode token or 64: 5 us of GPU time, the launch and two round trips.
+// bf16: 43.8 us, 3.8 TB/s, where a large copy reaches 5.4 (31 us); 480 VALU
+// instructions a wave (some of them 64 bits wide) are 22 us, and 61 % of the wave
+// cycles wait.  Three passes a wave and four waves a SIMD: one pass 54 us, two 46,
+// five 45; six waves a SIMD spill, 50.  One decode token 4.7 us of GPU time, 64 of
+// 32 / 8 heads of 128 6.1.
 #include "common.hpp"
 #include "internal.hpp"
 

@@ -114,7 +114,8 @@ def paged_plan(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torc
     new_lens[i] tokens (all int32 on the GPU).  block_table [n_seq, max_blocks] gets the entries of the new blocks,
     which come from the end of free_blocks[:n_free[0]]; n_tok rows get a slot and a position (padding: -1 and 0).
     counts[:1] is the n_free of the next step; a sequence that could not be served in whole has kv_lens 0 and slots of
-    -1 (yhip_paged_plan has the rules).  `out`: the tensors of an earlier step, overwritten."""
+    -1 (yhip_paged_plan has the rules).  `out`: the tensors of an earlier step, overwritten; the inputs must not be among
+    them, so its counts[:1] and kv_lens are first copied (n_free.copy_(out.counts[:1])) to tensors of their own."""
     fn = "paged_plan"
     n, w, stride = _table(fn, block_table)
     _ints(fn, "ctx_lens", ctx_lens, n)
