@@ -195,3 +195,13 @@ def test_attn_overlaps(hiplib, kw):
 def test_store_overlaps(hiplib, kw):
     """What the call writes (the queries, the pools) is neither what it reads (q_out may be q) nor each other."""
     assert hiplib.yhip_qk_norm_rope_kv_store(*store_args(**kw)) == -22 and "overlap" in _err(hiplib)
+
+
+@pytest.mark.parametrize("kw", [{}, {"max_new": 5}, {"d": 64, "os": 512, "qs": 512}])
+def test_attn_workspace_of_calls_that_need_one(hiplib, kw):
+    kw = dict(w=64, stride=64, max_len=4096, **kw)
+    a = dict(zip(("T", "n", "max_new", "max_len", "nh", "nkv", "d"), (5, 3, kw.get("max_new", 2), 4096, 8, 2, kw.get("d", 128))))
+    need = hiplib.yhip_paged_attn_workspace(*a.values())
+    assert need > 0
+    for ws, n in ((None, need), (_at(1 << 40), need - 1), (_at(1 << 40), 0), (_at((1 << 40) + 8), need)):
+        assert hiplib.yhip_paged_attn(*attn_args(**kw, ws=ws, wsb=n)) == -28 and "workspace" in _err(hiplib)
