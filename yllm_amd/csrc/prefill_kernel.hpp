@@ -1200,7 +1200,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
 // 188 -> 153.  (The gate is the fp32 sigmoid of the other kernels; by the
 // approximate reciprocal of 1 + exp2 it took 6 us less and was up to 3.5e-6
 // off at gates of -60, 2.3e-7 now.)  The probabilities are f16, as there; their
-// lo parts would need 16 KB of LDS more than is left (150 KB of 160 are taken).
+// lo parts would need 16 KB of LDS more (146 of 160 KB are taken).
 //
 // Step t starts with the raw scores of tile t in registers and their maxima
 // in LDS.  The next tile's score MFMAs begin; the pair's common maximum is
