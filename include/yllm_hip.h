@@ -318,6 +318,59 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
 size_t yhip_paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
                                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 
+/* ---- Paged KV cache in 8 bits ------------------------------------------------
+ * The same pool with half the bytes.  Per layer:
+ *   K : codes [n_blocks][n_kv_heads][block][head_dim]        (e4m3)
+ *   V : codes [n_blocks][n_kv_heads][block/64][head_dim][64] (e4m3)
+ *   scales of K and of V [n_blocks][n_kv_heads][block]       (e5m2)
+ * A value is its code (OCP e4m3: no infinity) times the scale of its position
+ * and kv head, a power of two 2^k.  With amax the largest finite magnitude of
+ * the head_dim values, k is ceil(log2(amax / 448)) within -14..7, and a code
+ * is x * 2^-k rounded to nearest even, +-448 where x lies beyond (only past
+ * 57344), NaN where x is infinite or NaN.  Every value held is a f16 number
+ * exactly (e5m2 is the upper byte of f16).  A row's bytes depend on that row
+ * alone: on no other row, call or order.  block is a power of two in
+ * 64..65536 (yhip_qk_norm_rope_kv8_store: a multiple of 64); pools are
+ * 16-byte aligned.  Plans, tables, slots and lengths as above.
+ *
+ * Append: yhip_qk_norm_rope_kv_store into that pool (its arguments, rules and
+ * queries; K and V are quantised from the fp32 results). */
+int yhip_qk_norm_rope_kv8_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
+                                uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                                uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
+                                uint32_t norm_dtype, float eps, uint8_t* kpool, uint8_t* vpool, uint8_t* kscale,
+                                uint8_t* vscale, uint32_t n_blocks, uint32_t block, const int32_t* positions,
+                                const int32_t* slots, uint32_t pos_start, uint32_t n_tok, uint32_t n_heads,
+                                uint32_t n_kv_heads, uint32_t head_dim, uint32_t rope, uint32_t n_rot, float theta,
+                                void* stream);
+
+/* Attention: yhip_paged_attn over that pool (its arguments, rules, types,
+ * bounds and precision, with the held values as K and V). */
+int yhip_paged_attn8(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                     uint32_t q_stride, const uint8_t* kpool, const uint8_t* vpool, const uint8_t* kscale,
+                     const uint8_t* vscale, uint32_t n_blocks, uint32_t block, const int32_t* block_table,
+                     uint32_t max_blocks, uint32_t table_stride, const int32_t* kv_lens, const int32_t* cu_new,
+                     uint32_t n_seq, uint32_t n_tok, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                     uint32_t n_kv_heads, uint32_t head_dim, const float* gate, uint32_t gate_stride, void* workspace,
+                     size_t workspace_bytes, void* stream);
+size_t yhip_paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
+                                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Whole pages between the two pools (a prompt computed on f16 pages kept in 8
+ * bits; a sequence handed out in f16, exactly): page dst[i] of the one gets
+ * what page src[i] of the other holds, i < n_pages (int32 in DEVICE memory).
+ * A pair with a page outside its pool is skipped; each dst at most once.  Both
+ * pools have pages of `block` positions; no overlap of what is written with
+ * anything else. */
+int yhip_kv8_from_pages(uint8_t* kpool8, uint8_t* vpool8, uint8_t* kscale, uint8_t* vscale, uint32_t n_blocks8,
+                        const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks, const int32_t* dst,
+                        const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv_heads, uint32_t head_dim,
+                        void* stream);
+int yhip_kv8_to_pages(uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks, const uint8_t* kpool8,
+                      const uint8_t* vpool8, const uint8_t* kscale, const uint8_t* vscale, uint32_t n_blocks8,
+                      const int32_t* dst, const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv_heads,
+                      uint32_t head_dim, void* stream);
+
 /* ---- o_proj (the step after attention) -------------------------------------
  * x[b] += W_o . att[b] for B tokens: matmul(att_out, x2, SLOT_O) then the
  * residual add (engine.c:969-973; qwen35 after its gate, 958-973), with

@@ -70,6 +70,17 @@ SIGNATURES = {
                                 c_uint32, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p] + [c_uint32] * 7 +
                         [c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
     "yhip_paged_attn_workspace": (c_size_t, [c_uint32] * 7),
+    "yhip_qk_norm_rope_kv8_store": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_void_p, c_uint32, c_void_p,
+                                            c_uint32, c_uint32, c_void_p, c_void_p, c_uint32, c_float] + [c_void_p] * 4 +
+                                    [c_uint32, c_uint32, c_void_p, c_void_p] + [c_uint32] * 7 + [c_float, c_void_p]),
+    "yhip_paged_attn8": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32] + [c_void_p] * 4 +
+                         [c_uint32, c_uint32, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p] + [c_uint32] * 7 +
+                         [c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
+    "yhip_paged_attn8_workspace": (c_size_t, [c_uint32] * 7),
+    "yhip_kv8_from_pages": (c_int, [c_void_p] * 4 + [c_uint32, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p] +
+                            [c_uint32] * 4 + [c_void_p]),
+    "yhip_kv8_to_pages": (c_int, [c_void_p, c_void_p, c_uint32] + [c_void_p] * 4 + [c_uint32, c_void_p, c_void_p] +
+                          [c_uint32] * 4 + [c_void_p]),
     "yhip_synth_normal": (None, [c_uint64, c_uint64, c_float, POINTER(c_float), c_uint64]),
     "yhip_synth_round_f16": (None, [POINTER(c_float), c_uint64]),
     "yhip_synth_round_bf16": (None, [POINTER(c_float), c_uint64]),

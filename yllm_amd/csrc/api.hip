@@ -750,19 +750,34 @@ int yhip_paged_plan(int32_t* block_table, uint32_t max_blocks, uint32_t table_st
     return done(yhip::launch_paged_plan(a, (hipStream_t)stream), fn);
 }
 
-int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
-                               uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
-                               uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
-                               uint32_t norm_dtype, float eps, uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks,
-                               uint32_t block, const int32_t* positions, const int32_t* slots, uint32_t pos_start,
-                               uint32_t n_tok, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
-                               uint32_t rope, uint32_t n_rot, float theta, void* stream)
+}  // extern "C"
+
+namespace {
+
+// bytes that a call writes (or reads)
+struct Span {
+    const void* p;
+    uint64_t n;
+};
+
+// The checks of the two stores, and a's fields but the pools.  pools: what the call writes beside q_out (K, V, and the
+// scales of the 8-bit pool).  1: nothing to do.
+int store_common(const char* fn, yhip::QkNormRopeArgs& a, const Span* pools, int n_pools, void* q_out, uint32_t q_out_dtype,
+                 uint32_t q_out_stride, const void* q, uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                 uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm, uint32_t norm_dtype, float eps,
+                 uint32_t n_blocks, uint32_t block, const int32_t* positions, const int32_t* slots, uint32_t pos_start,
+                 uint32_t n_tok, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t rope, uint32_t n_rot,
+                 float theta)
 {
-    const char* fn = "yhip_qk_norm_rope_kv_store";
     // (one kv head's page takes the place of its contiguous cache)
     if (block == 0 || block % 64) return fail(YHIP_EINVAL, "%s: block %u must be a positive multiple of 64", fn, block);
     if (int rc = check_heads(fn, n_heads, n_kv_heads, head_dim, block)) return rc;
-    if (n_tok && (!k || !v || !kpool || !vpool || (q_out && !q))) return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    bool null_pool = false, bad_pool = false;
+    for (int i = 0; i < n_pools; ++i) {
+        null_pool = null_pool || !pools[i].p;
+        bad_pool = bad_pool || (uintptr_t)pools[i].p % 16;
+    }
+    if (n_tok && (!k || !v || null_pool || (q_out && !q))) return fail(YHIP_EINVAL, "%s: null pointer", fn);
     if (!q_norm != !k_norm) return fail(YHIP_EINVAL, "%s: q_norm and k_norm come together", fn);
     if (!valid_dtype(dtype) || (q_out && !valid_dtype(q_out_dtype))) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
     if (q_norm && norm_dtype != YHIP_F32 && norm_dtype != YHIP_F16)
@@ -786,14 +801,17 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
     // runs of four elements move as one access
     const uint32_t al = dtype == YHIP_F32 ? 16u : 8u, qo_al = q_out_dtype == YHIP_F32 ? 16u : 8u,
                    w_al = norm_dtype == YHIP_F32 ? 16u : 8u;
-    if ((uintptr_t)k % al || (uintptr_t)v % al || (uintptr_t)kpool % 16 || (uintptr_t)vpool % 16 || k_stride % 4 ||
+    if ((uintptr_t)k % al || (uintptr_t)v % al || bad_pool || k_stride % 4 ||
         v_stride % 4 || (q_out && ((uintptr_t)q % al || (uintptr_t)q_out % qo_al || q_stride % 4 || q_out_stride % 4)) ||
         (q_norm && ((uintptr_t)q_norm % w_al || (uintptr_t)k_norm % w_al)))
         return fail(YHIP_EINVAL, "%s: rows, weights and pools must be aligned to four elements (pools to 16 bytes)", fn);
-    if (n_tok == 0) return done(hipSuccess, "");
+    if (n_tok == 0) {
+        done(hipSuccess, "");
+        return 1;
+    }
     // nothing that the call writes is read by it (q_out may be q itself) or written twice
     const yhip::Rows rk = rows_of(k, dtype, k_stride, kv_dim, n_tok), rv = rows_of(v, dtype, v_stride, kv_dim, n_tok);
-    const uint64_t pool = 2ull * n_blocks * block * kv_dim, w_bytes = q_norm ? (norm_dtype == YHIP_F32 ? 4ull : 2ull) * head_dim : 0,
+    const uint64_t w_bytes = q_norm ? (norm_dtype == YHIP_F32 ? 4ull : 2ull) * head_dim : 0,
                    row_ints = 4ull * n_tok;
     if (q_out) {
         const yhip::Rows ro = rows_of(q_out, q_out_dtype, q_out_stride, qd, n_tok), rq = rows_of(q, dtype, q_stride, qd, n_tok);
@@ -801,21 +819,23 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
         if ((!same && rows_overlap(ro, rq)) || rows_overlap(ro, rk) || rows_overlap(ro, rv) || hits(ro, q_norm, w_bytes) ||
             hits(ro, k_norm, w_bytes) || hits(ro, positions, row_ints) || hits(ro, slots, row_ints))
             return fail(YHIP_EINVAL, "%s: q_out overlaps its inputs (it may be q itself, of the same type and stride)", fn);
-        if (hits(ro, kpool, pool) || hits(ro, vpool, pool) || hits(rq, kpool, pool) || hits(rq, vpool, pool))
-            return fail(YHIP_EINVAL, "%s: a pool overlaps q or q_out", fn);
+        for (int i = 0; i < n_pools; ++i)
+            if (hits(ro, pools[i].p, pools[i].n) || hits(rq, pools[i].p, pools[i].n))
+                return fail(YHIP_EINVAL, "%s: a pool overlaps q or q_out", fn);
     }
-    if (overlap(kpool, pool, vpool, pool)) return fail(YHIP_EINVAL, "%s: the pools overlap", fn);
-    for (const uint16_t* p : {kpool, vpool})
-        if (hits(rk, p, pool) || hits(rv, p, pool) || overlap(p, pool, q_norm, w_bytes) || overlap(p, pool, k_norm, w_bytes) ||
-            overlap(p, pool, positions, positions ? row_ints : 0) || overlap(p, pool, slots, slots ? row_ints : 0))
+    for (int i = 0; i < n_pools; ++i) {
+        const void* const p = pools[i].p;
+        const uint64_t n = pools[i].n;
+        for (int j = 0; j < i; ++j)
+            if (overlap(p, n, pools[j].p, pools[j].n)) return fail(YHIP_EINVAL, "%s: the pools overlap", fn);
+        if (hits(rk, p, n) || hits(rv, p, n) || overlap(p, n, q_norm, w_bytes) || overlap(p, n, k_norm, w_bytes) ||
+            overlap(p, n, positions, positions ? row_ints : 0) || overlap(p, n, slots, slots ? row_ints : 0))
             return fail(YHIP_EINVAL, "%s: a pool overlaps the call's inputs", fn);
-    yhip::QkNormRopeArgs a = {};
+    }
     a.q_out = q_out;
     a.q = q;
     a.k = k;
     a.v = v;
-    a.kc = kpool;
-    a.vc = vpool;
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.positions = positions;
@@ -850,7 +870,56 @@ int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out
         }
         memcpy(a.turns, t_turns, sizeof(double) * (a.n_rot / 2));
     }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int yhip_qk_norm_rope_kv_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
+                               uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                               uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
+                               uint32_t norm_dtype, float eps, uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks,
+                               uint32_t block, const int32_t* positions, const int32_t* slots, uint32_t pos_start,
+                               uint32_t n_tok, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               uint32_t rope, uint32_t n_rot, float theta, void* stream)
+{
+    const char* fn = "yhip_qk_norm_rope_kv_store";
+    yhip::QkNormRopeArgs a = {};
+    const uint64_t pool = 2ull * n_blocks * block * n_kv_heads * head_dim;
+    const Span pools[] = {{kpool, pool}, {vpool, pool}};
+    if (int rc = store_common(fn, a, pools, 2, q_out, q_out_dtype, q_out_stride, q, q_stride, k, k_stride, v, v_stride, dtype,
+                              q_norm, k_norm, norm_dtype, eps, n_blocks, block, positions, slots, pos_start, n_tok, n_heads,
+                              n_kv_heads, head_dim, rope, n_rot, theta))
+        return rc > 0 ? YHIP_OK : rc;
+    a.kc = kpool;
+    a.vc = vpool;
     return done(yhip::launch_qk_norm_rope(a, (hipStream_t)stream), fn);
+}
+
+int yhip_qk_norm_rope_kv8_store(void* q_out, uint32_t q_out_dtype, uint32_t q_out_stride, const void* q,
+                                uint32_t q_stride, const void* k, uint32_t k_stride, const void* v,
+                                uint32_t v_stride, uint32_t dtype, const void* q_norm, const void* k_norm,
+                                uint32_t norm_dtype, float eps, uint8_t* kpool, uint8_t* vpool, uint8_t* kscale,
+                                uint8_t* vscale, uint32_t n_blocks, uint32_t block, const int32_t* positions,
+                                const int32_t* slots, uint32_t pos_start, uint32_t n_tok, uint32_t n_heads,
+                                uint32_t n_kv_heads, uint32_t head_dim, uint32_t rope, uint32_t n_rot, float theta,
+                                void* stream)
+{
+    const char* fn = "yhip_qk_norm_rope_kv8_store";
+    yhip::QkNormRope8Args a = {};
+    const uint64_t rows = (uint64_t)n_blocks * block * n_kv_heads, pool = rows * head_dim;
+    const Span pools[] = {{kpool, pool}, {vpool, pool}, {kscale, rows}, {vscale, rows}};
+    if (int rc = store_common(fn, a, pools, 4, q_out, q_out_dtype, q_out_stride, q, q_stride, k, k_stride, v, v_stride, dtype,
+                              q_norm, k_norm, norm_dtype, eps, n_blocks, block, positions, slots, pos_start, n_tok, n_heads,
+                              n_kv_heads, head_dim, rope, n_rot, theta))
+        return rc > 0 ? YHIP_OK : rc;
+    a.kc = reinterpret_cast<uint16_t*>(kpool);
+    a.vc = reinterpret_cast<uint16_t*>(vpool);
+    a.ks = kscale;
+    a.vs = vscale;
+    return done(yhip::launch_qk_norm_rope8(a, (hipStream_t)stream), fn);
 }
 
 size_t yhip_paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
@@ -860,15 +929,26 @@ size_t yhip_paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_ne
     return yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
 }
 
-int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
-                    uint32_t q_stride, const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks,
-                    uint32_t block, const int32_t* block_table, uint32_t max_blocks, uint32_t table_stride,
-                    const int32_t* kv_lens, const int32_t* cu_new, uint32_t n_seq, uint32_t n_tok, uint32_t max_new,
-                    uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float* gate,
-                    uint32_t gate_stride, void* workspace, size_t workspace_bytes, void* stream)
+}  // extern "C"
+
+namespace {
+
+// The checks of the two attentions, and a's fields but the pools (at most four, which the call reads); `bytes`: the
+// workspace that it needs.  1: nothing to do.
+int paged_attn_common(const char* fn, yhip::PagedAttnArgs& a, const Span* pools, int n_pools, decltype(yhip::paged_attn_workspace)* bytes,
+                      void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                      uint32_t q_stride, uint32_t n_blocks, uint32_t block, const int32_t* block_table, uint32_t max_blocks,
+                      uint32_t table_stride, const int32_t* kv_lens, const int32_t* cu_new, uint32_t n_seq, uint32_t n_tok,
+                      uint32_t max_new, uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                      const float* gate, uint32_t gate_stride, void* workspace, size_t workspace_bytes)
 {
-    const char* fn = "yhip_paged_attn";
-    if (n_tok && n_seq && (!att_out || !q || !kpool || !vpool || !block_table || !kv_lens || !cu_new))
+    bool null_pool = false;
+    uintptr_t pool_bits = 0;
+    for (int i = 0; i < n_pools; ++i) {
+        null_pool = null_pool || !pools[i].p;
+        pool_bits |= (uintptr_t)pools[i].p;
+    }
+    if (n_tok && n_seq && (!att_out || !q || null_pool || !block_table || !kv_lens || !cu_new))
         return fail(YHIP_EINVAL, "%s: null pointer", fn);
     if (!valid_dtype(out_dtype) || !valid_dtype(q_dtype)) return fail(YHIP_EINVAL, "%s: bad dtype", fn);
     uint32_t shift;
@@ -886,9 +966,12 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8)
         return fail(YHIP_EINVAL, "%s: q_stride/out_stride must be >= n_heads*head_dim and a multiple of 8", fn);
     if (gate && gate_stride < row) return fail(YHIP_EINVAL, "%s: gate_stride too small", fn);
-    if (((uintptr_t)q | (uintptr_t)att_out | (uintptr_t)kpool | (uintptr_t)vpool) % 16)
+    if (((uintptr_t)q | (uintptr_t)att_out | pool_bits) % 16)
         return fail(YHIP_EINVAL, "%s: q, att_out and the pools must be 16-byte aligned", fn);
-    if (n_tok == 0 || n_seq == 0 || max_new == 0) return done(hipSuccess, "");
+    if (n_tok == 0 || n_seq == 0 || max_new == 0) {
+        done(hipSuccess, "");
+        return 1;
+    }
     const yhip::Rows ro = rows_of(att_out, out_dtype, out_stride, row, n_tok), rq = rows_of(q, q_dtype, q_stride, row, n_tok),
                      rg = rows_of(gate, YHIP_F32, gate_stride, row, n_tok);
     if (rows_overlap(ro, rq) || (gate && rows_overlap(ro, rg)))
@@ -900,13 +983,12 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     if ((nb * (tiles + nb + 8) + tiles) * gmax * n_kv_heads >= 1ull << 31 || items * (tiles + 8) >= 1ull << 38)
         return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
                     max_new, max_len);
-    const struct { const void* p; uint64_t n; } in[] = {
-        {kpool, 2ull * n_blocks * n_kv_heads * block * head_dim}, {vpool, 2ull * n_blocks * n_kv_heads * block * head_dim},
-        {block_table, 4ull * ((n_seq - 1ull) * table_stride + max_blocks)}, {kv_lens, 4ull * n_seq}, {cu_new, 4ull * n_seq + 4}};
+    Span in[7] = {{block_table, 4ull * ((n_seq - 1ull) * table_stride + max_blocks)}, {kv_lens, 4ull * n_seq}, {cu_new, 4ull * n_seq + 4}};
+    for (int i = 0; i < n_pools; ++i) in[3 + i] = pools[i];
     bool clash = false;
     for (const auto& i : in) clash = clash || hits(ro, i.p, i.n);
     if (clash) return fail(YHIP_EINVAL, "%s: att_out overlaps its inputs", fn);
-    const size_t need = yhip::paged_attn_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
+    const size_t need = bytes(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(YHIP_ENOSPC, "%s: %zu bytes of workspace (16-byte aligned) needed, %zu given", fn, need,
                     workspace_bytes);
@@ -915,12 +997,9 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
         for (const auto& i : in) clash = clash || overlap(workspace, need, i.p, i.n);
         if (clash) return fail(YHIP_EINVAL, "%s: the workspace overlaps the call's tensors", fn);
     }
-    yhip::PagedAttnArgs a = {};
     a.q = q;
     a.q_dtype = q_dtype;
     a.q_stride = q_stride;
-    a.kc = kpool;
-    a.vc = vpool;
     a.table = block_table;
     a.kv_lens = kv_lens;
     a.cu_new = cu_new;
@@ -941,7 +1020,137 @@ int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, cons
     a.n_blocks = n_blocks;
     a.c = (float)(1.4426950408889634 / sqrt((double)head_dim));
     a.ws = need ? workspace : nullptr;
+    return 0;
+}
+
+// The checks of the two copies of pages, and their arguments (`from`: into the 8-bit pool).  1: nothing to do.
+int pages_common(const char* fn, yhip::Kv8PagesArgs& a, bool from, const uint8_t* k8, const uint8_t* v8, const uint8_t* ks,
+                 const uint8_t* vs, uint32_t n_blocks8, const uint16_t* kc, const uint16_t* vc, uint32_t n_blocks,
+                 const int32_t* dst, const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv, uint32_t head_dim)
+{
+    uint32_t shift;
+    if (int rc = block_shift(fn, block, shift)) return rc;
+    if (!valid_head_dim(head_dim) || n_kv == 0)
+        return fail(YHIP_EINVAL, "%s: bad n_kv_heads %u / head_dim %u", fn, n_kv, head_dim);
+    if (n_pages && (!k8 || !v8 || !ks || !vs || !kc || !vc || !dst || !src)) return fail(YHIP_EINVAL, "%s: null pointer", fn);
+    if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)ks | (uintptr_t)vs | (uintptr_t)kc | (uintptr_t)vc) % 16)
+        return fail(YHIP_EINVAL, "%s: pools must be 16-byte aligned", fn);
+    if ((uint64_t)n_blocks * n_kv > 0xffffffffull || (uint64_t)n_blocks8 * n_kv > 0xffffffffull ||
+        n_pages > 0x7fffffffu || (uint64_t)n_pages * n_kv > 0x7fffffffull / (block / 64))
+        return fail(YHIP_EINVAL, "%s: too many pages", fn);
+    if (n_pages == 0) {
+        done(hipSuccess, "");
+        return 1;
+    }
+    const uint64_t r8 = (uint64_t)n_blocks8 * n_kv * block, rf = (uint64_t)n_blocks * n_kv * block * 2;
+    const Span all[] = {{k8, r8 * head_dim}, {v8, r8 * head_dim}, {ks, r8}, {vs, r8}, {kc, rf * head_dim}, {vc, rf * head_dim},
+                        {dst, 4ull * n_pages}, {src, 4ull * n_pages}};
+    const int w0 = from ? 0 : 4, w1 = from ? 4 : 6;  // those that are written
+    for (int i = w0; i < w1; ++i)
+        for (int j = 0; j < 8; ++j)
+            if (i != j && overlap(all[i].p, all[i].n, all[j].p, all[j].n))
+                return fail(YHIP_EINVAL, "%s: a pool that is written overlaps another tensor", fn);
+    a.kc = const_cast<uint16_t*>(kc);
+    a.vc = const_cast<uint16_t*>(vc);
+    a.k8 = const_cast<uint8_t*>(k8);
+    a.v8 = const_cast<uint8_t*>(v8);
+    a.ks = const_cast<uint8_t*>(ks);
+    a.vs = const_cast<uint8_t*>(vs);
+    a.dst = dst;
+    a.src = src;
+    a.n = n_pages;
+    a.n_f16 = n_blocks;
+    a.n_8 = n_blocks8;
+    a.n_kv = n_kv;
+    a.D = head_dim;
+    a.block = block;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int yhip_paged_attn(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                    uint32_t q_stride, const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks,
+                    uint32_t block, const int32_t* block_table, uint32_t max_blocks, uint32_t table_stride,
+                    const int32_t* kv_lens, const int32_t* cu_new, uint32_t n_seq, uint32_t n_tok, uint32_t max_new,
+                    uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float* gate,
+                    uint32_t gate_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* fn = "yhip_paged_attn";
+    yhip::PagedAttnArgs a = {};
+    const uint64_t pool = 2ull * n_blocks * n_kv_heads * block * head_dim;
+    const Span pools[] = {{kpool, pool}, {vpool, pool}};
+    if (int rc = paged_attn_common(fn, a, pools, 2, yhip::paged_attn_workspace, att_out, out_dtype, out_stride, q, q_dtype,
+                                   q_stride, n_blocks, block, block_table, max_blocks, table_stride, kv_lens, cu_new, n_seq,
+                                   n_tok, max_new, max_len, n_heads, n_kv_heads, head_dim, gate, gate_stride, workspace,
+                                   workspace_bytes))
+        return rc > 0 ? YHIP_OK : rc;
+    a.kc = kpool;
+    a.vc = vpool;
     return done(yhip::launch_paged_attn(a, (hipStream_t)stream), fn);
+}
+
+size_t yhip_paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len,
+                                  uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim)
+{
+    if (n_kv_heads == 0 || !valid_head_dim(head_dim)) return 0;
+    return yhip::paged_attn8_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv_heads, head_dim);
+}
+
+int yhip_paged_attn8(void* att_out, uint32_t out_dtype, uint32_t out_stride, const void* q, uint32_t q_dtype,
+                     uint32_t q_stride, const uint8_t* kpool, const uint8_t* vpool, const uint8_t* kscale,
+                     const uint8_t* vscale, uint32_t n_blocks, uint32_t block, const int32_t* block_table,
+                     uint32_t max_blocks, uint32_t table_stride, const int32_t* kv_lens, const int32_t* cu_new,
+                     uint32_t n_seq, uint32_t n_tok, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                     uint32_t n_kv_heads, uint32_t head_dim, const float* gate, uint32_t gate_stride, void* workspace,
+                     size_t workspace_bytes, void* stream)
+{
+    const char* fn = "yhip_paged_attn8";
+    yhip::PagedAttn8Args a = {};
+    const uint64_t rows = (uint64_t)n_blocks * n_kv_heads * block, pool = rows * head_dim;
+    const Span pools[] = {{kpool, pool}, {vpool, pool}, {kscale, rows}, {vscale, rows}};
+    if (int rc = paged_attn_common(fn, a, pools, 4, yhip::paged_attn8_workspace, att_out, out_dtype, out_stride, q, q_dtype,
+                                   q_stride, n_blocks, block, block_table, max_blocks, table_stride, kv_lens, cu_new, n_seq,
+                                   n_tok, max_new, max_len, n_heads, n_kv_heads, head_dim, gate, gate_stride, workspace,
+                                   workspace_bytes))
+        return rc > 0 ? YHIP_OK : rc;
+    // (units of one sequence's row blocks, paged_decode8.hip)
+    if ((((uint64_t)n_heads + n_kv_heads - 1) / n_kv_heads * max_new / 16 + 1) * n_kv_heads * (max_len / 256 + 2ull) >= 1ull << 31)
+        return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
+                    max_new, max_len);
+    a.kc = reinterpret_cast<const uint16_t*>(kpool);
+    a.vc = reinterpret_cast<const uint16_t*>(vpool);
+    a.ks = kscale;
+    a.vs = vscale;
+    return done(yhip::launch_paged_attn8(a, (hipStream_t)stream), fn);
+}
+
+int yhip_kv8_from_pages(uint8_t* kpool8, uint8_t* vpool8, uint8_t* kscale, uint8_t* vscale, uint32_t n_blocks8,
+                        const uint16_t* kpool, const uint16_t* vpool, uint32_t n_blocks, const int32_t* dst,
+                        const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv_heads, uint32_t head_dim,
+                        void* stream)
+{
+    const char* fn = "yhip_kv8_from_pages";
+    yhip::Kv8PagesArgs a = {};
+    if (int rc = pages_common(fn, a, true, kpool8, vpool8, kscale, vscale, n_blocks8, kpool, vpool, n_blocks, dst, src,
+                              n_pages, block, n_kv_heads, head_dim))
+        return rc > 0 ? YHIP_OK : rc;
+    return done(yhip::launch_kv8_from_pages(a, (hipStream_t)stream), fn);
+}
+
+int yhip_kv8_to_pages(uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks, const uint8_t* kpool8,
+                      const uint8_t* vpool8, const uint8_t* kscale, const uint8_t* vscale, uint32_t n_blocks8,
+                      const int32_t* dst, const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv_heads,
+                      uint32_t head_dim, void* stream)
+{
+    const char* fn = "yhip_kv8_to_pages";
+    yhip::Kv8PagesArgs a = {};
+    if (int rc = pages_common(fn, a, false, kpool8, vpool8, kscale, vscale, n_blocks8, kpool, vpool, n_blocks, dst, src,
+                              n_pages, block, n_kv_heads, head_dim))
+        return rc > 0 ? YHIP_OK : rc;
+    return done(yhip::launch_kv8_to_pages(a, (hipStream_t)stream), fn);
 }
 
 }  // extern "C"

@@ -169,6 +169,28 @@ struct QkNormRopeArgs {
     double turns[128];
 };
 hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st);
+// into the 8-bit pool (kv8.hpp): kc and vc are its codes
+struct QkNormRope8Args : QkNormRopeArgs {
+    uint8_t* ks;            // scales of K and V [n_blocks][n_kv][block]
+    uint8_t* vs;
+};
+hipError_t launch_qk_norm_rope8(QkNormRope8Args a, hipStream_t st);
+
+// ---- kv8_pages.hip ----
+struct Kv8PagesArgs {
+    uint16_t* kc;           // the f16 pool
+    uint16_t* vc;
+    uint8_t* k8;            // the 8-bit pool
+    uint8_t* v8;
+    uint8_t* ks;
+    uint8_t* vs;
+    const int* dst;         // [n] pages written, pages read
+    const int* src;
+    uint32_t n, n_f16, n_8, n_kv, D, block;
+};
+// pages src of the f16 pool to pages dst of the 8-bit one, and the other way
+hipError_t launch_kv8_from_pages(const Kv8PagesArgs& a, hipStream_t st);
+hipError_t launch_kv8_to_pages(const Kv8PagesArgs& a, hipStream_t st);
 
 // ---- attn_paged.hip ----
 struct PagedAttnArgs {
@@ -202,6 +224,16 @@ hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t st);
 bool paged_decode_fits(uint32_t n_heads, uint32_t n_kv, uint32_t max_new);
 size_t paged_decode_workspace(uint32_t n_seq, uint32_t max_len, uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t st);
+
+// ---- attn_paged8.hip ----
+// attention over the 8-bit pool (kv8.hpp): kc and vc are its codes
+struct PagedAttn8Args : PagedAttnArgs {
+    const uint8_t* ks;      // scales of K and V [n_blocks][n_kv][block]
+    const uint8_t* vs;
+};
+size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                             uint32_t n_kv, uint32_t D);
+hipError_t launch_paged_attn8(const PagedAttn8Args& a, hipStream_t st);
 
 // ---- o_proj.hip ----
 struct OProjArgs {

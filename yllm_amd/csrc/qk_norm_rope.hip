@@ -33,6 +33,9 @@
 // 32 / 8 heads of 128 6.1.
 #include "common.hpp"
 #include "internal.hpp"
+#include "kv8.hpp"
+
+#include <type_traits>
 
 namespace yhip {
 namespace {
@@ -124,6 +127,32 @@ __device__ inline float group_sum(float x)
     if constexpr (N >= 16) x += dpp_mov<0x140>(x);  // row_mirror
     if constexpr (N == 32) x = sum_xor16(x);
     return x;
+}
+
+// the largest of each aligned group of N lanes, by the same moves
+template <int N>
+__device__ inline uint32_t group_max(uint32_t x)
+{
+    auto with = [&](float o) { x = max(x, __builtin_bit_cast(uint32_t, o)); };
+    auto f = [&] { return __builtin_bit_cast(float, x); };
+    with(dpp_mov<0xb1>(f()));
+    with(dpp_mov<0x4e>(f()));
+    with(dpp_mov<0x141>(f()));
+    if constexpr (N >= 16) with(dpp_mov<0x140>(f()));
+    if constexpr (N == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = max((uint32_t)r[0], (uint32_t)r[1]);
+    }
+    return x;
+}
+// k of a row that a group of N lanes holds, eight elements each
+template <int N>
+__device__ inline int group_exponent(const f32x4& y0, const f32x4& y1)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, max(finite_mag(y0[e]), finite_mag(y1[e])));
+    return kv8_exponent(group_max<N>(top));
 }
 
 // a row's slot (negative: none)
@@ -229,9 +258,124 @@ __device__ void v_block(const QkNormRopeArgs& a, uint32_t vb)
     }
 }
 
-template <uint32_t KIND, int D, uint32_t DT>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
+// The 8-bit pool: where a row's scale is, and its V column of codes
+__device__ inline size_t scale_at(const QkNormRopeArgs& a, uint32_t h, uint32_t slot)
 {
+    const uint32_t page = slot / a.block, off = slot - page * a.block;
+    return ((size_t)page * a.n_kv + h) * a.block + off;
+}
+template <int D>
+__device__ inline size_t v8_page_at(const QkNormRopeArgs& a, uint32_t h, uint32_t slot, uint32_t d)
+{
+    const uint32_t page = slot / a.block, off = slot - page * a.block;
+    return (((size_t)page * a.n_kv + h) * a.block + (off & ~63u)) * D + d * kV8Tile + (off & 63u);
+}
+
+// V workgroup of the 8-bit pool: 64 rows of one kv head.  A row's lanes form its
+// scale and codes and leave them in LDS, four codes a word; sixteen rows whose
+// slots are consecutive from a multiple of 16 on leave as one 16-byte store per
+// dimension, by the workgroup of their first row (which therefore reads up to
+// 15 rows more), four dimensions a thread, turned over by byte permutations; rows
+// outside such a group go a byte at a time.
+template <int D, uint32_t DT>
+__device__ void v8_block(const QkNormRope8Args& a, uint32_t vb)
+{
+    constexpr uint32_t LPH = D / 8, RPP = 256 / LPH, W = D / 4 + 1;  // lanes a row, rows a pass, words a row in LDS
+    constexpr uint32_t R = (79 + RPP) / RPP * RPP;                            // rows read: 79 are needed
+    __shared__ uint32_t tile[R * W];
+    __shared__ int slots[15 + 64 + 15];  // of rows r0 - 15 .. r0 + 78
+    __shared__ uint32_t lead[2], lone[2];
+    const uint32_t h = vb % a.n_kv, r0 = vb / a.n_kv * 64u;
+    const uint32_t t = threadIdx.x, i = t % LPH, rr = t / LPH;
+    if (t < 94u) {
+        const int b = (int)(r0 + t) - 15;
+        slots[t] = b >= 0 && (uint32_t)b < a.n_tok ? slot_of(a, (uint32_t)b) : -1;
+    }
+    __syncthreads();
+    constexpr uint32_t U = R / RPP > 5 ? 5 : R / RPP;  // passes whose loads go out together
+    static_assert(R / RPP % U == 0, "whole rounds");
+#pragma unroll 1
+    for (uint32_t p0 = 0; p0 < R / RPP; p0 += U) {
+        f32x4 x[U][2];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t b = min(r0 + (p0 + u) * RPP + rr, a.n_tok - 1u);
+            const size_t at = (size_t)b * a.v_stride + h * D + 4u * i;
+            x[u][0] = load4<DT>(a.v, at);
+            x[u][1] = load4<DT>(a.v, at + D / 2);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = (p0 + u) * RPP + rr;
+            const int k = group_exponent<LPH>(x[u][0], x[u][1]);
+            const float inv = kv8_inverse(k);
+            tile[r * W + i] = kv8_codes(x[u][0], inv);
+            tile[r * W + LPH + i] = kv8_codes(x[u][1], inv);
+            if (i == 0 && r < 64u) {
+                const int s = slots[15 + r];
+                if (s >= 0) a.vs[scale_at(a, h, (uint32_t)s)] = kv8_scale_byte(k);
+            }
+        }
+    }
+    if (t < 64u) {
+        // leads(j): rows j .. j + 15 of slots[] are one group
+        auto leads = [&](int j) {
+            if (j < 0) return false;
+            const int s = slots[j];
+            bool ok = s >= 0 && (s & 15) == 0;
+#pragma unroll
+            for (int e = 1; e < 16; ++e) ok = ok && slots[j + e] == s + e;
+            return ok;
+        };
+        const int j = 15 + (int)t, s = slots[j];
+        const uint64_t ml = __ballot(leads(j));
+        const uint64_t mn = __ballot(s >= 0 && !leads(j - (s & 15)));
+        if (t == 0) {
+            lead[0] = (uint32_t)ml;
+            lead[1] = (uint32_t)(ml >> 32);
+            lone[0] = (uint32_t)mn;
+            lone[1] = (uint32_t)(mn >> 32);
+        }
+    }
+    __syncthreads();
+    // first rows of groups are at least 16 apart: at most one in each 16 rows
+    for (uint32_t j = t; j < D; j += 256u) {
+        const uint32_t g = j & 3u, c = j >> 2;  // a group, four dimensions
+        const uint32_t m = lead[g >> 1] >> (16u * (g & 1u)) & 0xffffu;
+        if (!m) continue;
+        const uint32_t r = 16u * g + (uint32_t)__builtin_ctz(m);
+        u32x4 w[4];  // [dimension][four rows a word]
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) {
+            const uint32_t* p = &tile[(r + 4u * q) * W + c];
+            const uint32_t a0 = p[0], a1 = p[W], a2 = p[2 * W], a3 = p[3 * W];
+            const uint32_t lo01 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), hi01 = __builtin_amdgcn_perm(a1, a0, 0x07030602u),
+                           lo23 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), hi23 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+            w[0][q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+            w[1][q] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+            w[2][q] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+            w[3][q] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+        }
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slots[15 + r], 4u * c);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<u32x4*>(dst + e * kV8Tile) = w[e];
+    }
+    uint64_t left = (uint64_t)lone[1] << 32 | lone[0];
+    for (uint32_t n = 0; left; ++n, left &= left - 1) {  // uniform: each wave takes every fourth
+        if (n % 4u != t >> 6) continue;
+        const uint32_t r = (uint32_t)__builtin_ctzll(left);
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slots[15 + r], 0);
+        for (uint32_t d = t & 63u; d < D; d += 64u)
+            dst[d * kV8Tile] = reinterpret_cast<const uint8_t*>(&tile[r * W])[d];
+    }
+}
+
+// A = QkNormRope8Args: K and V go as codes and scales into the 8-bit pool; then
+// the V of few rows are passes of their own.
+template <uint32_t KIND, int D, uint32_t DT, class A = QkNormRopeArgs>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
+{
+    constexpr bool KV8 = std::is_same<A, QkNormRope8Args>::value;
     // the two roles alternate over the first 2 * min(rotation, V) workgroups (rope.hip)
     uint32_t blk = blockIdx.x;
     {
@@ -245,7 +389,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
             blk -= m;
         }
         if (v_role) {  // workgroup-uniform
-            v_block<D, DT>(a, blk);
+            if constexpr (KV8) v8_block<D, DT>(a, blk);
+            else v_block<D, DT>(a, blk);
             return;
         }
     }
@@ -272,11 +417,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
 
     // This wave's passes: HPP heads each, those of q (none without q_out), then those of k.  A pass is of one kind,
     // so that everything but the lane's offsets is wave-uniform.
-    const uint32_t pq = a.q_out ? (a.n_heads + HPP - 1) / HPP : 0u, passes = pq + (a.n_kv + HPP - 1) / HPP;
+    const uint32_t pq = a.q_out ? (a.n_heads + HPP - 1) / HPP : 0u, pk = (a.n_kv + HPP - 1) / HPP,
+                   passes = pq + pk + (KV8 && a.n_tok <= kScatterRows ? pk : 0u);
     const uint32_t p_lo = g * a.passes, p_hi = min(passes, p_lo + a.passes);
     const size_t esz = DT == kF32 ? 4 : 2;
     const char* const qrow = reinterpret_cast<const char*>(a.q) + (size_t)b * a.q_stride * esz;
     const char* const krow = reinterpret_cast<const char*>(a.k) + (size_t)b * a.k_stride * esz;
+    const char* const vrow = KV8 ? reinterpret_cast<const char*>(a.v) + (size_t)b * a.v_stride * esz : nullptr;
     const size_t kstep = (size_t)a.block * D;  // between a page's heads
     size_t kpage = 0;
     float c[4], s[4];
@@ -289,9 +436,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t p = min(p0 + u, p_hi - 1u);
-            const bool is_q = p < pq;
-            const uint32_t h = min((is_q ? p : p - pq) * HPP + sub, (is_q ? a.n_heads : a.n_kv) - 1u);
-            const char* src = is_q ? qrow : krow;
+            const bool is_q = p < pq, is_v = KV8 && p >= pq + pk;
+            const uint32_t h = min((is_q ? p : is_v ? p - pq - pk : p - pq) * HPP + sub, (is_q ? a.n_heads : a.n_kv) - 1u);
+            const char* src = is_q ? qrow : is_v ? vrow : krow;
             x[u][0] = load4<DT>(src, h * D + e0);
             x[u][1] = load4<DT>(src, h * D + e1);
         }
@@ -323,9 +470,26 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t p = p0 + u;
             if (p >= p_hi) break;  // wave-uniform
-            const bool is_q = p < pq;
-            const uint32_t h = (is_q ? p : p - pq) * HPP + sub;
+            const bool is_q = p < pq, is_v = KV8 && p >= pq + pk;
+            const uint32_t h = (is_q ? p : is_v ? p - pq - pk : p - pq) * HPP + sub;
             f32x4 y0 = x[u][0], y1 = x[u][1];
+            if constexpr (KV8) {
+                if (is_v) {
+                    const int k = group_exponent<LPH>(y0, y1);
+                    const float inv = kv8_inverse(k);
+                    const uint32_t w0 = kv8_codes(y0, inv), w1 = kv8_codes(y1, inv);
+                    if (h < a.n_kv) {
+                        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slot, 0);
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            dst[(e0 + e) * kV8Tile] = (uint8_t)(w0 >> 8 * e);
+                            dst[(e1 + e) * kV8Tile] = (uint8_t)(w1 >> 8 * e);
+                        }
+                        if (i == 0) a.vs[scale_at(a, h, (uint32_t)slot)] = kv8_scale_byte(k);
+                    }
+                    continue;
+                }
+            }
             if (norm) {
                 float ss = 0.0f;
 #pragma unroll
@@ -359,6 +523,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
                     store4(a.q_out, at + e0, a.q_out_dtype, y0);
                     store4(a.q_out, at + e1, a.q_out_dtype, y1);
                 }
+            } else if constexpr (KV8) {
+                const int k = group_exponent<LPH>(y0, y1);
+                const float inv = kv8_inverse(k);
+                const uint32_t w0 = kv8_codes(y0, inv), w1 = kv8_codes(y1, inv);
+                if (h < a.n_kv) {
+                    uint8_t* row = reinterpret_cast<uint8_t*>(a.kc) + kpage + h * kstep;
+                    *reinterpret_cast<uint32_t*>(row + e0) = w0;
+                    *reinterpret_cast<uint32_t*>(row + e1) = w1;
+                    if (i == 0) a.ks[scale_at(a, h, (uint32_t)slot)] = kv8_scale_byte(k);
+                }
             } else if (h < a.n_kv) {
                 uint16_t* row = a.kc + kpage + h * kstep;
                 *reinterpret_cast<u16x4*>(row + e0) = to_cache4(y0);
@@ -366,7 +540,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
             }
         }
     }
-    if (a.n_tok <= kScatterRows) {
+    if constexpr (!KV8) if (a.n_tok <= kScatterRows) {
         const uint32_t kv_dim = a.n_kv * D;
         for (uint32_t j = g * 64u + lane; j < kv_dim; j += 64u * a.groups) {
             const size_t at = (size_t)b * a.v_stride + j;
@@ -377,19 +551,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
     }
 }
 
-template <uint32_t KIND, int D>
-hipError_t launch_dt(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
+template <uint32_t KIND, int D, class A>
+hipError_t launch_dt(const A& a, dim3 grid, hipStream_t st)
 {
     switch (a.dtype) {
-    case kF32: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF32>), grid, dim3(256), 0, st, a); break;
-    case kF16: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF16>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kBF16>), grid, dim3(256), 0, st, a); break;
+    case kF32: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF32, A>), grid, dim3(256), 0, st, a); break;
+    case kF16: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF16, A>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kBF16, A>), grid, dim3(256), 0, st, a); break;
     }
     return hipGetLastError();
 }
 
-template <uint32_t KIND>
-hipError_t launch_kind(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
+template <uint32_t KIND, class A>
+hipError_t launch_kind(const A& a, dim3 grid, hipStream_t st)
 {
     switch (a.D) {
     case 64: return launch_dt<KIND, 64>(a, grid, st);
@@ -399,18 +573,19 @@ hipError_t launch_kind(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
     }
 }
 
-}  // namespace
-
-hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st)
+template <class A>
+hipError_t launch_any(A& a, hipStream_t st)
 {
-    const uint32_t hpp = 64u / (a.D / 8u);
-    const uint32_t passes = (a.q_out ? (a.n_heads + hpp - 1) / hpp : 0u) + (a.n_kv + hpp - 1) / hpp;
-    const uint32_t per0 = a.n_tok <= kScatterRows ? 1u : 3u;
+    constexpr bool KV8 = std::is_same<A, QkNormRope8Args>::value;
+    const uint32_t hpp = 64u / (a.D / 8u), pk = (a.n_kv + hpp - 1) / hpp;
+    const bool few = a.n_tok <= kScatterRows;
+    const uint32_t passes = (a.q_out ? (a.n_heads + hpp - 1) / hpp : 0u) + pk + (KV8 && few ? pk : 0u);
+    const uint32_t per0 = few ? 1u : 3u;
     const uint32_t groups = (passes + per0 - 1) / per0;
     a.passes = (passes + groups - 1) / groups;  // per wave, evenly
     a.groups = (passes + a.passes - 1) / a.passes;
     a.rope_blocks = (uint32_t)(((uint64_t)a.n_tok * a.groups + 3u) / 4u);
-    a.v_blocks = a.n_tok > kScatterRows ? a.n_kv * a.D / 64u * ((a.n_tok + 63u) / 64u) : 0u;
+    a.v_blocks = few ? 0u : (KV8 ? a.n_kv : a.n_kv * a.D / 64u) * ((a.n_tok + 63u) / 64u);
     const dim3 grid(a.rope_blocks + a.v_blocks);
     switch (a.kind) {
     case kRopeNone: return launch_kind<kRopeNone>(a, grid, st);
@@ -420,5 +595,10 @@ hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st)
     default: return hipErrorInvalidValue;
     }
 }
+
+}  // namespace
+
+hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st) { return launch_any(a, st); }
+hipError_t launch_qk_norm_rope8(QkNormRope8Args a, hipStream_t st) { return launch_any(a, st); }
 
 }  // namespace yhip

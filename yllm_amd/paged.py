@@ -4,6 +4,12 @@
     qk_norm_rope_kv_store(cache, q, k, v, ...)    QK norm, rotation and the K/V store in one pass
     paged_attn(q, cache, block_table, ...)        the new tokens of every sequence over its pages
 
+and the same over a pool held in 8 bits (PagedKV8: half the bytes):
+
+    qk_norm_rope_kv8_store(cache, q, k, v, ...)   the append, quantising
+    paged_attn8(q, cache, block_table, ...)       the attention
+    kv8_from_pages(kv8, kv, dst, src), kv8_to_pages(kv, kv8, dst, src)   whole pages between the two pools
+
 A step of a layer, for sequences of any lengths (decode tokens and prompt chunks together):
 
     step = paged_plan(block_table, ctx_lens, new_lens, free_blocks, n_free, block, n_tok)
@@ -65,6 +71,53 @@ class PagedKV:
         return cls(k, v)
 
 
+_E4M3, _E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
+
+
+@dataclass
+class PagedKV8:
+    """One layer's pool of KV pages in 8 bits: a value is its e4m3 code times the scale, a power of two in e5m2, of its
+    position and kv head.
+
+    k: e4m3 [n_blocks, n_kv, block, head_dim]
+    v: e4m3 [n_blocks, n_kv, block // 64, head_dim, 64] (64-position tiles, d-major)
+    k_scale, v_scale: e5m2 [n_blocks, n_kv, block]
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @property
+    def n_blocks(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def n_kv(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def block(self) -> int:
+        return self.k.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.k.shape[3]
+
+    @classmethod
+    def empty(cls, n_blocks: int, n_kv: int, head_dim: int, block: int = 64, device: str | torch.device = "cuda",
+              zero: bool = True) -> "PagedKV8":
+        if not 64 <= block <= 65536 or block & (block - 1):
+            raise YhipError(-22, f"PagedKV8: block {block} must be a power of two in 64..65536")
+        alloc = torch.zeros if zero else torch.empty
+
+        def held(t, *shape):  # (zero bytes are zero in every type; torch fills bytes, not these types, everywhere)
+            return alloc((n_blocks, n_kv, *shape), dtype=torch.uint8, device=device).view(t)
+
+        return cls(held(_E4M3, block, head_dim), held(_E4M3, block // 64, head_dim, 64), held(_E5M2, block), held(_E5M2, block))
+
+
 # Small calls are bound by this module's own work (a decode step's kernels take 4 to 6 us), so the checks below ask a
 # tensor for as little as they can, and build messages only when they fail.
 
@@ -77,6 +130,20 @@ def _pool(cache: PagedKV | LayerKV, fn: str) -> tuple[int, int, int, int]:
     if len(shape) != 4 or k.dtype is not _F16 or v.dtype is not _F16 or not k.is_contiguous() \
             or not v.is_contiguous() or v.numel() != k.numel() or v.shape[-2:] != (shape[3], 32):
         raise YhipError(-22, f"{fn}: the cache must hold contiguous f16 K and V of one size, V in tiles of 32 positions")
+    return shape
+
+
+def _pool8(cache: PagedKV8, fn: str) -> tuple[int, int, int, int]:
+    """(n_blocks, n_kv, block, head_dim)."""
+    if not isinstance(cache, PagedKV8):
+        raise YhipError(-22, f"{fn}: the cache must be a PagedKV8")
+    k, v, ks, vs = cache.k, cache.v, cache.k_scale, cache.v_scale
+    shape = k.shape
+    if len(shape) != 4 or k.dtype is not _E4M3 or v.dtype is not _E4M3 or ks.dtype is not _E5M2 or vs.dtype is not _E5M2 \
+            or not k.is_contiguous() or not v.is_contiguous() or not ks.is_contiguous() or not vs.is_contiguous() \
+            or v.numel() != k.numel() or v.shape[-2:] != (shape[3], 64) or ks.shape != shape[:3] or vs.shape != shape[:3]:
+        raise YhipError(-22, f"{fn}: the cache must hold contiguous e4m3 K and V of one size, V in tiles of 64 positions, "
+                             "and an e5m2 scale of each for every position and kv head")
     return shape
 
 
@@ -178,8 +245,29 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
     one projection output.  rope: ROPE_PAIRS, ROPE_HALF, ROPE_MROPE (first n_rot dims) or ROPE_NONE.  Returns the
     rotated q (q_out, allocated in q_out_dtype or q's type if not given; q_out may be q itself), or None when q is
     None.  Rows without a slot (negative) are skipped."""
-    fn = "qk_norm_rope_kv_store"
-    n_blocks, n_kv, block, d = _pool(cache, fn)
+    kc, vc = cache.k, cache.v
+    return _store("qk_norm_rope_kv_store", lib().yhip_qk_norm_rope_kv_store, _pool(cache, "qk_norm_rope_kv_store"), (kc, vc),
+                  q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out, q_out_dtype)
+
+
+def qk_norm_rope_kv8_store(cache: PagedKV8, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                           n_heads: int, rope: int, theta: float, n_rot: int = 0, *,
+                           positions: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                           pos_start: int = 0, q_norm: torch.Tensor | None = None,
+                           k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                           q_out: torch.Tensor | None = None,
+                           q_out_dtype: torch.dtype | None = None) -> torch.Tensor | None:
+    """qk_norm_rope_kv_store into a pool held in 8 bits: each row of k (after its norm and rotation) and v gets a scale
+    2^k, the smallest (k in -14..7) whose 448 reaches its largest magnitude, and e4m3 codes to nearest even.  Magnitudes
+    past 57344 are held as that, inf and NaN as NaN.  A row's bytes depend on that row alone."""
+    return _store("qk_norm_rope_kv8_store", lib().yhip_qk_norm_rope_kv8_store, _pool8(cache, "qk_norm_rope_kv8_store"),
+                  (cache.k, cache.v, cache.k_scale, cache.v_scale), q, k, v, n_heads, rope, theta, n_rot, positions, slots,
+                  pos_start, q_norm, k_norm, eps, q_out, q_out_dtype)
+
+
+def _store(fn, f, shape, pools, q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out,
+           q_out_dtype):
+    n_blocks, n_kv, block, d = shape
     dt = k.dtype
     T = k.shape[0]
     ks, vs = _rows(fn, "k", k, T, n_kv * d), _rows(fn, "v", v, T, n_kv * d)
@@ -213,12 +301,10 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
             raise YhipError(-22, f"{fn}: q_norm and k_norm must both be [{d}], f32 or f16")
         norm = _DT[q_norm.dtype]
         wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
-    kc, vc = cache.k, cache.v
-    args = (qop, qdt, qos, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DT[dt], wq, wk, norm, eps, kc.data_ptr(),
-            vc.data_ptr(), n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
+    args = (qop, qdt, qos, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DT[dt], wq, wk, norm, eps,
+            *[p.data_ptr() for p in pools], n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
             n_rot if rope == ROPE_MROPE else 0, theta if rope != ROPE_NONE else 1.0)
-    _launch(lib().yhip_qk_norm_rope_kv_store, args,
-            elsewhere(fn, k.get_device(), kc, vc, q, v, q_out, positions, slots, q_norm, k_norm))
+    _launch(f, args, elsewhere(fn, k.get_device(), *pools, q, v, q_out, positions, slots, q_norm, k_norm))
     return q_out
 
 
@@ -245,7 +331,37 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, kv_le
     fn = "paged_attn"
     if not isinstance(cache, PagedKV):
         raise YhipError(-22, f"{fn}: the cache must be a PagedKV")
-    n_blocks, n_kv, block, d = _pool(cache, fn)
+    return _attn(fn, lib().yhip_paged_attn, paged_attn_workspace_bytes, _pool(cache, fn), (cache.k, cache.v), q, block_table,
+                 kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype, workspace)
+
+
+def paged_attn8_workspace_bytes(n_tok: int, n_seq: int, max_new: int, max_len: int, n_heads: int, n_kv: int,
+                                head_dim: int) -> int:
+    """Workspace of every paged_attn8 call within these bounds."""
+    return int(lib().yhip_paged_attn8_workspace(n_tok, n_seq, max_new, max_len, n_heads, n_kv, head_dim))
+
+
+def paged_attn8_workspace(n_tok: int, n_seq: int, max_new: int, max_len: int, n_heads: int, n_kv: int, head_dim: int,
+                          device: torch.device | str = "cuda") -> torch.Tensor:
+    nbytes = paged_attn8_workspace_bytes(n_tok, n_seq, max_new, max_len, n_heads, n_kv, head_dim)
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+
+
+def paged_attn8(q: torch.Tensor, cache: PagedKV8, block_table: torch.Tensor, kv_lens: torch.Tensor, cu_new: torch.Tensor,
+                n_heads: int, max_new: int, max_len: int | None = None, gate: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attn over a pool held in 8 bits, with the values that it holds as keys and values (workspaces by
+    paged_attn8_workspace)."""
+    fn = "paged_attn8"
+    return _attn(fn, lib().yhip_paged_attn8, paged_attn8_workspace_bytes, _pool8(cache, fn),
+                 (cache.k, cache.v, cache.k_scale, cache.v_scale), q, block_table, kv_lens, cu_new, n_heads, max_new, max_len,
+                 gate, out, out_dtype, workspace)
+
+
+def _attn(fn, f, space, shape, pools, q, block_table, kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype,
+          workspace):
+    n_blocks, n_kv, block, d = shape
     n, w, stride = _table(fn, block_table)
     _ints(fn, "kv_lens", kv_lens, n)
     _ints(fn, "cu_new", cu_new, n + 1)
@@ -265,13 +381,11 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, kv_le
         gp = gate.data_ptr()
         if gate.dtype is not torch.float32:
             raise YhipError(-22, f"{fn}: gate must be fp32")
-    kc, vc = cache.k, cache.v
     dev = q.get_device()
-    there = elsewhere(fn, dev, kc, vc, block_table, kv_lens, cu_new, out, gate)
-    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, kc.data_ptr(), vc.data_ptr(),
+    there = elsewhere(fn, dev, *pools, block_table, kv_lens, cu_new, out, gate)
+    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, *[p.data_ptr() for p in pools],
             n_blocks, block, block_table.data_ptr(), w, stride, kv_lens.data_ptr(), cu_new.data_ptr(), n, T, max_new,
             max_len, n_heads, n_kv, d, gp, gs)
-    f = lib().yhip_paged_attn
     if there is None and workspace is not None and workspace.get_device() == dev:
         rc = f(*args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
         if rc == OK:
@@ -279,10 +393,37 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, kv_le
         if rc != ENOSPC:
             check(rc)
         workspace = None  # too short: allocated below
-    need = lambda: paged_attn_workspace_bytes(T, n, max_new, max_len, n_heads, n_kv, d)  # noqa: E731
+    need = lambda: space(T, n, max_new, max_len, n_heads, n_kv, d)  # noqa: E731
     if there is None:
         _with_workspace(f, args, workspace, need, q.device)
     else:
         with there:
             _with_workspace(f, args, workspace, need, q.device)
     return out
+
+
+def kv8_from_pages(kv8: PagedKV8, kv: PagedKV, dst: torch.Tensor, src: torch.Tensor) -> None:
+    """Page dst[i] of kv8 gets page src[i] of kv, quantised as qk_norm_rope_kv8_store does (int32 on the GPU; each dst at
+    most once).  A pair with a page outside its pool is skipped."""
+    _pages("kv8_from_pages", kv8, kv, dst, src, False)
+
+
+def kv8_to_pages(kv: PagedKV, kv8: PagedKV8, dst: torch.Tensor, src: torch.Tensor) -> None:
+    """Page dst[i] of kv gets the values that page src[i] of kv8 holds, which f16 holds exactly (otherwise as
+    kv8_from_pages)."""
+    _pages("kv8_to_pages", kv8, kv, dst, src, True)
+
+
+def _pages(fn: str, kv8: PagedKV8, kv: PagedKV, dst: torch.Tensor, src: torch.Tensor, to: bool) -> None:
+    n8, n_kv, block, d = _pool8(kv8, fn)
+    n16, *rest = _pool(kv, fn)
+    if rest != [n_kv, block, d]:
+        raise YhipError(-22, f"{fn}: the pools must have pages of one shape")
+    n = dst.numel()
+    _ints(fn, "dst", dst, n)
+    _ints(fn, "src", src, n)
+    eight = (kv8.k.data_ptr(), kv8.v.data_ptr(), kv8.k_scale.data_ptr(), kv8.v_scale.data_ptr(), n8)
+    half = (kv.k.data_ptr(), kv.v.data_ptr(), n16)
+    f = lib().yhip_kv8_to_pages if to else lib().yhip_kv8_from_pages
+    args = (*(half + eight if to else eight + half), dst.data_ptr(), src.data_ptr(), n, block, n_kv, d)
+    _launch(f, args, elsewhere(fn, dst.get_device(), src, kv8.k, kv8.v, kv8.k_scale, kv8.v_scale, kv.k, kv.v))
