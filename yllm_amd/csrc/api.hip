@@ -1116,10 +1116,6 @@ int yhip_paged_attn8(void* att_out, uint32_t out_dtype, uint32_t out_stride, con
                                    n_tok, max_new, max_len, n_heads, n_kv_heads, head_dim, gate, gate_stride, workspace,
                                    workspace_bytes))
         return rc > 0 ? YHIP_OK : rc;
-    // (units of one sequence's row blocks, paged_decode8.hip)
-    if ((((uint64_t)n_heads + n_kv_heads - 1) / n_kv_heads * max_new / 16 + 1) * n_kv_heads * (max_len / 256 + 2ull) >= 1ull << 31)
-        return fail(YHIP_EINVAL, "%s: max_new %u over max_len %u is too much for one call: send the tokens in chunks", fn,
-                    max_new, max_len);
     a.kc = reinterpret_cast<const uint16_t*>(kpool);
     a.vc = reinterpret_cast<const uint16_t*>(vpool);
     a.ks = kscale;

@@ -184,28 +184,17 @@ size_t paged_bytes(uint32_t wgs, uint32_t D)
     return align256a((size_t)wgs * sizeof(PagedDesc)) + align256a(rows * 2 * sizeof(float)) + rows * D * sizeof(float);
 }
 
-template <int D, int NG, bool QS>
-void launch_tiles(const PagedAttnArgs& a, uint32_t grid, hipStream_t st)
+template <int D, int NG, bool QS, class A>
+void launch_tiles(const A& a, uint32_t grid, hipStream_t st)
 {
     constexpr int threads = 256 * NG * (D > 128 ? 2 : 1);
-    hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, PagedAttnArgs>), dim3(grid), dim3(threads), 0, st, a);
+    hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, A>), dim3(grid), dim3(threads), 0, st, a);
 }
 
-}  // namespace
-
-size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
-                            uint32_t n_kv, uint32_t D)
+template <class A>
+hipError_t launch_items(const A& in, hipStream_t st)
 {
-    // (the decode kernel's, where it serves every call within the bounds; else also large enough for its calls)
-    const size_t decode = paged_decode_workspace(n_seq, max_len, n_kv, D);
-    if (paged_decode_fits(n_heads, n_kv, max_new)) return decode;
-    return std::max(decode, paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1, kMinUnits), D));
-}
-
-hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
-{
-    if (paged_decode_fits(in.n_heads, in.n_kv, in.max_new)) return launch_paged_decode(in, st);
-    PagedAttnArgs a = in;
+    A a = in;
     const bool qs = a.q_dtype == kF32;
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
     a.min_units = min_units(a.max_len);
@@ -224,7 +213,7 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
     case 128: qs ? launch_tiles<128, 2, true>(a, grid, st) : launch_tiles<128, 1, false>(a, grid, st); break;
     case 256:
         if (qs) launch_tiles<256, 1, true>(a, grid, st);
-        else hipLaunchKernelGGL((prefill_halves_kernel<256, false, PagedAttnArgs>), dim3(grid), dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((prefill_halves_kernel<256, false, A>), dim3(grid), dim3(512), 0, st, a);
         break;
     default: return hipErrorInvalidValue;
     }
@@ -234,12 +223,34 @@ hipError_t launch_paged_attn(const PagedAttnArgs& in, hipStream_t st)
         const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
         const dim3 merge(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
         switch (a.D) {
-        case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, merge, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, merge, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(paged_merge_kernel<256>, merge, dim3(256), 0, st, a); break;
+        case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, merge, dim3(256), 0, st, static_cast<const PagedAttnArgs&>(a)); break;
+        case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, merge, dim3(256), 0, st, static_cast<const PagedAttnArgs&>(a)); break;
+        default: hipLaunchKernelGGL(paged_merge_kernel<256>, merge, dim3(256), 0, st, static_cast<const PagedAttnArgs&>(a)); break;
         }
     }
     return hipGetLastError();
 }
+
+}  // namespace
+
+size_t paged_attn_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                            uint32_t n_kv, uint32_t D)
+{
+    // (the decode kernel's, where it serves every call within the bounds; else also large enough for its calls)
+    const size_t decode = paged_decode_workspace(n_seq, max_len, n_kv, D);
+    if (paged_decode_fits(n_heads, n_kv, max_new)) return decode;
+    return std::max(decode, paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1, kMinUnits), D));
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t st)
+{
+    return paged_decode_fits(a.n_heads, a.n_kv, a.max_new) ? launch_paged_decode(a, st) : launch_items(a, st);
+}
+
+size_t paged_tiles8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
+{
+    return paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1, kMinUnits), D);
+}
+hipError_t launch_paged_tiles8(const PagedAttn8Args& a, hipStream_t st) { return launch_items(a, st); }
 
 }  // namespace yhip

@@ -225,15 +225,21 @@ bool paged_decode_fits(uint32_t n_heads, uint32_t n_kv, uint32_t max_new);
 size_t paged_decode_workspace(uint32_t n_seq, uint32_t max_len, uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t st);
 
-// ---- attn_paged8.hip ----
+// ---- paged_decode8.hip, attn_paged.hip ----
 // attention over the 8-bit pool (kv8.hpp): kc and vc are its codes
 struct PagedAttn8Args : PagedAttnArgs {
     const uint8_t* ks;      // scales of K and V [n_blocks][n_kv][block]
     const uint8_t* vs;
+    // set by the launcher: sequences of up to this many rows (new tokens of a kv head's query heads) are the decode
+    // kernel's, the others the tiles'
+    uint32_t few;
 };
 size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
                              uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_attn8(const PagedAttn8Args& a, hipStream_t st);
+// the part of the sequences that are not few
+size_t paged_tiles8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D);
+hipError_t launch_paged_tiles8(const PagedAttn8Args& a, hipStream_t st);
 
 // ---- o_proj.hip ----
 struct OProjArgs {

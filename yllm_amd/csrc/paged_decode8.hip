@@ -19,6 +19,8 @@
 #include "kv8.hpp"
 #include "paged_items8.hpp"
 
+#include <algorithm>
+
 namespace yhip {
 namespace {
 
@@ -35,7 +37,7 @@ struct Decode8Line {
     static __device__ uint32_t blocks(const PagedAttnArgs& a, const PagedSeq& s) { return (a.gmax * s.nq + kRows - 1) / kRows; }
     static __device__ uint64_t units(const PagedAttnArgs& a, const PagedSeq& s)
     {
-        return (uint64_t)a.n_kv * blocks(a, s) * item(s);
+        return few_rows(static_cast<const PagedAttn8Args&>(a), s) ? (uint64_t)a.n_kv * blocks(a, s) * item(s) : 0;
     }
     static __device__ uint32_t item(const PagedSeq& s)
     {
@@ -104,14 +106,14 @@ __device__ inline bool decode8_next(const PagedAttnArgs& a, PagedCursor& C, Deco
 
 // The item of this workgroup where none is cut (short contexts): one each, by
 // its number, without the line; false where there is none.
-__device__ inline bool decode8_whole(const PagedAttnArgs& a, Decode8Piece& I)
+__device__ inline bool decode8_whole(const PagedAttn8Args& a, Decode8Piece& I)
 {
-    const uint32_t nb = (a.gmax * a.max_new + kRows - 1) / kRows, w = blockIdx.x / nb;
+    const uint32_t nb = (min(a.gmax * a.max_new, a.few) + kRows - 1) / kRows, w = blockIdx.x / nb;
     I.rb = blockIdx.x - w * nb;
     I.seq = w / a.n_kv;
     I.kvh = w - I.seq * a.n_kv;
     const PagedSeq s = cursor_seq(a, I.seq);
-    if (rows_of(a, I.kvh, I.rb, s.nq).rows == 0) return false;
+    if (!few_rows(a, s) || rows_of(a, I.kvh, I.rb, s.nq).rows == 0) return false;
     I.row0 = s.row0;
     I.nq = s.nq;
     I.pos0 = s.pos0;
@@ -493,14 +495,24 @@ uint32_t units_of_bytes(uint32_t bytes, uint32_t D) { return bytes / (2 * D * kU
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Sequences of up to this many rows are walked here, in blocks of 16, the others
+// in tiles of 128 rows.
+constexpr uint32_t kFewRows = 16;
+
+// row blocks of a sequence at most
+uint32_t row_blocks(uint32_t max_new, uint32_t n_heads, uint32_t n_kv)
+{
+    const uint64_t rows = (uint64_t)((n_heads + n_kv - 1) / n_kv) * max_new;
+    return (uint32_t)((std::min(rows, (uint64_t)kFewRows) + kRows - 1) / kRows);
+}
+
 // Chunks of a launch: what the GPU holds at once, or all that the bounds can
 // fill; 0: none is cut.
-uint32_t decode8_wgs(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
+uint32_t decode8_wgs(uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
 {
     const uint32_t units = (max_len + kUnit8 - 1) / kUnit8;
     if (units <= units_of_bytes(kWholeBytes, D)) return 0;  // no item is cut: a workgroup each
-    const uint64_t gmax = (n_heads + n_kv - 1) / n_kv;
-    const uint64_t most = ((uint64_t)n_tok * gmax / kRows + n_seq) * n_kv * (units + kItem8Units);
+    const uint64_t most = (uint64_t)n_seq * row_blocks(max_new, n_heads, n_kv) * n_kv * (units + kItem8Units);
     const uint64_t full = (uint64_t)(D <= 128 ? 2 : 1) * (uint64_t)n_cus();
     return (uint32_t)(((most < full ? most : full) + 7) / 8 * 8);
 }
@@ -521,19 +533,10 @@ void launch_decode8_pieces(const PagedAttn8Args& a, uint32_t grid, bool stream, 
         hipLaunchKernelGGL((paged_decode8_kernel<D, PREC, 0>), dim3(grid), dim3(256), 0, st, a);
 }
 
-}  // namespace
-
-size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
-                             uint32_t n_kv, uint32_t D)
-{
-    return decode8_bytes(decode8_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D), D);
-}
-
-hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
+hipError_t launch_decode8(const PagedAttn8Args& in, hipStream_t st)
 {
     PagedAttn8Args a = in;
-    a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
-    a.n_wg = decode8_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, a.D);
+    a.n_wg = decode8_wgs(a.n_seq, a.max_new, a.max_len, a.n_heads, a.n_kv, a.D);
     a.snap_units = units_of_bytes(kSnapBytes, a.D);
     a.min_units = 1 + kItem8Units;
     char* p = reinterpret_cast<char*>(a.ws);
@@ -541,7 +544,7 @@ hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
     p += align256((size_t)a.n_wg * sizeof(PagedDesc));
     a.part_ml = reinterpret_cast<float*>(p);
     a.part_o = reinterpret_cast<float*>(p + align256((size_t)2 * a.n_wg * kRows * 2 * sizeof(float)));
-    const uint32_t nb = (a.gmax * a.max_new + kRows - 1) / kRows;
+    const uint32_t nb = row_blocks(a.max_new, a.n_heads, a.n_kv);
     const uint32_t grid = a.n_wg ? a.n_wg : a.n_seq * a.n_kv * nb;
     // non-temporal loads where the batch reads more than the caches keep (an upper bound)
     const bool stream = nb == 1 && (uint64_t)a.n_seq * a.n_kv * a.max_len * a.D * 2u >= (32ull << 20);
@@ -553,7 +556,7 @@ hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
     default: return hipErrorInvalidValue;
     }
     if (a.n_wg) {
-        const dim3 merge(a.n_wg, min((uint32_t)kRows, a.gmax * a.max_new));
+        const dim3 merge(a.n_wg, std::min((uint64_t)kRows, (uint64_t)a.gmax * a.max_new));
         switch (a.D) {
         case 64: hipLaunchKernelGGL(paged_decode8_merge_kernel<64>, merge, dim3(256), 0, st, a); break;
         case 128: hipLaunchKernelGGL(paged_decode8_merge_kernel<128>, merge, dim3(256), 0, st, a); break;
@@ -561,6 +564,41 @@ hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
         }
     }
     return hipGetLastError();
+}
+
+// whether every sequence within the bounds is few
+bool all_few(uint32_t n_heads, uint32_t n_kv, uint32_t max_new)
+{
+    return (uint64_t)((n_heads + n_kv - 1) / n_kv) * max_new <= kFewRows;
+}
+
+}  // namespace
+
+// Both parts at once: they run one after the other, but a workspace that serves
+// a call serves smaller ones of either kind.
+size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
+                             uint32_t n_kv, uint32_t D)
+{
+    const size_t few = align256(decode8_bytes(decode8_wgs(n_seq, max_new, max_len, n_heads, n_kv, D), D));
+    return all_few(n_heads, n_kv, max_new) ? few : few + paged_tiles8_workspace(n_tok, n_seq, max_len, n_heads, n_kv, D);
+}
+
+// Sequences with few rows go to the kernel above, the others to the tiles; which
+// are which is known on the device only, so both lines are walked, but for
+// one sequence (a prompt's chunk), which is the tiles' whatever it brings.
+hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
+{
+    PagedAttn8Args a = in;
+    a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
+    a.few = kFewRows;
+    if (all_few(a.n_heads, a.n_kv, a.max_new)) return launch_decode8(a, st);
+    if (a.n_seq > 1) {
+        if (const hipError_t e = launch_decode8(a, st)) return e;
+        a.ws = reinterpret_cast<char*>(a.ws) + align256(decode8_bytes(decode8_wgs(a.n_seq, a.max_new, a.max_len, a.n_heads, a.n_kv, a.D), a.D));
+    } else {
+        a.few = 0;
+    }
+    return launch_paged_tiles8(a, st);
 }
 
 }  // namespace yhip

@@ -244,9 +244,9 @@ __device__ inline bool paged_cut(const PagedAttnArgs& a, PagedCursor& C, uint32_
     return true;
 }
 
-// The chunk's next piece in tiles of BN keys; false past its end.
-template <int BN>
-__device__ inline bool paged_next(const PagedAttnArgs& a, PagedCursor& C, PagedItem& I)
+// The chunk's next piece in tiles of BN keys; false past its end.  (Args: see PagedLine)
+template <int BN, class Args>
+__device__ inline bool paged_next(const Args& a, PagedCursor& C, PagedItem& I)
 {
     constexpr uint32_t TU = kUnitKeys / BN;  // tiles per unit
     for (;;) {
@@ -349,14 +349,14 @@ __device__ inline bool paged_whole(const PagedAttnArgs& a, PagedItem& I)
 }
 
 // The workgroup's first piece; false if it has none.
-template <int NT, int BN>
-__device__ inline bool paged_first(const PagedAttnArgs& args, uint64_t* scratch, PagedCursor& C, PagedItem& I)
+template <int NT, int BN, class Line = PagedLine, class Args>
+__device__ inline bool paged_first(const Args& args, uint64_t* scratch, PagedCursor& C, PagedItem& I)
 {
     if (args.n_wg == 0) {
         C = PagedCursor{};  // an empty chunk: nothing comes after the item
         return paged_whole<BN>(fresh_args(args), I);
     }
-    if (paged_start<NT>(fresh_args(args), scratch, C) && paged_next<BN>(fresh_args(args), C, I)) return true;
+    if (paged_start<NT, Line>(fresh_args(args), scratch, C) && paged_next<BN>(fresh_args(args), C, I)) return true;
     if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(args.desc)[C.j].n = 0;
     return false;
 }

@@ -19,6 +19,20 @@ __device__ inline const PagedAttn8Args& fresh_args(const PagedAttn8Args&)
     return *(const PagedAttn8Args*)p;
 }
 
+// A sequence's units among the tiles' items: those with few tokens are the
+// decode kernel's (its line has the others' complement).
+__device__ inline bool few_rows(const PagedAttn8Args& a, const PagedSeq& s) { return a.gmax * s.nq <= a.few; }
+__device__ inline uint64_t seq_units(const PagedAttn8Args& a, const PagedSeq& s)
+{
+    return few_rows(a, s) ? 0 : seq_units(static_cast<const PagedAttnArgs&>(a), s);
+}
+struct Paged8Line {
+    static __device__ uint64_t units(const PagedAttnArgs& a, const PagedSeq& s)
+    {
+        return seq_units(static_cast<const PagedAttn8Args&>(a), s);
+    }
+};
+
 // first byte and number (0: outside the pool) of the scales of kv head kvh's part of a page; its codes are D times both
 struct Paged8Tile {
     uint64_t at;

@@ -33,6 +33,7 @@
 #include "common.hpp"
 #include "internal.hpp"
 #include "paged_items.hpp"
+#include "paged_items8.hpp"
 
 #include <math.h>
 
@@ -113,6 +114,68 @@ __device__ inline int chunk_swz(int r)
     else if constexpr (NCH == 8) return (r & 7) ^ ((r >> 3) & 1);
     else return (((r >> 1) ^ (r >> 3)) & 1) | ((r >> 1) & 2);
 }
+
+// A tile of BN keys of the 8-bit pool (kv8.hpp) on its way into LDS, where it
+// lies as an f16 one does: a thread loads CB times sixteen codes of K and of V,
+// with their scales, into registers, and later writes their f16 values (exactly
+// what is held) as two swizzled chunks each.  The conversion is done once a
+// workgroup, not by every wave that reads the tile.
+template <int D, int BN, int LT>
+struct Stage8 {
+    static constexpr int CB = BN * D / (16 * LT), KC = D / 16, VC = BN / 16;  // 16-code chunks a thread, a K row, a V row
+    static_assert(LT % VC == 0, "a thread's V chunks are of the same positions");
+    u32x4 k[CB], v[CB], vs;
+    uint32_t ks[CB];
+
+    static __device__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint64_t at, uint32_t bytes)
+    {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + at, 0, bytes, 0x00020000);
+    }
+    // the tile from key `key` on, in the page at p; t: the thread's number
+    __device__ void load_k(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t)
+    {
+        const __amdgpu_buffer_rsrc_t r = rsrc(a.kc, p.at * D, p.bytes * D), rs = rsrc(a.ks, p.at, p.bytes);
+        const uint32_t at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (t + LT * i) * 16, at * D, 0));
+            ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, (t + LT * i) / KC, at, 0);
+        }
+    }
+    __device__ void load_v(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t)
+    {
+        const __amdgpu_buffer_rsrc_t r = rsrc(a.vc, p.at * D, p.bytes * D), rs = rsrc(a.vs, p.at, p.bytes);
+        const uint32_t at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
+        const uint32_t tile = (at & ~(kV8Tile - 1)) * D + (at & (kV8Tile - 1));  // (a tile may be half of one of 64 positions)
+#pragma unroll
+        for (int i = 0; i < CB; ++i)
+            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                 r, (t + LT * i) / VC * (int)kV8Tile + t % VC * 16, tile, 0));
+        vs = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, t % VC * 16, at, 0));
+    }
+    __device__ void store_k(_Float16* lds, int t) const
+    {
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int L = t + LT * i, r = lds_row_of_key(L / KC), c = 2 * (L % KC), swz = chunk_swz<D / 8>(r);
+            const float scale = kv8_scale(ks[i]);
+            *reinterpret_cast<f16x8*>(lds + r * D + ((c ^ swz) << 3)) = kv8_values(k[i][0], k[i][1], scale);
+            *reinterpret_cast<f16x8*>(lds + r * D + (((c + 1) ^ swz) << 3)) = kv8_values(k[i][2], k[i][3], scale);
+        }
+    }
+    __device__ void store_v(_Float16* lds, int t) const
+    {
+        f16x2 f[2][4];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) f[w >> 2][w & 3] = kv8_factors(vs[w >> 1], w & 1);
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int d = (t + LT * i) / VC, c = 2 * (t % VC), swz = chunk_swz<BN / 8>(d);
+            *reinterpret_cast<f16x8*>(lds + d * BN + ((c ^ swz) << 3)) = kv8_values(v[i][0], v[i][1], f[0]);
+            *reinterpret_cast<f16x8*>(lds + d * BN + (((c + 1) ^ swz) << 3)) = kv8_values(v[i][2], v[i][3], f[1]);
+        }
+    }
+};
 
 // Values that a query does not see must not reach its output, whatever their
 // bits: a masked key's probability is 0, but 0 * inf and 0 * NaN are NaN.
@@ -387,7 +450,7 @@ __device__ inline bool split_item(const PrefillArgs& a, PItem& I)
 template <int D, int NG, bool SPLIT, bool QS = false, class A = PrefillArgs>
 __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 && !QS) ? 2 : 1) void prefill_kernel(A args)
 {
-    constexpr bool PAGED = std::is_same<A, PagedAttnArgs>::value;
+    constexpr bool PAGED = std::is_base_of<PagedAttnArgs, A>::value, KV8 = std::is_same<A, PagedAttn8Args>::value;
     constexpr bool PS = PAGED && QS;
     using Item = typename std::conditional<PAGED, PagedItem, PItem>::type;
     using Pos = typename std::conditional<PAGED, int, uint32_t>::type;  // positions of paged rows may be negative
@@ -475,14 +538,15 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // stores.  With a gate the epilogue loads the gate values, which would
     // then wait behind these loads; such items issue their loads at their
     // own start.
-    const bool early = args.gate == nullptr && !PAIR;
+    const bool early = args.gate == nullptr && !PAIR && !KV8;
     // paged, 16-bit queries: an item waits for the next one's first loads before
     // its output stores instead of behind them, so the stores drain during the
     // next item's first step
-    constexpr bool AHEAD = PAGED && !QS && NB == 2;
+    constexpr bool AHEAD = PAGED && !KV8 && !QS && NB == 2;
     Item cur;
     if constexpr (PAGED) {
-        if (!paged_first<256 * NG * (PAIR ? 2 : 1), BN>(args, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C, cur)) return;
+        using Line = typename std::conditional<KV8, Paged8Line, PagedLine>::type;
+        if (!paged_first<256 * NG * (PAIR ? 2 : 1), BN, Line>(args, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C, cur)) return;
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
@@ -551,8 +615,23 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if constexpr (PAGED) return paged_page(a, I.seq, min(kt, I.t0 + I.nt - 1) * BN);
             else return 0;
         };
-        auto dma_page_k = [&](const PagedTile& p, int par, uint32_t kt) {
-            if constexpr (PAGED) {
+        // (8 bits: loaded into registers here, written to LDS by put_k and put_v)
+        using Tile = typename std::conditional<KV8, Paged8Tile, PagedTile>::type;
+        typename std::conditional<KV8, Stage8<D, BN, LT>, int>::type stage;
+        auto tile_in = [&](uint32_t page, uint32_t kv) {
+            if constexpr (KV8) return paged8_tile(a, page, kv);
+            else if constexpr (PAGED) return paged_tile<D>(a, page, kv);
+            else return Tile{};
+        };
+        auto put_k = [&](int par) {
+            if constexpr (KV8) stage.store_k(kbuf(par), gtid);
+        };
+        auto put_v = [&](int par) {
+            if constexpr (KV8) stage.store_v(vbuf(par), gtid);
+        };
+        auto dma_page_k = [&](const Tile& p, int par, uint32_t kt) {
+            if constexpr (KV8) stage.load_k(a, p, kt * BN, gtid);
+            else if constexpr (PAGED) {
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.kc)) + p.at, 0, p.bytes, 0x00020000);
                 const uint32_t at = p.bytes ? ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2 : 0u;
@@ -560,8 +639,9 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], at);
             }
         };
-        auto dma_page_v = [&](const PagedTile& p, int par, uint32_t kt) {
-            if constexpr (PAGED) {
+        auto dma_page_v = [&](const Tile& p, int par, uint32_t kt) {
+            if constexpr (KV8) stage.load_v(a, p, kt * BN, gtid);
+            else if constexpr (PAGED) {
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
                     reinterpret_cast<char*>(const_cast<uint16_t*>(a.vc)) + p.at, 0, p.bytes, 0x00020000);
                 const uint32_t at = p.bytes ? ((kt * BN) & ((1u << a.shift) - 1u)) * D * 2 : 0u;
@@ -571,15 +651,19 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         };
         // tile kt of a K (V) resource into K (V) buffer par
         auto dma_k_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) dma_page_k(paged_tile<D>(a, page_of(I, kt), r), par, kt);
-            else {
+            if constexpr (PAGED) {
+                dma_page_k(tile_in(page_of(I, kt), r), par, kt);
+                put_k(par);
+            } else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], kt * BN * D * 2);
             }
         };
         auto dma_v_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) dma_page_v(paged_tile<D>(a, page_of(I, kt), r), par, kt);
-            else {
+            if constexpr (PAGED) {
+                dma_page_v(tile_in(page_of(I, kt), r), par, kt);
+                put_v(par);
+            } else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, vbuf(par) + (LT * i + 64 * wave) * 8, vgo[i], kt * BN * D * 2);
             }
@@ -685,10 +769,10 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
 
         const auto rK = rsrc_k(kvh), rV = rsrc_v(kvh);
         // paged: where the tiles are whose K and V the coming step loads
-        PagedTile at_k{}, at_v{};
+        Tile at_k{}, at_v{};
         if constexpr (PAGED) {
-            at_k = paged_tile<D>(a, page_of(cur, tile_of(NB)), kvh);
-            at_v = paged_tile<D>(a, page_of(cur, tile_of(NB - 1)), kvh);
+            at_k = tile_in(page_of(cur, tile_of(NB)), kvh);
+            at_v = tile_in(page_of(cur, tile_of(NB - 1)), kvh);
         }
         auto dma_k = [&](int par, uint32_t st) {
             if constexpr (PAGED) dma_page_k(at_k, par, tile_of(st));
@@ -986,9 +1070,12 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             }
             if constexpr (PAGED) {
                 at_v = at_k;
-                at_k = paged_tile<D>(a, page, kvh);
+                at_k = tile_in(page, kvh);
             }
-            if constexpr (NB > 2) {
+            if constexpr (KV8) {
+                if (lk) put_k(ph);
+                if (lv) put_v((ph + NB - 1) % NB);
+            } else if constexpr (NB > 2) {
                 // the previous steps' loads (this step's have two steps to land)
                 dma_wait_but((lk ? CH : 0) + (lv ? CH : 0));
             } else {
@@ -1113,7 +1200,14 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // four of the row's output values (unnormalised ones in a piece)
         auto with_odd = [&](f32x4 v, uint32_t d) {
             if constexpr (PAGED) {
-                if (add_odd)
+                if constexpr (KV8) {
+                    if (add_odd) {
+                        const uint32_t nan = nan_dims<D>(a_e, cur.seq, cur.kvh, d, pos_e, cut_tile * BN,
+                                                         (int)min(cur.kmax + 1, (cur.t0 + cur.nt) * BN));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = nan >> e & 1u ? NAN : v[e];
+                    }
+                } else if (add_odd)
 #pragma unroll 1
                     for (int e = 0; e < 4; ++e) {
                         const float x = special_sum<D>(a_e, cur.seq, cur.kvh, d + e, pos_e, cut_tile * BN,
@@ -1215,7 +1309,7 @@ template <int D, bool SPLIT, class A = PrefillArgs>
 __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
 {
     static_assert(D == 256, "two waves of 128 output dimensions");
-    constexpr bool PAGED = std::is_same<A, PagedAttnArgs>::value;
+    constexpr bool PAGED = std::is_base_of<PagedAttnArgs, A>::value, KV8 = std::is_same<A, PagedAttn8Args>::value;
     using Item = typename std::conditional<PAGED, PagedItem, PItem>::type;
     static_assert(!(PAGED && SPLIT), "paged items are split by their chunks");
     constexpr int BN = 64, DH = D / 2;
@@ -1237,7 +1331,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
     };
     Item cur;
     if constexpr (PAGED) {
-        if (!paged_first<512, BN>(args, reinterpret_cast<uint64_t*>(&Kl0[0]), C, cur)) return;
+        using Line = typename std::conditional<KV8, Paged8Line, PagedLine>::type;
+        if (!paged_first<512, BN, Line>(args, reinterpret_cast<uint64_t*>(&Kl0[0]), C, cur)) return;
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
@@ -1266,6 +1361,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             if constexpr (PAGED) return paged_page(a, I.seq, p0 + min(kt, I.nt - 1) * BN);
             else return 0;
         };
+        using Tile = typename std::conditional<KV8, Paged8Tile, PagedTile>::type;
+        typename std::conditional<KV8, Stage8<D, BN, 512>, int>::type stage;  // (see prefill_kernel)
         auto rsrc_at = [&](const uint16_t* pool, uint32_t kv, uint32_t p0, const PagedTile& p) {
             if constexpr (PAGED) {
                 return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(const_cast<uint16_t*>(pool)) + p.at, 0,
@@ -1280,22 +1377,35 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             else return kt * BN * D * 2;
         };
         auto place = [&](const Item& I, uint32_t p0, uint32_t kt) {  // of tile kt
-            if constexpr (PAGED) return paged_tile<D>(a, page_of(I, p0, kt), I.kvh);
+            if constexpr (KV8) return paged8_tile(a, page_of(I, p0, kt), I.kvh);
+            else if constexpr (PAGED) return paged_tile<D>(a, page_of(I, p0, kt), I.kvh);
             else return PagedTile{};
         };
-        auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
-            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.kc, kv, p0, p);
-            const uint32_t at = tile_at(p0, kt, p);
-#pragma unroll
-            for (int i = 0; i < CH; ++i)
-                lds_load16(r, kbuf(par) + (512 * i + 64 * wave) * 8, kgo, at + i * (16 * D * 2));
+        auto put_k = [&](int par) {
+            if constexpr (KV8) stage.store_k(kbuf(par), tid);
         };
-        auto dma_v = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const PagedTile& p) {
-            const __amdgpu_buffer_rsrc_t r = rsrc_at(a.vc, kv, p0, p);
-            const uint32_t at = tile_at(p0, kt, p);
+        auto put_v = [&](int par) {
+            if constexpr (KV8) stage.store_v(vbuf(par), tid);
+        };
+        auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const Tile& p) {
+            if constexpr (KV8) stage.load_k(a, p, p0 + kt * BN, tid);
+            else {
+                const __amdgpu_buffer_rsrc_t r = rsrc_at(a.kc, kv, p0, p);
+                const uint32_t at = tile_at(p0, kt, p);
 #pragma unroll
-            for (int i = 0; i < CH; ++i)
-                lds_load16(r, vbuf(par) + (512 * i + 64 * wave) * 8, vgo, at + i * (64 * (int)kVTile * 2));
+                for (int i = 0; i < CH; ++i)
+                    lds_load16(r, kbuf(par) + (512 * i + 64 * wave) * 8, kgo, at + i * (16 * D * 2));
+            }
+        };
+        auto dma_v = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const Tile& p) {
+            if constexpr (KV8) stage.load_v(a, p, p0 + kt * BN, tid);
+            else {
+                const __amdgpu_buffer_rsrc_t r = rsrc_at(a.vc, kv, p0, p);
+                const uint32_t at = tile_at(p0, kt, p);
+#pragma unroll
+                for (int i = 0; i < CH; ++i)
+                    lds_load16(r, vbuf(par) + (512 * i + 64 * wave) * 8, vgo, at + i * (64 * (int)kVTile * 2));
+            }
         };
         auto dma_done = [] { __builtin_amdgcn_s_waitcnt(0x0f70); };  // vmcnt(0)
         // an item's tiles: how many, from position p0 on, and its last key (split_tiles counts 32 keys, an even
@@ -1325,17 +1435,22 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             uint32_t km, p0;
             const uint32_t n = tiles_of(I, km, p0);
             dma_k(I.kvh, p0, 0, 0, place(I, p0, 0));
-            if (n > 1) dma_k(I.kvh, p0, 1, 1, place(I, p0, 1));
+            put_k(0);
+            if (n > 1) {
+                dma_k(I.kvh, p0, 1, 1, place(I, p0, 1));
+                put_k(1);
+            }
         };
         auto issue_v = [&](const Item& I) {
             uint32_t km, p0;
             tiles_of(I, km, p0);
             dma_v(I.kvh, p0, 0, 0, place(I, p0, 0));
+            put_v(0);
         };
         const uint32_t kvh = cur.kvh;
         uint32_t kmax, p0;
         const uint32_t ntiles = tiles_of(cur, kmax, p0);
-        if (it == 0) {
+        if (KV8 || it == 0) {
             issue_k(cur);
             issue_v(cur);
         }
@@ -1494,7 +1609,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
 
         // step st < ntiles - 1 (ph = st % 2): K(st + 2) replaces K(st), read by the previous step's scores, and
         // V(st + 1) V(st - 1)
-        PagedTile at_k = place(cur, p0, 2), at_v = place(cur, p0, 1);  // of the coming step's loads
+        Tile at_k = place(cur, p0, 2), at_v = place(cur, p0, 1);  // of the coming step's loads
         auto step = [&](int ph, uint32_t st, f32x16& Scur, f32x16& Snext) {
             if (st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, at_k);
             dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
@@ -1540,15 +1655,21 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             }
             if constexpr (PAGED) {
                 at_v = at_k;
-                at_k = paged_tile<D>(a, page, kvh);
+                if constexpr (KV8) at_k = paged8_tile(a, page, kvh);
+                else at_k = paged_tile<D>(a, page, kvh);
             }
-            dma_done();
+            if constexpr (KV8) {
+                if (st + 2 < ntiles) put_k(ph);
+                put_v(ph ^ 1);
+            } else {
+                dma_done();
+            }
             lds_barrier();
         };
         // the item's last tile: no scores follow, so both K buffers are free and the next item's first loads go out
         auto last = [&](int ph, uint32_t st, f32x16& Scur) {
             if constexpr (PAGED) has_next = item_of(it + 1, nxt);
-            if (has_next) {
+            if (!KV8 && has_next) {
                 issue_k(nxt);
                 if (ph == 1) issue_v(nxt);
             }
@@ -1578,7 +1699,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             l = sum_xor32(l);
             Ml[wave][lane] = l;  // read for the last time before the barrier above
             lds_barrier();       // and V is read
-            if (has_next && ph == 0) issue_v(nxt);
+            if (!KV8 && has_next && ph == 0) issue_v(nxt);
         };
         uint32_t st = 0;
         bool odd = false;
@@ -1672,7 +1793,15 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                 for (int u = 0; u < 4; ++u) {
                     f32x4 v = area[(8 * u + er) * 8 + (ec ^ er)];
                     if constexpr (PAGED) {
-                        if (add_odd) {
+                        if (KV8 && add_odd) {
+                            if constexpr (KV8) {
+                                const uint32_t nan = nan_dims<D>(a_e, cur.seq, cur.kvh, col + 32 * b,
+                                                                 cur.pos0 + (int)row_from(a_e, cur, qw * 32 + 8 * u + er).t,
+                                                                 (cur.t0 + cut_tile) * BN, (int)min(cur.kmax + 1, (cur.t0 + cur.nt) * BN));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) v[e] = nan >> e & 1u ? NAN : v[e];
+                            }
+                        } else if (add_odd) {
                             const int pos = cur.pos0 + (int)row_from(a_e, cur, qw * 32 + 8 * u + er).t;
 #pragma unroll 1
                             for (int e = 0; e < 4; ++e) {
