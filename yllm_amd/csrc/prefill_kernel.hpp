@@ -123,7 +123,8 @@ __device__ inline int chunk_swz(int r)
 template <int D, int BN, int LT>
 struct Stage8 {
     static constexpr int CB = BN * D / (16 * LT), KC = D / 16, VC = BN / 16;  // 16-code chunks a thread, a K row, a V row
-    static_assert(LT % VC == 0, "a thread's V chunks are of the same positions");
+    static constexpr int KR = LT / KC, VR = LT / VC;                          // rows between a thread's chunks
+    static_assert(LT % VC == 0 && KR % 16 == 0 && VR % 16 == 0, "a thread's chunks differ by a constant");
     u32x4 k[CB], v[CB], vs;
     uint32_t ks[CB];
 
@@ -131,48 +132,60 @@ struct Stage8 {
     {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + at, 0, bytes, 0x00020000);
     }
-    // the tile from key `key` on, in the page at p; t: the thread's number
-    __device__ void load_k(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t)
+    // (the thread's number passes through an opaque move in each of these: what is derived from it is a few instructions,
+    // and kept from step to step it spilled, whose reloads then waited for the loads in flight)
+    static __device__ uint32_t fresh(int t)
     {
+        uint32_t u = (uint32_t)t;
+        asm volatile("" : "+v"(u));
+        return u;
+    }
+    // the tile from key `key` on, in the page at p; t0: the thread's number
+    __device__ void load_k(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t0)
+    {
+        const uint32_t t = fresh(t0), at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
         const __amdgpu_buffer_rsrc_t r = rsrc(a.kc, p.at * D, p.bytes * D), rs = rsrc(a.ks, p.at, p.bytes);
-        const uint32_t at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (t + LT * i) * 16, at * D, 0));
-            ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, (t + LT * i) / KC, at, 0);
+            k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, t * 16, at * D + i * (LT * 16), 0));
+            ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, t / KC, at + i * KR, 0);
         }
     }
-    __device__ void load_v(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t)
+    __device__ void load_v(const PagedAttn8Args& a, const Paged8Tile& p, uint32_t key, int t0)
     {
+        const uint32_t t = fresh(t0), at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
         const __amdgpu_buffer_rsrc_t r = rsrc(a.vc, p.at * D, p.bytes * D), rs = rsrc(a.vs, p.at, p.bytes);
-        const uint32_t at = p.bytes ? key & ((1u << a.shift) - 1u) : 0u;
         const uint32_t tile = (at & ~(kV8Tile - 1)) * D + (at & (kV8Tile - 1));  // (a tile may be half of one of 64 positions)
 #pragma unroll
         for (int i = 0; i < CB; ++i)
-            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                 r, (t + LT * i) / VC * (int)kV8Tile + t % VC * 16, tile, 0));
+            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, t / VC * kV8Tile + t % VC * 16,
+                                                                                   tile + i * (VR * kV8Tile), 0));
         vs = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, t % VC * 16, at, 0));
     }
-    __device__ void store_k(_Float16* lds, int t) const
+    __device__ void store_k(_Float16* lds, int t0) const
     {
+        const uint32_t t = fresh(t0), c = 2 * (t % KC);
+        const int r = lds_row_of_key(t / KC), swz = chunk_swz<D / 8>(r);  // (both of the row's low four bits only)
+        _Float16 *const p0 = lds + r * D + ((c ^ swz) << 3), *const p1 = lds + r * D + (((c + 1) ^ swz) << 3);
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            const int L = t + LT * i, r = lds_row_of_key(L / KC), c = 2 * (L % KC), swz = chunk_swz<D / 8>(r);
             const float scale = kv8_scale(ks[i]);
-            *reinterpret_cast<f16x8*>(lds + r * D + ((c ^ swz) << 3)) = kv8_values(k[i][0], k[i][1], scale);
-            *reinterpret_cast<f16x8*>(lds + r * D + (((c + 1) ^ swz) << 3)) = kv8_values(k[i][2], k[i][3], scale);
+            *reinterpret_cast<f16x8*>(p0 + i * (KR * D)) = kv8_values(k[i][0], k[i][1], scale);
+            *reinterpret_cast<f16x8*>(p1 + i * (KR * D)) = kv8_values(k[i][2], k[i][3], scale);
         }
     }
-    __device__ void store_v(_Float16* lds, int t) const
+    __device__ void store_v(_Float16* lds, int t0) const
     {
+        const uint32_t t = fresh(t0), c = 2 * (t % VC);
+        const int d = t / VC, swz = chunk_swz<BN / 8>(d);
+        _Float16 *const p0 = lds + d * BN + ((c ^ swz) << 3), *const p1 = lds + d * BN + (((c + 1) ^ swz) << 3);
         f16x2 f[2][4];
 #pragma unroll
         for (int w = 0; w < 8; ++w) f[w >> 2][w & 3] = kv8_factors(vs[w >> 1], w & 1);
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
-            const int d = (t + LT * i) / VC, c = 2 * (t % VC), swz = chunk_swz<BN / 8>(d);
-            *reinterpret_cast<f16x8*>(lds + d * BN + ((c ^ swz) << 3)) = kv8_values(v[i][0], v[i][1], f[0]);
-            *reinterpret_cast<f16x8*>(lds + d * BN + (((c + 1) ^ swz) << 3)) = kv8_values(v[i][2], v[i][3], f[1]);
+            *reinterpret_cast<f16x8*>(p0 + i * (VR * BN)) = kv8_values(v[i][0], v[i][1], f[0]);
+            *reinterpret_cast<f16x8*>(p1 + i * (VR * BN)) = kv8_values(v[i][2], v[i][3], f[1]);
         }
     }
 };
@@ -1612,7 +1625,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
         Tile at_k = place(cur, p0, 2), at_v = place(cur, p0, 1);  // of the coming step's loads
         auto step = [&](int ph, uint32_t st, f32x16& Scur, f32x16& Snext) {
             if (st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, at_k);
-            dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
+            if constexpr (!KV8) dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
             const uint32_t page = page_of(cur, p0, st + 3);  // (read here, used at the step's end)
             // opaque each step, or the compiler keeps a second set of offsets for the other buffers (and spills)
 #pragma unroll
@@ -1645,6 +1658,10 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                 Pl[wave][1][lane] = pf[1];
                 pv(pf, ph, 0);
             }
+            if constexpr (KV8) {  // half a step each, so that the registers of one are free for the other
+                if (st + 2 < ntiles) put_k(ph);
+                dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
+            }
             lds_barrier();  // the pair's probabilities are in LDS
             if (st < wsteps) {
                 f16x8 po[2];
@@ -1659,7 +1676,6 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                 else at_k = paged_tile<D>(a, page, kvh);
             }
             if constexpr (KV8) {
-                if (st + 2 < ntiles) put_k(ph);
                 put_v(ph ^ 1);
             } else {
                 dma_done();
