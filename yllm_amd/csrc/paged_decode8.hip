@@ -27,6 +27,7 @@ namespace {
 constexpr uint32_t kUnit8 = 256;      // keys of a unit: one 64-key block a wave
 constexpr uint32_t kItem8Units = 1;   // an item's fixed cost
 constexpr int kRows = 16;
+constexpr int kWaves64 = 2;           // waves a SIMD at head_dim 64 (its blocks are 8 KB)
 
 __device__ inline f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c)
 {
@@ -127,16 +128,20 @@ __device__ inline bool decode8_whole(const PagedAttn8Args& a, Decode8Piece& I)
 // one 64-key block of K and V as loaded by a lane: of MFMA a's key the dimensions 64 c + 16 g .. + 15; of dimension
 // 16 b + n the positions 16 g .. + 15; and sixteen scales of each
 template <int D>
-struct Frag8 {
-    u32x4 k[4][D / 64];
-    u32x4 v[D / 16];
-    u32x4 ks, vs;
+struct FragK8 {
+    u32x4 k[4][D / 64], s;
+};
+template <int D>
+struct FragV8 {
+    u32x4 v[D / 16], s;
 };
 
 template <int D, bool PREC, int POL>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(PagedAttn8Args args)
+__global__ __launch_bounds__(256, D == 64 ? kWaves64 : D == 128 ? 2 : 1) void paged_decode8_kernel(PagedAttn8Args args)
 {
     constexpr int kWaves = 4, D4 = D / 4, NC = D / 64, NB = D / 16, QROW = D + 8;
+    // (head_dim 256: one block of V at a time, the next one's loads go out behind its products; two are too many registers)
+    constexpr bool ONE = D > 128;
     // each wave's O rows; before the key loop, the queries (hi, lo) [2][16][QROW]
     __shared__ __attribute__((aligned(16))) float s_o[kWaves][kRows][D + 4];
     __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
@@ -182,31 +187,40 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(Pa
                 for (int e = 0; e < 4; ++e) qv[r][e] = a.q_dtype == kBF16 ? bf16_bits_to_f32(w[e]) : f16_bits_to_f32(w[e]);
             }
         }
-        auto load = [&](Frag8<D>& f, uint32_t i, uint32_t page) {
-            const Paged8Tile p = paged8_tile(a, page, I.kvh);  // outside the pool: no bytes, zeros are read
-            const uint32_t off = key_of(i) & ((1u << a.shift) - 1u), codes = p.bytes * D;
-            auto rsrc = [&](const void* base, uint64_t at, uint32_t bytes) {
-                return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + at, 0, bytes, 0x00020000);
-            };
-            const __amdgpu_buffer_rsrc_t rK = rsrc(a.kc, p.at * D, codes), rV = rsrc(a.vc, p.at * D, codes);
-            const __amdgpu_buffer_rsrc_t rKs = rsrc(a.ks, p.at, p.bytes), rVs = rsrc(a.vs, p.at, p.bytes);
-            const uint32_t at = p.bytes ? off : 0u;
-            f.ks = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rKs, (n >> 2) * 16, at, POL));
+        auto rsrc = [&](const void* base, uint64_t at, uint32_t bytes) {
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(reinterpret_cast<const char*>(base)) + at, 0, bytes, 0x00020000);
+        };
+        // block i, in page `page` (outside the pool: no bytes, zeros are read); all but 4 KB of what a load adds to its
+        // lane's place is scalar, or every load keeps a register of its own for its address
+        auto load_k = [&](FragK8<D>& f, uint32_t i, uint32_t page) {
+            const Paged8Tile p = paged8_tile(a, page, I.kvh);
+            const uint32_t at = p.bytes ? key_of(i) & ((1u << a.shift) - 1u) : 0u;
+            const __amdgpu_buffer_rsrc_t r = rsrc(a.kc, p.at * D, p.bytes * D);
+            f.s = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.ks, p.at, p.bytes), (n >> 2) * 16, at, POL));
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
                     f.k[q][c] = __builtin_bit_cast(
-                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(rK, k_lane + 4 * q * D + c * 64, at * D, POL));
-            f.vs = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rVs, g * 16, at, POL));
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + c * 64, at * D + 4 * q * D, POL));
+        };
+        auto load_v = [&](FragV8<D>& f, uint32_t i, uint32_t page) {
+            const Paged8Tile p = paged8_tile(a, page, I.kvh);
+            const uint32_t at = p.bytes ? key_of(i) & ((1u << a.shift) - 1u) : 0u;
+            const __amdgpu_buffer_rsrc_t r = rsrc(a.vc, p.at * D, p.bytes * D);
+            f.s = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(a.vs, p.at, p.bytes), g * 16, at, POL));
 #pragma unroll
             for (int b = 0; b < NB; ++b)
                 f.v[b] = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(rV, v_lane + b * 16 * (int)kV8Tile, at * D, POL));
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + (b & 3) * 16 * kV8Tile,
+                                                                 at * D + (b >> 2) * 64 * kV8Tile, POL));
         };
-        Frag8<D> f0, f1;
-        load(f0, 0, page_of(0));
-        load(f1, 1, page_of(1));
+        FragK8<D> k0, k1;
+        FragV8<D> v0, v1;
+        load_k(k0, 0, page_of(0));
+        load_v(v0, 0, page_of(0));
+        load_k(k1, 1, page_of(1));
+        if constexpr (!ONE) load_v(v1, 1, page_of(1));
         uint32_t page0 = page_of(2), page1 = page_of(3);
         __builtin_amdgcn_sched_barrier(0);  // nothing below waits before these are issued
 
@@ -246,22 +260,23 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(Pa
         for (int b = 0; b < NB; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
         // (only a wave's last block can hold keys that some row does not see: they are among the last 16)
-        auto compute = [&](Frag8<D>& f, uint32_t i, auto last) {
+        auto compute = [&](FragK8<D>& fk, FragV8<D>& fv, uint32_t i, auto last, auto&& refill) {
             const int key0 = (int)key_of(i);
             f32x4 s[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float scale = kv8_scale(f.ks[q] >> 8 * (n & 3) & 0xffu);
+                const float scale = kv8_scale(fk.s[q] >> 8 * (n & 3) & 0xffu);
                 s[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2 * NC; ++c) {
-                    const u32x4& w = f.k[q][c >> 1];
+                    const u32x4& w = fk.k[q][c >> 1];
                     const f16x8 k = kv8_values(w[2 * (c & 1)], w[2 * (c & 1) + 1], scale);
                     s[q] = mfma16(k, qhi[c], s[q]);
                     if constexpr (LO) s[q] = mfma16(k, qlo[c], s[q]);
                     else if constexpr (PREC) s[q] = mfma16(k, read_q(1, c), s[q]);
                 }
             }
+            if constexpr (ONE) refill();
             float x[16];  // row n, key key0 + 16 g + j
 #pragma unroll
             for (int j = 0; j < 16; ++j) x[j] = s[j >> 2][j & 3];
@@ -283,15 +298,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(Pa
                     keep[w] = kp;
                     hid[w] = hd;
                 }
-                f.vs &= keep;
+                fv.s &= keep;
                 uint32_t any = 0;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const uint32_t v = f.v[b][w] & keep[w], t = kv8_nans(v) & hid[w];
+                        const uint32_t v = fv.v[b][w] & keep[w], t = kv8_nans(v) & hid[w];
                         any |= t;
-                        f.v[b][w] = v & ~(t | (t - (t >> 7)));
+                        fv.v[b][w] = v & ~(t | (t - (t >> 7)));
                     }
                 odd = odd || any != 0;
             }
@@ -317,27 +332,52 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(Pa
             }
             f16x2 fac[2][4];
 #pragma unroll
-            for (int w = 0; w < 8; ++w) fac[w >> 2][w & 3] = kv8_factors(f.vs[w >> 1], w & 1);
+            for (int w = 0; w < 8; ++w) fac[w >> 2][w & 3] = kv8_factors(fv.s[w >> 1], w & 1);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const f16x8 v = kv8_values(f.v[b][2 * h], f.v[b][2 * h + 1], fac[h]);
+                    const f16x8 v = kv8_values(fv.v[b][2 * h], fv.v[b][2 * h + 1], fac[h]);
                     o[b] = mfma16(v, pf[h], o[b]);
                     o[b] = mfma16(v, pl[h], o[b]);
                 }
         };
+        auto none = [] {};
         uint32_t i = 0;
-        for (; i + 2 < nbw; i += 2) {
-            compute(f0, i, std::false_type{});
-            load(f0, i + 2, page0);
-            page0 = page_of(i + 4);
-            compute(f1, i + 1, std::false_type{});
-            load(f1, i + 3, page1);  // (past the wave's last block: page ~0, zeros without a read)
-            page1 = page_of(i + 5);
+        // (past the wave's last block: page ~0, zeros without a read)
+        if constexpr (ONE) {
+            uint32_t page2 = page0, page_v = page_of(1);  // of K(i + 2), K(i + 3) and V(i + 1)
+            for (; i + 2 < nbw; i += 2) {
+                compute(k0, v0, i, std::false_type{}, [&] { load_k(k0, i + 2, page2); });
+                load_v(v0, i + 1, page_v);
+                page_v = page2;
+                page2 = page_of(i + 4);
+                compute(k1, v0, i + 1, std::false_type{}, [&] { load_k(k1, i + 3, page1); });
+                load_v(v0, i + 2, page_v);
+                page_v = page1;
+                page1 = page_of(i + 5);
+            }
+            if (i < nbw) {
+                compute(k0, v0, i, std::true_type{}, none);
+                if (i + 1 < nbw) {
+                    load_v(v0, i + 1, page_v);
+                    compute(k1, v0, i + 1, std::true_type{}, none);
+                }
+            }
+        } else {
+            for (; i + 2 < nbw; i += 2) {
+                compute(k0, v0, i, std::false_type{}, none);
+                load_k(k0, i + 2, page0);
+                load_v(v0, i + 2, page0);
+                page0 = page_of(i + 4);
+                compute(k1, v1, i + 1, std::false_type{}, none);
+                load_k(k1, i + 3, page1);
+                load_v(v1, i + 3, page1);
+                page1 = page_of(i + 5);
+            }
+            if (i < nbw) compute(k0, v0, i, std::true_type{}, none);
+            if (i + 1 < nbw) compute(k1, v1, i + 1, std::true_type{}, none);
         }
-        if (i < nbw) compute(f0, i, std::true_type{});
-        if (i + 1 < nbw) compute(f1, i + 1, std::true_type{});
 
         l = sum_xor32(sum_xor16(l));
         lds_barrier();  // every wave has read its queries
@@ -513,7 +553,7 @@ uint32_t decode8_wgs(uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_
     const uint32_t units = (max_len + kUnit8 - 1) / kUnit8;
     if (units <= units_of_bytes(kWholeBytes, D)) return 0;  // no item is cut: a workgroup each
     const uint64_t most = (uint64_t)n_seq * row_blocks(max_new, n_heads, n_kv) * n_kv * (units + kItem8Units);
-    const uint64_t full = (uint64_t)(D <= 128 ? 2 : 1) * (uint64_t)n_cus();
+    const uint64_t full = (uint64_t)(D == 64 ? kWaves64 : D == 128 ? 2 : 1) * (uint64_t)n_cus();
     return (uint32_t)(((most < full ? most : full) + 7) / 8 * 8);
 }
 

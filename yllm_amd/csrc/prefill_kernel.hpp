@@ -162,31 +162,46 @@ struct Stage8 {
                                                                                    tile + i * (VR * kV8Tile), 0));
         vs = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, t % VC * 16, at, 0));
     }
-    __device__ void store_k(_Float16* lds, int t0) const
+    // Where the thread's chunks go, and chunk n of 2 CB (constant after unrolling): so that they can be written between
+    // other work.
+    struct Place {
+        _Float16 *p0, *p1;
+    };
+    static __device__ Place place_k(_Float16* lds, int t0)
     {
         const uint32_t t = fresh(t0), c = 2 * (t % KC);
         const int r = lds_row_of_key(t / KC), swz = chunk_swz<D / 8>(r);  // (both of the row's low four bits only)
-        _Float16 *const p0 = lds + r * D + ((c ^ swz) << 3), *const p1 = lds + r * D + (((c + 1) ^ swz) << 3);
-#pragma unroll
-        for (int i = 0; i < CB; ++i) {
-            const float scale = kv8_scale(ks[i]);
-            *reinterpret_cast<f16x8*>(p0 + i * (KR * D)) = kv8_values(k[i][0], k[i][1], scale);
-            *reinterpret_cast<f16x8*>(p1 + i * (KR * D)) = kv8_values(k[i][2], k[i][3], scale);
-        }
+        return Place{lds + r * D + ((c ^ swz) << 3), lds + r * D + (((c + 1) ^ swz) << 3)};
     }
-    __device__ void store_v(_Float16* lds, int t0) const
+    static __device__ Place place_v(_Float16* lds, int t0)
     {
         const uint32_t t = fresh(t0), c = 2 * (t % VC);
         const int d = t / VC, swz = chunk_swz<BN / 8>(d);
-        _Float16 *const p0 = lds + d * BN + ((c ^ swz) << 3), *const p1 = lds + d * BN + (((c + 1) ^ swz) << 3);
-        f16x2 f[2][4];
+        return Place{lds + d * BN + ((c ^ swz) << 3), lds + d * BN + (((c + 1) ^ swz) << 3)};
+    }
+    __device__ void put_k(const Place& p, int n) const
+    {
+        const int i = n >> 1, h = n & 1;
+        *reinterpret_cast<f16x8*>((h ? p.p1 : p.p0) + i * (KR * D)) = kv8_values(k[i][2 * h], k[i][2 * h + 1], kv8_scale(ks[i]));
+    }
+    __device__ void put_v(const Place& p, int n) const
+    {
+        const int i = n / CB ? n - CB : n, h = n / CB;  // (the halves one after the other: their factors differ)
+        const f16x2 f[4] = {kv8_factors(vs[2 * h], 0), kv8_factors(vs[2 * h], 1), kv8_factors(vs[2 * h + 1], 0),
+                            kv8_factors(vs[2 * h + 1], 1)};
+        *reinterpret_cast<f16x8*>((h ? p.p1 : p.p0) + i * (VR * BN)) = kv8_values(v[i][2 * h], v[i][2 * h + 1], f);
+    }
+    __device__ void store_k(_Float16* lds, int t0) const
+    {
+        const Place p = place_k(lds, t0);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) f[w >> 2][w & 3] = kv8_factors(vs[w >> 1], w & 1);
+        for (int n = 0; n < 2 * CB; ++n) put_k(p, n);
+    }
+    __device__ void store_v(_Float16* lds, int t0) const
+    {
+        const Place p = place_v(lds, t0);
 #pragma unroll
-        for (int i = 0; i < CB; ++i) {
-            *reinterpret_cast<f16x8*>(p0 + i * (VR * BN)) = kv8_values(v[i][0], v[i][1], f[0]);
-            *reinterpret_cast<f16x8*>(p1 + i * (VR * BN)) = kv8_values(v[i][2], v[i][3], f[1]);
-        }
+        for (int n = 0; n < 2 * CB; ++n) put_v(p, n);
     }
 };
 
@@ -551,11 +566,11 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     // stores.  With a gate the epilogue loads the gate values, which would
     // then wait behind these loads; such items issue their loads at their
     // own start.
-    const bool early = args.gate == nullptr && !PAIR && !KV8;
+    const bool early = args.gate == nullptr && !PAIR && !(KV8 && QS);
     // paged, 16-bit queries: an item waits for the next one's first loads before
     // its output stores instead of behind them, so the stores drain during the
     // next item's first step
-    constexpr bool AHEAD = PAGED && !KV8 && !QS && NB == 2;
+    constexpr bool AHEAD = PAGED && !QS && NB == 2;
     Item cur;
     if constexpr (PAGED) {
         using Line = typename std::conditional<KV8, Paged8Line, PagedLine>::type;
@@ -563,6 +578,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
+    // (8 bits: tiles on their way from memory to LDS; an item's second K tile from the end of the one before)
+    typename std::conditional<KV8, Stage8<D, BN, LT>, int>::type stage;
     for (uint32_t it = 0;; ++it) {
         const A& a = fresh_args(args);
         // Thread indices pass through an opaque move each item so that nothing
@@ -630,7 +647,6 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         };
         // (8 bits: loaded into registers here, written to LDS by put_k and put_v)
         using Tile = typename std::conditional<KV8, Paged8Tile, PagedTile>::type;
-        typename std::conditional<KV8, Stage8<D, BN, LT>, int>::type stage;
         auto tile_in = [&](uint32_t page, uint32_t kv) {
             if constexpr (KV8) return paged8_tile(a, page, kv);
             else if constexpr (PAGED) return paged_tile<D>(a, page, kv);
@@ -664,19 +680,15 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         };
         // tile kt of a K (V) resource into K (V) buffer par
         auto dma_k_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) {
-                dma_page_k(tile_in(page_of(I, kt), r), par, kt);
-                put_k(par);
-            } else {
+            if constexpr (PAGED) dma_page_k(tile_in(page_of(I, kt), r), par, kt);
+            else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, kbuf(par) + (LT * i + 64 * wave) * 8, kgo[i], kt * BN * D * 2);
             }
         };
         auto dma_v_of = [&](const Item& I, auto r, int par, uint32_t kt) {
-            if constexpr (PAGED) {
-                dma_page_v(tile_in(page_of(I, kt), r), par, kt);
-                put_v(par);
-            } else {
+            if constexpr (PAGED) dma_page_v(tile_in(page_of(I, kt), r), par, kt);
+            else {
 #pragma unroll
                 for (int i = 0; i < CH; ++i) lds_load16(r, vbuf(par) + (LT * i + 64 * wave) * 8, vgo[i], kt * BN * D * 2);
             }
@@ -740,8 +752,34 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if (n > 1) dma_v_of(I, rsrc_v(I.kvh), 1, t0 + 1);
             return (n > 2 ? CH : 0) + (n > 1 ? CH : 0);
         };
+        // 8 bits: an item's first K and V tile into registers, from there into LDS, and its second K tile on its way
+        // (written in the prologue): the same registers as in the key loop
+        auto load_first = [&](const Item& I) {
+            if constexpr (KV8) {
+                uint32_t t0;
+                if (item_steps(I, t0) == 0) return;
+                dma_k_of(I, rsrc_k(I.kvh), 0, t0 + grp);
+                dma_v_of(I, rsrc_v(I.kvh), 0, t0 + grp);
+            }
+        };
+        auto put_first = [&](const Item& I) {
+            if constexpr (KV8) {
+                uint32_t t0;
+                const uint32_t n = item_steps(I, t0);
+                if (n > 0) {
+                    put_k(0);
+                    put_v(0);
+                }
+                if (n > 1) dma_k_of(I, rsrc_k(I.kvh), 1, t0 + grp + NG);
+            }
+        };
         uint32_t deep_loads = 0;  // loads the prologue need not wait for
-        if (it == 0 || !early) {
+        if (KV8 && (it == 0 || !early)) {
+            if (it > 0) __syncthreads();
+            load_first(cur);
+            issue_item_q(cur);
+            put_first(cur);
+        } else if (it == 0 || !early) {
             if (it > 0) __syncthreads();  // the previous item's epilogue read LDS these loads overwrite
             issue_item_k(cur);
             issue_item_v(cur);
@@ -986,7 +1024,7 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // -> 79 us).  All loads are complete before the key loop, whose waits then
         // count only tile loads (in pair mode K(2) and V(1) may still be in
         // flight; the first step waits for them).
-        if constexpr (!AHEAD) dma_wait_but(deep_loads);
+        if constexpr (!AHEAD && !KV8) dma_wait_but(deep_loads);
         if (QL && it > 0) lds_barrier();  // the merge has read (max, sum)
         if constexpr (QS) {
             const float* qp = reinterpret_cast<const float*>(a.q) + (size_t)myrow.b * a.q_stride + (size_t)myrow.h * D +
@@ -1010,6 +1048,19 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         if (wsteps > 0) {
             qk(Sa, 0);
             xwrite(Sa, 0);
+        }
+        if constexpr (KV8) {
+            if (gsteps > 1) put_k(1);
+            if constexpr (NB > 2) {  // K(2) and V(1)
+                if (gsteps > 2) {
+                    dma_k_of(cur, rK, 2, tile_of(2));
+                    put_k(2);
+                }
+                if (gsteps > 1) {
+                    dma_v_of(cur, rV, 1, tile_of(1));
+                    put_v(1);
+                }
+            }
         }
         // step 0 loads K(NB) over K(0), whose last readers are the scores above
         if constexpr (NB > 2 || AHEAD) lds_barrier();
@@ -1054,8 +1105,12 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
             if (PAGED && early && st == last_st) prefetch = has_next = item_of(it + 1, nxt);
             if (prefetch && st == last_st) {
                 // K buffers are free (no scores follow), V buffer 1-p too
-                issue_item_k(nxt);
-                if (ph == 1 || gsteps == 0) issue_item_v(nxt);
+                if constexpr (KV8) {
+                    load_first(nxt);  // (written after the key loop)
+                } else {
+                    issue_item_k(nxt);
+                    if (ph == 1 || gsteps == 0) issue_item_v(nxt);
+                }
             }
             if constexpr (PAGED) {
                 // workgroup-uniform: some group's tile is cut, or the last one
@@ -1124,7 +1179,8 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
         // the next item's first V tile when the last step still read V buffer 0,
         // and its queries
         if (prefetch) {
-            if (gsteps > 0 && (last_st & 1u) == 0) issue_item_v(nxt);
+            if constexpr (KV8) put_first(nxt);  // (the step's barrier is behind every read of these buffers)
+            else if (gsteps > 0 && (last_st & 1u) == 0) issue_item_v(nxt);
             issue_item_q(nxt);
         }
         {
@@ -1349,6 +1405,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
+    typename std::conditional<KV8, Stage8<D, BN, 512>, int>::type stage;  // (see prefill_kernel)
     for (uint32_t it = 0;; ++it) {
         const A& a = fresh_args(args);
         int tid;  // opaque per item, as in prefill_kernel
@@ -1375,7 +1432,6 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             else return 0;
         };
         using Tile = typename std::conditional<KV8, Paged8Tile, PagedTile>::type;
-        typename std::conditional<KV8, Stage8<D, BN, 512>, int>::type stage;  // (see prefill_kernel)
         auto rsrc_at = [&](const uint16_t* pool, uint32_t kv, uint32_t p0, const PagedTile& p) {
             if constexpr (PAGED) {
                 return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(const_cast<uint16_t*>(pool)) + p.at, 0,
@@ -1393,12 +1449,6 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             if constexpr (KV8) return paged8_tile(a, page_of(I, p0, kt), I.kvh);
             else if constexpr (PAGED) return paged_tile<D>(a, page_of(I, p0, kt), I.kvh);
             else return PagedTile{};
-        };
-        auto put_k = [&](int par) {
-            if constexpr (KV8) stage.store_k(kbuf(par), tid);
-        };
-        auto put_v = [&](int par) {
-            if constexpr (KV8) stage.store_v(vbuf(par), tid);
         };
         auto dma_k = [&](uint32_t kv, uint32_t p0, int par, uint32_t kt, const Tile& p) {
             if constexpr (KV8) stage.load_k(a, p, p0 + kt * BN, tid);
@@ -1448,22 +1498,41 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             uint32_t km, p0;
             const uint32_t n = tiles_of(I, km, p0);
             dma_k(I.kvh, p0, 0, 0, place(I, p0, 0));
-            put_k(0);
-            if (n > 1) {
-                dma_k(I.kvh, p0, 1, 1, place(I, p0, 1));
-                put_k(1);
-            }
+            if (n > 1) dma_k(I.kvh, p0, 1, 1, place(I, p0, 1));
         };
         auto issue_v = [&](const Item& I) {
             uint32_t km, p0;
             tiles_of(I, km, p0);
             dma_v(I.kvh, p0, 0, 0, place(I, p0, 0));
-            put_v(0);
+        };
+        // (8 bits: as in prefill_kernel)
+        auto load_first = [&](const Item& I) {
+            if constexpr (KV8) {
+                uint32_t km, p0;
+                tiles_of(I, km, p0);
+                const Tile p = place(I, p0, 0);
+                stage.load_k(a, p, p0, tid);
+                stage.load_v(a, p, p0, tid);
+            }
+        };
+        auto put_first = [&](const Item& I) {
+            if constexpr (KV8) {
+                uint32_t km, p0;
+                tiles_of(I, km, p0);
+                stage.store_k(kbuf(0), tid);
+                stage.store_v(vbuf(0), tid);
+            }
         };
         const uint32_t kvh = cur.kvh;
         uint32_t kmax, p0;
         const uint32_t ntiles = tiles_of(cur, kmax, p0);
-        if (KV8 || it == 0) {
+        if constexpr (KV8) {
+            if (it == 0) {
+                load_first(cur);
+                put_first(cur);
+            }
+            stage.load_k(a, place(cur, p0, 1), p0 + BN, tid);  // (of a single tile's page again: not read)
+        } else if (it == 0) {
             issue_k(cur);
             issue_v(cur);
         }
@@ -1574,7 +1643,8 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             pf[i >> 3][i & 7] = (_Float16)p;
         };
         // O^T += V^T P^T over the wave's own or its partner's keys of the tile in V buffer par
-        auto pv = [&](const f16x8 (&pf)[2], int par, int other) {
+        // (between: called after each MFMA)
+        auto pv = [&](const f16x8 (&pf)[2], int par, int other, auto&& between) {
             constexpr int NM = 2 * NDB;  // MFMA n: k-slot n / NDB, block n % NDB
             f16x8 vf[3];
             vf[0] = read_v(par, 0, other, 0);
@@ -1583,8 +1653,10 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             for (int n = 0; n < NM; ++n) {
                 if (n + 2 < NM) vf[(n + 2) % 3] = read_v(par, (n + 2) % NDB, other, (n + 2) / NDB);
                 o[n % NDB] = mfma32(vf[n % 3], pf[n / NDB], o[n % NDB]);
+                between(n);
             }
         };
+        auto nothing = [](int) {};
 
         // paged: the tiles cut by the item's mask (clean_v)
         uint32_t cut_tile = ~0u;
@@ -1606,7 +1678,7 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
         };
 
         // prologue: the item's first loads are in flight
-        dma_done();
+        if constexpr (!KV8) dma_done();
         if (a.q_dtype == kBF16) {
 #pragma unroll
             for (int kk = 0; kk < NKK; ++kk) bf16_to_f16(qf[kk]);
@@ -1618,14 +1690,16 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
             for (int kk = 0; kk < NKK; ++kk) Sa = mfma32(read_k(0, kk), qf[kk], kk == 0 ? f32x16{} : Sa);
             tile_max(Sa, 0);
         }
+        if constexpr (KV8) stage.store_k(kbuf(1), tid);
         lds_barrier();
 
         // step st < ntiles - 1 (ph = st % 2): K(st + 2) replaces K(st), read by the previous step's scores, and
         // V(st + 1) V(st - 1)
         Tile at_k = place(cur, p0, 2), at_v = place(cur, p0, 1);  // of the coming step's loads
         auto step = [&](int ph, uint32_t st, f32x16& Scur, f32x16& Snext) {
-            if (st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, at_k);
-            if constexpr (!KV8) dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
+            // (8 bits: the last K tile again where none is left; nothing reads it)
+            if (KV8 || st + 2 < ntiles) dma_k(kvh, p0, ph, st + 2, at_k);
+            dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
             const uint32_t page = page_of(cur, p0, st + 3);  // (read here, used at the step's end)
             // opaque each step, or the compiler keeps a second set of offsets for the other buffers (and spills)
 #pragma unroll
@@ -1656,30 +1730,40 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                 }
                 Pl[wave][0][lane] = pf[0];
                 Pl[wave][1][lane] = pf[1];
-                pv(pf, ph, 0);
-            }
-            if constexpr (KV8) {  // half a step each, so that the registers of one are free for the other
-                if (st + 2 < ntiles) put_k(ph);
-                dma_v(kvh, p0, ph ^ 1, st + 1, at_v);
+                if constexpr (KV8) {  // the conversions between the MFMAs (after them, all waves at once: 0.3 us a step)
+                    const auto at = stage.place_k(kbuf(ph), tid);
+                    pv(pf, ph, 0, [&](int n) {
+                        if (n & 1) stage.put_k(at, n >> 1);
+                    });
+                } else {
+                    pv(pf, ph, 0, nothing);
+                }
+            } else if constexpr (KV8) {
+                stage.store_k(kbuf(ph), tid);
             }
             lds_barrier();  // the pair's probabilities are in LDS
             if (st < wsteps) {
                 f16x8 po[2];
                 po[0] = Pl[wave ^ 1][0][lane];
                 po[1] = Pl[wave ^ 1][1][lane];
-                pv(po, ph, 1);
+                if constexpr (KV8) {
+                    const auto at = stage.place_v(vbuf(ph ^ 1), tid);
+                    pv(po, ph, 1, [&](int n) {
+                        if (n & 1) stage.put_v(at, n >> 1);
+                    });
+                } else {
+                    pv(po, ph, 1, nothing);
+                }
                 tile_max(Snext, st + 1);
+            } else if constexpr (KV8) {
+                stage.store_v(vbuf(ph ^ 1), tid);
             }
             if constexpr (PAGED) {
                 at_v = at_k;
                 if constexpr (KV8) at_k = paged8_tile(a, page, kvh);
                 else at_k = paged_tile<D>(a, page, kvh);
             }
-            if constexpr (KV8) {
-                put_v(ph ^ 1);
-            } else {
-                dma_done();
-            }
+            if constexpr (!KV8) dma_done();
             lds_barrier();
         };
         // the item's last tile: no scores follow, so both K buffers are free and the next item's first loads go out
@@ -1703,19 +1787,20 @@ __global__ __launch_bounds__(512) void prefill_halves_kernel(A args)
                 for (int i = 0; i < 16; ++i) prob(Scur, pf, i);
                 Pl[wave][0][lane] = pf[0];
                 Pl[wave][1][lane] = pf[1];
-                pv(pf, ph, 0);
+                pv(pf, ph, 0, nothing);
             }
             lds_barrier();
             if (st < wsteps) {
                 f16x8 po[2];
                 po[0] = Pl[wave ^ 1][0][lane];
                 po[1] = Pl[wave ^ 1][1][lane];
-                pv(po, ph, 1);
+                pv(po, ph, 1, nothing);
             }
             l = sum_xor32(l);
             Ml[wave][lane] = l;  // read for the last time before the barrier above
             lds_barrier();       // and V is read
-            if (!KV8 && has_next && ph == 0) issue_v(nxt);
+            if (KV8 && has_next) {load_first(nxt); put_first(nxt);}
+            else if (has_next && ph == 0) issue_v(nxt);
         };
         uint32_t st = 0;
         bool odd = false;
