@@ -27,7 +27,6 @@ namespace {
 constexpr uint32_t kUnit8 = 256;      // keys of a unit: one 64-key block a wave
 constexpr uint32_t kItem8Units = 1;   // an item's fixed cost
 constexpr int kRows = 16;
-constexpr int kWaves64 = 2;           // waves a SIMD at head_dim 64 (its blocks are 8 KB)
 
 __device__ inline f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c)
 {
@@ -137,7 +136,7 @@ struct FragV8 {
 };
 
 template <int D, bool PREC, int POL>
-__global__ __launch_bounds__(256, D == 64 ? kWaves64 : D == 128 ? 2 : 1) void paged_decode8_kernel(PagedAttn8Args args)
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(PagedAttn8Args args)
 {
     constexpr int kWaves = 4, D4 = D / 4, NC = D / 64, NB = D / 16, QROW = D + 8;
     // (head_dim 256: one block of V at a time, the next one's loads go out behind its products; two are too many registers)
@@ -526,10 +525,21 @@ __global__ __launch_bounds__(256) void paged_decode8_merge_kernel(PagedAttn8Args
     store_out4(a.out, row * a.out_stride + col, a.out_dtype, v);
 }
 
-// Where no item's K and V take more than this many bytes per kv head, none is
-// cut; on the line, beside longer ones, fewer (see paged_decode.hip).
-constexpr uint32_t kWholeBytes = 256 * 1024;
-constexpr uint32_t kSnapBytes = 160 * 1024;
+// Cutting an item costs two partial results and the merge's launch.  Where no
+// item's K and V take more than this many bytes per kv head, none is cut: whole
+// and cut, us for one sequence: 14 / 2 heads of 64, 2048 keys 10.4 and 11.0, 2560
+// 12.0 and 11.1; 28 / 4 of 128, 1024 keys 11.8 and 13.2, 1280 13.2 and 13.6, 1792
+// 15.9 and 13.2; 16 / 2 of 256, 768 keys 15.9 and 16.6, 1024 18.7 and 18.1.
+constexpr uint32_t whole_bytes(uint32_t D) { return (D == 64 ? 256 : D == 128 ? 320 : 384) * 1024; }
+// Up to this many where there are items for half the GPU, but no more than it
+// holds at once: 64 sequences of 2048 keys, 28 / 4 heads of 128, 24.8 whole, 37.6
+// cut; of 4096, 14 / 2 of 64, 18.3 and 21.4; 128 of 1024, 16 / 2 of 256, 27.1 and
+// 30.8.  (16 sequences of 2048 keys: 18.9 and 20.0, of 4096 of 64 18.0 and 13.1.)
+constexpr uint32_t kWholeMany = 512 * 1024, kManyItems = 128;
+// On the line, beside longer ones, fewer: there the merge comes anyway and items
+// that are not cut make chunks uneven (64 sequences of 1k to 32k keys, 14 / 2
+// heads of 64: 35.4 us, 38.3 with 160 KB; 200 of up to 3000 21.3 and 22.5).
+constexpr uint32_t kSnapBytes = 64 * 1024;
 
 uint32_t units_of_bytes(uint32_t bytes, uint32_t D) { return bytes / (2 * D * kUnit8); }
 
@@ -546,15 +556,26 @@ uint32_t row_blocks(uint32_t max_new, uint32_t n_heads, uint32_t n_kv)
     return (uint32_t)((std::min(rows, (uint64_t)kFewRows) + kRows - 1) / kRows);
 }
 
-// Chunks of a launch: what the GPU holds at once, or all that the bounds can
-// fill; 0: none is cut.
-uint32_t decode8_wgs(uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
+uint32_t decode8_slots(uint32_t D) { return (D <= 128 ? 2u : 1u) * (uint32_t)n_cus(); }
+
+// Chunks of a line: what the GPU holds at once, or all that the bounds can fill;
+// 0: no item is cut whatever their number.
+uint32_t line8_wgs(uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
 {
     const uint32_t units = (max_len + kUnit8 - 1) / kUnit8;
-    if (units <= units_of_bytes(kWholeBytes, D)) return 0;  // no item is cut: a workgroup each
+    if (units <= units_of_bytes(whole_bytes(D), D)) return 0;
     const uint64_t most = (uint64_t)n_seq * row_blocks(max_new, n_heads, n_kv) * n_kv * (units + kItem8Units);
-    const uint64_t full = (uint64_t)(D == 64 ? kWaves64 : D == 128 ? 2 : 1) * (uint64_t)n_cus();
+    const uint64_t full = decode8_slots(D);
     return (uint32_t)(((most < full ? most : full) + 7) / 8 * 8);
+}
+
+// Chunks of a launch; 0: a workgroup for each item.  (The workspace goes by the
+// line all the same: one that serves a call serves smaller ones.)
+uint32_t decode8_wgs(uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D)
+{
+    const uint64_t items = (uint64_t)n_seq * row_blocks(max_new, n_heads, n_kv) * n_kv;
+    if (items >= kManyItems && items <= decode8_slots(D) && (max_len + kUnit8 - 1) / kUnit8 <= units_of_bytes(kWholeMany, D)) return 0;
+    return line8_wgs(n_seq, max_new, max_len, n_heads, n_kv, D);
 }
 
 size_t decode8_bytes(uint32_t wgs, uint32_t D)
@@ -619,7 +640,7 @@ bool all_few(uint32_t n_heads, uint32_t n_kv, uint32_t max_new)
 size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
                              uint32_t n_kv, uint32_t D)
 {
-    const size_t few = align256(decode8_bytes(decode8_wgs(n_seq, max_new, max_len, n_heads, n_kv, D), D));
+    const size_t few = align256(decode8_bytes(line8_wgs(n_seq, max_new, max_len, n_heads, n_kv, D), D));
     return all_few(n_heads, n_kv, max_new) ? few : few + paged_tiles8_workspace(n_tok, n_seq, max_len, n_heads, n_kv, D);
 }
 
