@@ -169,6 +169,8 @@ struct QkNormRopeArgs {
     double turns[128];
 };
 hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st);
+
+// ---- qk_norm_rope8.hip ----
 // into the 8-bit pool (kv8.hpp): kc and vc are its codes
 struct QkNormRope8Args : QkNormRopeArgs {
     uint8_t* ks;            // scales of K and V [n_blocks][n_kv][block]

@@ -33,31 +33,13 @@
 // 32 / 8 heads of 128 6.1.
 #include "common.hpp"
 #include "internal.hpp"
-#include "kv8.hpp"
-
-#include <type_traits>
+#include "qk_norm_rope_parts.hpp"
 
 namespace yhip {
 namespace {
 
 // Up to this many rows the rotation waves write V too, as in rope.hip.
 constexpr uint32_t kScatterRows = 128;
-
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-
-template <uint32_t DT>
-__device__ inline f32x4 load4(const void* p, size_t i)
-{
-    if constexpr (DT == kF32) {
-        return __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i));
-    } else {
-        const u16x4 w = __builtin_nontemporal_load(reinterpret_cast<const u16x4*>(reinterpret_cast<const uint16_t*>(p) + i));
-        f32x4 r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = DT == kBF16 ? bf16_bits_to_f32(w[e]) : f16_bits_to_f32(w[e]);
-        return r;
-    }
-}
 
 // The value whose truncation to f16 is f32_to_f16_ref(x), without branches:
 // half a step of the result is added (to the magnitude's bits where it is
@@ -79,87 +61,6 @@ __device__ inline u16x4 to_cache4(const f32x4& x)
     const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(half_away(x[0]), half_away(x[1]))),
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(half_away(x[2]), half_away(x[3])))};
     return __builtin_bit_cast(u16x4, w);
-}
-
-// (the conversions to bf16 and f16 are gfx950's own, to nearest even)
-__device__ inline void store4(void* p, size_t i, uint32_t dt, const f32x4& x)
-{
-    if (dt == kF32) {
-        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i) = x;
-    } else if (dt == kF16) {
-        f16x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (_Float16)x[e];
-        *reinterpret_cast<f16x4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
-    } else {
-        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        bf16x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = (__bf16)x[e];
-        *reinterpret_cast<bf16x4*>(reinterpret_cast<uint16_t*>(p) + i) = w;
-    }
-}
-
-// sine and cosine of u turns: whole turns and then quarters are taken off in
-// 64 bits, and the Taylor series over an eighth of a turn to either side follow
-// (what they leave out is below 2.5e-8)
-__device__ inline void sincos_turns(double u, float* sn, float* cs)
-{
-    const double q4 = 4.0 * (u - __builtin_rint(u)), whole = __builtin_rint(q4);
-    const float x = 1.5707963267948966f * (float)(q4 - whole), z = x * x;
-    const int q = (int)whole;
-    const float s = x + x * z * (-1.6666667e-1f + z * (8.3333333e-3f + z * (-1.9841270e-4f + z * 2.7557319e-6f)));
-    const float c = 1.0f + z * (-0.5f + z * (4.1666667e-2f + z * (-1.3888889e-3f + z * 2.4801587e-5f)));
-    const float a = q & 1 ? c : s, b = q & 1 ? s : c;
-    *sn = q & 2 ? -a : a;
-    *cs = (q + 1) & 2 ? -b : b;
-}
-
-// the sum over each aligned group of N lanes, by DPP moves: within quads, the
-// other quad of eight (mirrored), the other eight of a row, the other row
-template <int N>
-__device__ inline float group_sum(float x)
-{
-    static_assert(N == 8 || N == 16 || N == 32, "a head is 8, 16 or 32 lanes");
-    x += dpp_mov<0xb1>(x);   // quad_perm [1, 0, 3, 2]
-    x += dpp_mov<0x4e>(x);   // quad_perm [2, 3, 0, 1]
-    x += dpp_mov<0x141>(x);  // row_half_mirror
-    if constexpr (N >= 16) x += dpp_mov<0x140>(x);  // row_mirror
-    if constexpr (N == 32) x = sum_xor16(x);
-    return x;
-}
-
-// the largest of each aligned group of N lanes, by the same moves
-template <int N>
-__device__ inline uint32_t group_max(uint32_t x)
-{
-    auto with = [&](float o) { x = max(x, __builtin_bit_cast(uint32_t, o)); };
-    auto f = [&] { return __builtin_bit_cast(float, x); };
-    with(dpp_mov<0xb1>(f()));
-    with(dpp_mov<0x4e>(f()));
-    with(dpp_mov<0x141>(f()));
-    if constexpr (N >= 16) with(dpp_mov<0x140>(f()));
-    if constexpr (N == 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        x = max((uint32_t)r[0], (uint32_t)r[1]);
-    }
-    return x;
-}
-// k of a row that a group of N lanes holds, eight elements each
-template <int N>
-__device__ inline int group_exponent(const f32x4& y0, const f32x4& y1)
-{
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = max(top, max(finite_mag(y0[e]), finite_mag(y1[e])));
-    return kv8_exponent(group_max<N>(top));
-}
-
-// a row's slot (negative: none)
-__device__ inline int slot_of(const QkNormRopeArgs& a, uint32_t b)
-{
-    const uint32_t s = a.slots ? (uint32_t)a.slots[b] : a.pos_start + b;
-    return s < a.n_slots ? (int)s : -1;
 }
 
 // K row and V column of a slot, as element offsets into the pools
@@ -258,124 +159,9 @@ __device__ void v_block(const QkNormRopeArgs& a, uint32_t vb)
     }
 }
 
-// The 8-bit pool: where a row's scale is, and its V column of codes
-__device__ inline size_t scale_at(const QkNormRopeArgs& a, uint32_t h, uint32_t slot)
+template <uint32_t KIND, int D, uint32_t DT>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a)
 {
-    const uint32_t page = slot / a.block, off = slot - page * a.block;
-    return ((size_t)page * a.n_kv + h) * a.block + off;
-}
-template <int D>
-__device__ inline size_t v8_page_at(const QkNormRopeArgs& a, uint32_t h, uint32_t slot, uint32_t d)
-{
-    const uint32_t page = slot / a.block, off = slot - page * a.block;
-    return (((size_t)page * a.n_kv + h) * a.block + (off & ~63u)) * D + d * kV8Tile + (off & 63u);
-}
-
-// V workgroup of the 8-bit pool: 64 rows of one kv head.  A row's lanes form its
-// scale and codes and leave them in LDS, four codes a word; sixteen rows whose
-// slots are consecutive from a multiple of 16 on leave as one 16-byte store per
-// dimension, by the workgroup of their first row (which therefore reads up to
-// 15 rows more), four dimensions a thread, turned over by byte permutations; rows
-// outside such a group go a byte at a time.
-template <int D, uint32_t DT>
-__device__ void v8_block(const QkNormRope8Args& a, uint32_t vb)
-{
-    constexpr uint32_t LPH = D / 8, RPP = 256 / LPH, W = D / 4 + 1;  // lanes a row, rows a pass, words a row in LDS
-    constexpr uint32_t R = (79 + RPP) / RPP * RPP;                            // rows read: 79 are needed
-    __shared__ uint32_t tile[R * W];
-    __shared__ int slots[15 + 64 + 15];  // of rows r0 - 15 .. r0 + 78
-    __shared__ uint32_t lead[2], lone[2];
-    const uint32_t h = vb % a.n_kv, r0 = vb / a.n_kv * 64u;
-    const uint32_t t = threadIdx.x, i = t % LPH, rr = t / LPH;
-    if (t < 94u) {
-        const int b = (int)(r0 + t) - 15;
-        slots[t] = b >= 0 && (uint32_t)b < a.n_tok ? slot_of(a, (uint32_t)b) : -1;
-    }
-    __syncthreads();
-    constexpr uint32_t U = R / RPP > 5 ? 5 : R / RPP;  // passes whose loads go out together
-    static_assert(R / RPP % U == 0, "whole rounds");
-#pragma unroll 1
-    for (uint32_t p0 = 0; p0 < R / RPP; p0 += U) {
-        f32x4 x[U][2];
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t b = min(r0 + (p0 + u) * RPP + rr, a.n_tok - 1u);
-            const size_t at = (size_t)b * a.v_stride + h * D + 4u * i;
-            x[u][0] = load4<DT>(a.v, at);
-            x[u][1] = load4<DT>(a.v, at + D / 2);
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t r = (p0 + u) * RPP + rr;
-            const int k = group_exponent<LPH>(x[u][0], x[u][1]);
-            const float inv = kv8_inverse(k);
-            tile[r * W + i] = kv8_codes(x[u][0], inv);
-            tile[r * W + LPH + i] = kv8_codes(x[u][1], inv);
-            if (i == 0 && r < 64u) {
-                const int s = slots[15 + r];
-                if (s >= 0) a.vs[scale_at(a, h, (uint32_t)s)] = kv8_scale_byte(k);
-            }
-        }
-    }
-    if (t < 64u) {
-        // leads(j): rows j .. j + 15 of slots[] are one group
-        auto leads = [&](int j) {
-            if (j < 0) return false;
-            const int s = slots[j];
-            bool ok = s >= 0 && (s & 15) == 0;
-#pragma unroll
-            for (int e = 1; e < 16; ++e) ok = ok && slots[j + e] == s + e;
-            return ok;
-        };
-        const int j = 15 + (int)t, s = slots[j];
-        const uint64_t ml = __ballot(leads(j));
-        const uint64_t mn = __ballot(s >= 0 && !leads(j - (s & 15)));
-        if (t == 0) {
-            lead[0] = (uint32_t)ml;
-            lead[1] = (uint32_t)(ml >> 32);
-            lone[0] = (uint32_t)mn;
-            lone[1] = (uint32_t)(mn >> 32);
-        }
-    }
-    __syncthreads();
-    // first rows of groups are at least 16 apart: at most one in each 16 rows
-    for (uint32_t j = t; j < D; j += 256u) {
-        const uint32_t g = j & 3u, c = j >> 2;  // a group, four dimensions
-        const uint32_t m = lead[g >> 1] >> (16u * (g & 1u)) & 0xffffu;
-        if (!m) continue;
-        const uint32_t r = 16u * g + (uint32_t)__builtin_ctz(m);
-        u32x4 w[4];  // [dimension][four rows a word]
-#pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) {
-            const uint32_t* p = &tile[(r + 4u * q) * W + c];
-            const uint32_t a0 = p[0], a1 = p[W], a2 = p[2 * W], a3 = p[3 * W];
-            const uint32_t lo01 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), hi01 = __builtin_amdgcn_perm(a1, a0, 0x07030602u),
-                           lo23 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), hi23 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
-            w[0][q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
-            w[1][q] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
-            w[2][q] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
-            w[3][q] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
-        }
-        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slots[15 + r], 4u * c);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<u32x4*>(dst + e * kV8Tile) = w[e];
-    }
-    uint64_t left = (uint64_t)lone[1] << 32 | lone[0];
-    for (uint32_t n = 0; left; ++n, left &= left - 1) {  // uniform: each wave takes every fourth
-        if (n % 4u != t >> 6) continue;
-        const uint32_t r = (uint32_t)__builtin_ctzll(left);
-        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slots[15 + r], 0);
-        for (uint32_t d = t & 63u; d < D; d += 64u)
-            dst[d * kV8Tile] = reinterpret_cast<const uint8_t*>(&tile[r * W])[d];
-    }
-}
-
-// A = QkNormRope8Args: K and V go as codes and scales into the 8-bit pool; then
-// the V of few rows are passes of their own.
-template <uint32_t KIND, int D, uint32_t DT, class A = QkNormRopeArgs>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
-{
-    constexpr bool KV8 = std::is_same<A, QkNormRope8Args>::value;
     // the two roles alternate over the first 2 * min(rotation, V) workgroups (rope.hip)
     uint32_t blk = blockIdx.x;
     {
@@ -389,8 +175,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
             blk -= m;
         }
         if (v_role) {  // workgroup-uniform
-            if constexpr (KV8) v8_block<D, DT>(a, blk);
-            else v_block<D, DT>(a, blk);
+            v_block<D, DT>(a, blk);
             return;
         }
     }
@@ -417,13 +202,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
 
     // This wave's passes: HPP heads each, those of q (none without q_out), then those of k.  A pass is of one kind,
     // so that everything but the lane's offsets is wave-uniform.
-    const uint32_t pq = a.q_out ? (a.n_heads + HPP - 1) / HPP : 0u, pk = (a.n_kv + HPP - 1) / HPP,
-                   passes = pq + pk + (KV8 && a.n_tok <= kScatterRows ? pk : 0u);
+    const uint32_t pq = a.q_out ? (a.n_heads + HPP - 1) / HPP : 0u, passes = pq + (a.n_kv + HPP - 1) / HPP;
     const uint32_t p_lo = g * a.passes, p_hi = min(passes, p_lo + a.passes);
     const size_t esz = DT == kF32 ? 4 : 2;
     const char* const qrow = reinterpret_cast<const char*>(a.q) + (size_t)b * a.q_stride * esz;
     const char* const krow = reinterpret_cast<const char*>(a.k) + (size_t)b * a.k_stride * esz;
-    const char* const vrow = KV8 ? reinterpret_cast<const char*>(a.v) + (size_t)b * a.v_stride * esz : nullptr;
     const size_t kstep = (size_t)a.block * D;  // between a page's heads
     size_t kpage = 0;
     float c[4], s[4];
@@ -436,9 +219,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t p = min(p0 + u, p_hi - 1u);
-            const bool is_q = p < pq, is_v = KV8 && p >= pq + pk;
-            const uint32_t h = min((is_q ? p : is_v ? p - pq - pk : p - pq) * HPP + sub, (is_q ? a.n_heads : a.n_kv) - 1u);
-            const char* src = is_q ? qrow : is_v ? vrow : krow;
+            const bool is_q = p < pq;
+            const uint32_t h = min((is_q ? p : p - pq) * HPP + sub, (is_q ? a.n_heads : a.n_kv) - 1u);
+            const char* src = is_q ? qrow : krow;
             x[u][0] = load4<DT>(src, h * D + e0);
             x[u][1] = load4<DT>(src, h * D + e1);
         }
@@ -470,26 +253,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t p = p0 + u;
             if (p >= p_hi) break;  // wave-uniform
-            const bool is_q = p < pq, is_v = KV8 && p >= pq + pk;
-            const uint32_t h = (is_q ? p : is_v ? p - pq - pk : p - pq) * HPP + sub;
+            const bool is_q = p < pq;
+            const uint32_t h = (is_q ? p : p - pq) * HPP + sub;
             f32x4 y0 = x[u][0], y1 = x[u][1];
-            if constexpr (KV8) {
-                if (is_v) {
-                    const int k = group_exponent<LPH>(y0, y1);
-                    const float inv = kv8_inverse(k);
-                    const uint32_t w0 = kv8_codes(y0, inv), w1 = kv8_codes(y1, inv);
-                    if (h < a.n_kv) {
-                        uint8_t* dst = reinterpret_cast<uint8_t*>(a.vc) + v8_page_at<D>(a, h, (uint32_t)slot, 0);
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            dst[(e0 + e) * kV8Tile] = (uint8_t)(w0 >> 8 * e);
-                            dst[(e1 + e) * kV8Tile] = (uint8_t)(w1 >> 8 * e);
-                        }
-                        if (i == 0) a.vs[scale_at(a, h, (uint32_t)slot)] = kv8_scale_byte(k);
-                    }
-                    continue;
-                }
-            }
             if (norm) {
                 float ss = 0.0f;
 #pragma unroll
@@ -523,16 +289,6 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
                     store4(a.q_out, at + e0, a.q_out_dtype, y0);
                     store4(a.q_out, at + e1, a.q_out_dtype, y1);
                 }
-            } else if constexpr (KV8) {
-                const int k = group_exponent<LPH>(y0, y1);
-                const float inv = kv8_inverse(k);
-                const uint32_t w0 = kv8_codes(y0, inv), w1 = kv8_codes(y1, inv);
-                if (h < a.n_kv) {
-                    uint8_t* row = reinterpret_cast<uint8_t*>(a.kc) + kpage + h * kstep;
-                    *reinterpret_cast<uint32_t*>(row + e0) = w0;
-                    *reinterpret_cast<uint32_t*>(row + e1) = w1;
-                    if (i == 0) a.ks[scale_at(a, h, (uint32_t)slot)] = kv8_scale_byte(k);
-                }
             } else if (h < a.n_kv) {
                 uint16_t* row = a.kc + kpage + h * kstep;
                 *reinterpret_cast<u16x4*>(row + e0) = to_cache4(y0);
@@ -540,7 +296,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
             }
         }
     }
-    if constexpr (!KV8) if (a.n_tok <= kScatterRows) {
+    if (a.n_tok <= kScatterRows) {
         const uint32_t kv_dim = a.n_kv * D;
         for (uint32_t j = g * 64u + lane; j < kv_dim; j += 64u * a.groups) {
             const size_t at = (size_t)b * a.v_stride + j;
@@ -551,19 +307,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(A a)
     }
 }
 
-template <uint32_t KIND, int D, class A>
-hipError_t launch_dt(const A& a, dim3 grid, hipStream_t st)
+template <uint32_t KIND, int D>
+hipError_t launch_dt(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
 {
     switch (a.dtype) {
-    case kF32: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF32, A>), grid, dim3(256), 0, st, a); break;
-    case kF16: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF16, A>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kBF16, A>), grid, dim3(256), 0, st, a); break;
+    case kF32: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF32>), grid, dim3(256), 0, st, a); break;
+    case kF16: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kF16>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((qk_norm_rope_kernel<KIND, D, kBF16>), grid, dim3(256), 0, st, a); break;
     }
     return hipGetLastError();
 }
 
-template <uint32_t KIND, class A>
-hipError_t launch_kind(const A& a, dim3 grid, hipStream_t st)
+template <uint32_t KIND>
+hipError_t launch_kind(const QkNormRopeArgs& a, dim3 grid, hipStream_t st)
 {
     switch (a.D) {
     case 64: return launch_dt<KIND, 64>(a, grid, st);
@@ -573,19 +329,18 @@ hipError_t launch_kind(const A& a, dim3 grid, hipStream_t st)
     }
 }
 
-template <class A>
-hipError_t launch_any(A& a, hipStream_t st)
+}  // namespace
+
+hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st)
 {
-    constexpr bool KV8 = std::is_same<A, QkNormRope8Args>::value;
-    const uint32_t hpp = 64u / (a.D / 8u), pk = (a.n_kv + hpp - 1) / hpp;
-    const bool few = a.n_tok <= kScatterRows;
-    const uint32_t passes = (a.q_out ? (a.n_heads + hpp - 1) / hpp : 0u) + pk + (KV8 && few ? pk : 0u);
-    const uint32_t per0 = few ? 1u : 3u;
+    const uint32_t hpp = 64u / (a.D / 8u);
+    const uint32_t passes = (a.q_out ? (a.n_heads + hpp - 1) / hpp : 0u) + (a.n_kv + hpp - 1) / hpp;
+    const uint32_t per0 = a.n_tok <= kScatterRows ? 1u : 3u;
     const uint32_t groups = (passes + per0 - 1) / per0;
     a.passes = (passes + groups - 1) / groups;  // per wave, evenly
     a.groups = (passes + a.passes - 1) / a.passes;
     a.rope_blocks = (uint32_t)(((uint64_t)a.n_tok * a.groups + 3u) / 4u);
-    a.v_blocks = few ? 0u : (KV8 ? a.n_kv : a.n_kv * a.D / 64u) * ((a.n_tok + 63u) / 64u);
+    a.v_blocks = a.n_tok > kScatterRows ? a.n_kv * a.D / 64u * ((a.n_tok + 63u) / 64u) : 0u;
     const dim3 grid(a.rope_blocks + a.v_blocks);
     switch (a.kind) {
     case kRopeNone: return launch_kind<kRopeNone>(a, grid, st);
@@ -595,10 +350,5 @@ hipError_t launch_any(A& a, hipStream_t st)
     default: return hipErrorInvalidValue;
     }
 }
-
-}  // namespace
-
-hipError_t launch_qk_norm_rope(QkNormRopeArgs a, hipStream_t st) { return launch_any(a, st); }
-hipError_t launch_qk_norm_rope8(QkNormRope8Args a, hipStream_t st) { return launch_any(a, st); }
 
 }  // namespace yhip
