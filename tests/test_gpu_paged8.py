@@ -127,7 +127,7 @@ def _check_store(T, nh, nkv, d, kind, dtype, out_dtype, norm=True, block=64, n_r
 
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128), (16, 2, 256), (5, 5, 64), (3, 2, 128)])
-@pytest.mark.parametrize("T", [1, 7, 129])
+@pytest.mark.parametrize("T", [1, 7, 129, 401])
 def test_store(cuda, kind, nh, nkv, d, T):
     dt, out = [(F32, F32), (BF16, F16), (F16, BF16)][(T + nh) % 3]
     _check_store(T, nh, nkv, d, kind, dt, out, n_rot=64 if kind == "mrope" else 0)
@@ -136,11 +136,11 @@ def test_store(cuda, kind, nh, nkv, d, T):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("out", [F32, F16, BF16])
 def test_store_types(cuda, dtype, out):
-    _check_store(200, 8, 2, 128, "half", dtype, out, wide=24, spread=12.0)
+    _check_store(500, 8, 2, 128, "half", dtype, out, wide=24, spread=12.0)
     _check_store(30, 8, 2, 128, "pairs", dtype, out, wide=4, norm=False, spread=12.0)
 
 
-@pytest.mark.parametrize("T", [64, 127, 128, 130, 191, 200, 519])
+@pytest.mark.parametrize("T", [64, 127, 128, 130, 191, 200, 383, 384, 385, 386, 400, 447, 463, 519, 700])
 def test_store_row_counts(cuda, T):
     """Both forms of the V store, groups of sixteen that begin and end in any window."""
     _check_store(T, 4, 2, 64, "half", F32, F16, seed=T)
@@ -154,21 +154,23 @@ def test_store_partial_rotation(cuda, n_rot):
 
 
 def test_store_far_positions(cuda):
-    _check_store(140, 4, 2, 128, "pairs", F32, F32, far=131071 * 8)
+    for T in (140, 450):
+        _check_store(T, 4, 2, 128, "pairs", F32, F32, far=131071 * 8)
     _check_store(9, 4, 2, 64, "half", F32, F32, far=(1 << 31) - 100, theta=1e4)
 
 
 def test_store_rows_without_a_slot(cuda):
     big = 0x7fffffff
-    for T in (12, 200):
+    for T in (12, 200, 500):
         _check_store(T, 4, 2, 128, "half", BF16, BF16, skip=[(0, -1), (3, -5), (T - 1, big), (T - 2, -big)])
         _check_store(T, 4, 2, 128, "half", F32, F32, skip=[(i, -1) for i in range(T)])
 
 
 def test_store_in_place_f16_weights_and_keys_only(cuda):
-    _check_store(150, 6, 2, 128, "half", F32, F32, in_place=True, norm_dtype=F16)
+    _check_store(450, 6, 2, 128, "half", F32, F32, in_place=True, norm_dtype=F16)
     _check_store(3, 6, 2, 128, "pairs", BF16, BF16, in_place=True)
     _check_store(150, 6, 2, 128, "half", F16, F16, with_q=False)
+    _check_store(450, 6, 2, 64, "half", F16, F16, with_q=False)
 
 
 def _edges(T, d, dtype, seed):
@@ -191,7 +193,7 @@ def _edges(T, d, dtype, seed):
     return x.to(dtype)
 
 
-@pytest.mark.parametrize("T", [60, 160])
+@pytest.mark.parametrize("T", [60, 460])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_store_of_every_border_is_the_format_byte_for_byte(cuda, T, d, dtype):
@@ -200,9 +202,9 @@ def test_store_of_every_border_is_the_format_byte_for_byte(cuda, T, d, dtype):
 
     k = _edges(T, 2 * d, dtype, d)
     v = k.flip(0).contiguous()
-    p = pool8(3, 2, d, 128)
+    p = pool8(4, 2, d, 128)
     qk_norm_rope_kv8_store(p, None, k, v, 2, ROPE_NONE, 1.0, pos_start=5)
-    K, V, KS, VS = (t[5:5 + T] for t in rows_of_pool(p))
+    K, V, KS, VS = (t[5:5 + T] for t in rows_of_pool(p))  # (without slots: the positions from 5 on, in pages one behind the other)
     for x, c, s in ((k, K, KS), (v, V, VS)):
         code, scale = quantise(x.view(T, 2, d))
         assert torch.equal(s, scale.to(E5M2).view(U8))
@@ -216,19 +218,19 @@ def test_store_of_every_border_is_the_format_byte_for_byte(cuda, T, d, dtype):
 def test_store_gives_the_same_bytes_in_any_chunks(cuda, d):
     from yllm_amd.paged import qk_norm_rope_kv8_store
 
-    T, nkv, g = 300, 2, _gen(8)
+    T, nkv, g = 700, 2, _gen(8)
     k, v = (torch.randn(T, nkv * d, generator=g, device="cuda") for _ in range(2))
     w = 1 + 0.1 * torch.randn(d, generator=g, device="cuda")
     pos = torch.arange(T, dtype=torch.int32, device="cuda")
     pools = []
-    for cuts in ([0, T], [0, 1, 2, 60, 61, 190, 299, T], list(range(0, T, 7)) + [T]):
-        p = pool8(3, nkv, d, 128, fill=0)
+    for cuts in ([0, T], [0, 1, 2, 60, 61, 190, 299, T], [0, 400, T], list(range(0, T, 7)) + [T]):
+        p = pool8(6, nkv, d, 128, fill=0)
         for a, e in zip(cuts, cuts[1:]):
             qk_norm_rope_kv8_store(p, None, k[a:e], v[a:e], nkv, KINDS["half"], 1e6, positions=pos[a:e], slots=pos[a:e],
                                    q_norm=w, k_norm=w)
         pools.append(rows_of_pool(p))
     order = torch.randperm(T, generator=torch.Generator().manual_seed(1)).cuda()
-    p = pool8(3, nkv, d, 128, fill=0)
+    p = pool8(6, nkv, d, 128, fill=0)
     qk_norm_rope_kv8_store(p, None, k[order], v[order], nkv, KINDS["half"], 1e6, positions=pos[order], slots=pos[order],
                            q_norm=w, k_norm=w)
     pools.append(rows_of_pool(p))
@@ -239,12 +241,12 @@ def test_store_gives_the_same_bytes_in_any_chunks(cuda, d):
 def test_store_queries_are_those_of_the_f16_store(cuda):
     from yllm_amd.paged import PagedKV, qk_norm_rope_kv8_store, qk_norm_rope_kv_store
 
-    for T in (3, 140):
+    for T in (3, 140, 400):
         x = torch.randn(T, 12 * 128, generator=_gen(T), device="cuda").to(BF16)
         q, k, v = x[:, :1024], x[:, 1024:1280], x[:, 1280:]
         pos = torch.arange(T, dtype=torch.int32, device="cuda")
-        a = qk_norm_rope_kv_store(PagedKV.empty(4, 2, 128), q, k, v, 8, KINDS["pairs"], 5e5, positions=pos, slots=pos)
-        b = qk_norm_rope_kv8_store(pool8(4, 2, 128, 64), q, k, v, 8, KINDS["pairs"], 5e5, positions=pos, slots=pos)
+        a = qk_norm_rope_kv_store(PagedKV.empty(7, 2, 128), q, k, v, 8, KINDS["pairs"], 5e5, positions=pos, slots=pos)
+        b = qk_norm_rope_kv8_store(pool8(7, 2, 128, 64), q, k, v, 8, KINDS["pairs"], 5e5, positions=pos, slots=pos)
         assert torch.equal(a, b)
 
 
@@ -255,7 +257,7 @@ def test_store_into_a_pool_past_4_gib(cuda):
     nkv, d, block = 8, 128, 256
     nb = (5 << 30) // (nkv * d * block)  # 5 GiB of K
     big = PagedKV8.empty(nb, nkv, d, block, zero=False)
-    for T in (3, 200):
+    for T in (3, 200, 480):
         first = (nb - 2) * block + 17
         for t in (big.k, big.v, big.k_scale, big.v_scale):
             t.view(U8)[-2:] = 3

@@ -546,8 +546,12 @@ uint32_t units_of_bytes(uint32_t bytes, uint32_t D) { return bytes / (2 * D * kU
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Sequences of up to this many rows are walked here, in blocks of 16, the others
-// in tiles of 128 rows.
-constexpr uint32_t kFewRows = 16;
+// in tiles of 128 rows: 32 sequences of 4000 keys, 28 / 4 heads of 128, 3 tokens
+// (21 rows) 46.3 us, in tiles 53.8; 14 / 2 of 64, 4 tokens 19.2 and 31.7; 16 / 2 of
+// 256, 4 tokens 51.5 and 63; 5 tokens of 28 / 4 (35 rows) 75 and 60.  (64 sequences
+// of up to 20000 keys, 3 tokens of 28 / 4: 106 and 98: the second block reads K and
+// V again.)
+constexpr uint32_t kFewRows = 32;
 
 // row blocks of a sequence at most
 uint32_t row_blocks(uint32_t max_new, uint32_t n_heads, uint32_t n_kv)
@@ -607,7 +611,7 @@ hipError_t launch_decode8(const PagedAttn8Args& in, hipStream_t st)
     a.part_o = reinterpret_cast<float*>(p + align256((size_t)2 * a.n_wg * kRows * 2 * sizeof(float)));
     const uint32_t nb = row_blocks(a.max_new, a.n_heads, a.n_kv);
     const uint32_t grid = a.n_wg ? a.n_wg : a.n_seq * a.n_kv * nb;
-    // non-temporal loads where the batch reads more than the caches keep (an upper bound)
+    // non-temporal loads where the batch reads more than the caches keep (an upper bound), and once
     const bool stream = nb == 1 && (uint64_t)a.n_seq * a.n_kv * a.max_len * a.D * 2u >= (32ull << 20);
     const bool prec = a.q_dtype == kF32;
     switch (a.D) {
