@@ -371,6 +371,20 @@ int yhip_kv8_to_pages(uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks, const
                       const int32_t* dst, const int32_t* src, uint32_t n_pages, uint32_t block, uint32_t n_kv_heads,
                       uint32_t head_dim, void* stream);
 
+/* A paged entry point by its number, with its arguments in order as 64-bit
+ * words: pointers and integers as they are, a float as the bits of a double.
+ * For callers whose foreign-function layer pays by the argument: the same
+ * checks, results and codes; a word that does not fit its argument, or a wrong
+ * count, is YHIP_EINVAL. */
+#define YHIP_CALL_PAGED_PLAN 0u
+#define YHIP_CALL_QK_NORM_ROPE_KV_STORE 1u
+#define YHIP_CALL_PAGED_ATTN 2u
+#define YHIP_CALL_QK_NORM_ROPE_KV8_STORE 3u
+#define YHIP_CALL_PAGED_ATTN8 4u
+#define YHIP_CALL_KV8_FROM_PAGES 5u
+#define YHIP_CALL_KV8_TO_PAGES 6u
+int yhip_call(uint32_t call, const uint64_t* words, uint32_t n_words);
+
 /* ---- o_proj (the step after attention) -------------------------------------
  * x[b] += W_o . att[b] for B tokens: matmul(att_out, x2, SLOT_O) then the
  * residual add (engine.c:969-973; qwen35 after its gate, 958-973), with

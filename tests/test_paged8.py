@@ -209,3 +209,75 @@ def test_python_refusals():
     for f in bad:
         with pytest.raises(YhipError):
             f()
+
+
+# ---- yhip_call: the same entry points by number, their arguments as words ------------------------------
+
+def _calls():
+    from test_paged import plan_args
+
+    from yllm_amd._lib import CALLS
+
+    args = (plan_args, store16, attn16, store_args, attn_args, from_args, to_args)
+    return dict(zip(CALLS, args))
+
+
+def test_call_numbers_are_those_of_the_header():
+    import re
+    from pathlib import Path
+
+    from yllm_amd._lib import CALLS
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "yllm_hip.h").read_text()
+    numbers = {n.lower(): int(v) for n, v in re.findall(r"#define YHIP_CALL_(\w+) (\d+)u", text)}
+    assert numbers == {n[5:]: i for i, n in enumerate(CALLS)}
+
+
+@pytest.mark.parametrize("name", ["yhip_paged_plan", "yhip_qk_norm_rope_kv_store", "yhip_paged_attn", "yhip_qk_norm_rope_kv8_store",
+                                  "yhip_paged_attn8", "yhip_kv8_from_pages", "yhip_kv8_to_pages"])
+def test_calls_by_number_answer_as_the_entry_points_do(hiplib, name):
+    """Every argument in turn as 0, as 1 and as a large value: calls that are refused are refused with the same words (those
+    that would launch are left out: there is nothing at these addresses)."""
+    from yllm_amd import YhipError
+    from yllm_amd._lib import SIGNATURES, fast
+
+    base = [getattr(a, "value", a) for a in _calls()[name]()]
+    direct, types = getattr(hiplib, name), SIGNATURES[name][1]
+    floats = {i for i, t in enumerate(types) if t.__name__ == "c_float"}
+    assert len(base) == len(types)
+    # (a base that is refused last of all: its written tensors overlap)
+    same = {"yhip_paged_plan": (11, 12), "yhip_qk_norm_rope_kv_store": (15, 14), "yhip_paged_attn": (0, 6),
+            "yhip_qk_norm_rope_kv8_store": (15, 14), "yhip_paged_attn8": (0, 6), "yhip_kv8_from_pages": (1, 0), "yhip_kv8_to_pages": (1, 0)}[name]
+    base[same[0]] = base[same[1]]
+    assert direct(*base) == -22
+    said = 0
+    for i in range(len(base) - 1):
+        if i in same:
+            continue                                              # (without the overlap it would launch)
+        for v in (0, 1, 0x7ffffff0, base[i]):
+            a = list(base)
+            a[i] = float(v) if i in floats and v is not None else v
+            rc = direct(*a)
+            if rc == 0:
+                continue
+            msg = _err(hiplib)
+            assert fast(name)(*a) == rc and _err(hiplib) == msg, (i, v)
+            said += 1
+    assert said > len(base)
+    with pytest.raises(YhipError):
+        fast(name)(*base[:-1])                                    # too few
+    i = next(k for k, t in enumerate(types) if t.__name__ in ("c_uint", "c_uint32"))
+    a = list(base)
+    a[i] = (1 << 32) + 1
+    assert fast(name)(*a) == -22 and "does not fit" in _err(hiplib)
+    for bad in (-1, 1 << 64, "x"):
+        a[i] = bad
+        with pytest.raises(YhipError):
+            fast(name)(*a)
+
+
+def test_calls_that_are_none(hiplib):
+    words = bytes(8 * 40)
+    assert hiplib.yhip_call(7, words, 16) == -22 and "no call" in _err(hiplib)
+    assert hiplib.yhip_call(0, words, 15) == -22 and "words" in _err(hiplib)
+    assert hiplib.yhip_call(0, None, 16) == -22 and "words" in _err(hiplib)

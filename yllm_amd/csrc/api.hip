@@ -9,6 +9,10 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <tuple>
+#include <type_traits>
+#include <utility>
+
 namespace {
 
 thread_local char g_err[512];
@@ -1150,3 +1154,52 @@ int yhip_kv8_to_pages(uint16_t* kpool, uint16_t* vpool, uint32_t n_blocks, const
 }
 
 }  // extern "C"
+
+namespace {
+
+// one word as an argument of type T; `fits` becomes false where it does not
+template <class T>
+T word_as(uint64_t w, bool& fits)
+{
+    if constexpr (std::is_pointer<T>::value) {
+        return reinterpret_cast<T>((uintptr_t)w);
+    } else if constexpr (std::is_same<T, float>::value) {
+        double d;
+        memcpy(&d, &w, sizeof(d));
+        return (float)d;
+    } else {
+        fits = fits && (uint64_t)(T)w == w;
+        return (T)w;
+    }
+}
+
+template <class... P, size_t... I>
+int call_words(int (*f)(P...), const uint64_t* w, uint32_t n, std::index_sequence<I...>)
+{
+    if (n != sizeof...(P) || !w) return fail(YHIP_EINVAL, "yhip_call: %zu words are needed, %u given", sizeof...(P), n);
+    bool fits = true;
+    const std::tuple<P...> args{word_as<P>(w[I], fits)...};
+    if (!fits) return fail(YHIP_EINVAL, "yhip_call: a word does not fit its argument");
+    return f(std::get<I>(args)...);
+}
+template <class... P>
+int call_words(int (*f)(P...), const uint64_t* w, uint32_t n)
+{
+    return call_words(f, w, n, std::index_sequence_for<P...>{});
+}
+
+}  // namespace
+
+extern "C" int yhip_call(uint32_t call, const uint64_t* words, uint32_t n_words)
+{
+    switch (call) {
+    case YHIP_CALL_PAGED_PLAN: return call_words(yhip_paged_plan, words, n_words);
+    case YHIP_CALL_QK_NORM_ROPE_KV_STORE: return call_words(yhip_qk_norm_rope_kv_store, words, n_words);
+    case YHIP_CALL_PAGED_ATTN: return call_words(yhip_paged_attn, words, n_words);
+    case YHIP_CALL_QK_NORM_ROPE_KV8_STORE: return call_words(yhip_qk_norm_rope_kv8_store, words, n_words);
+    case YHIP_CALL_PAGED_ATTN8: return call_words(yhip_paged_attn8, words, n_words);
+    case YHIP_CALL_KV8_FROM_PAGES: return call_words(yhip_kv8_from_pages, words, n_words);
+    case YHIP_CALL_KV8_TO_PAGES: return call_words(yhip_kv8_to_pages, words, n_words);
+    default: return fail(YHIP_EINVAL, "yhip_call: no call %u", call);
+    }
+}

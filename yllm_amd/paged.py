@@ -25,7 +25,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import ENOSPC, F32, OK, YhipError, check, elsewhere, lib
+from ._lib import ENOSPC, F32, OK, YhipError, check, elsewhere, fast, lib
 from ._lib import current_stream as _stream
 from .attention import _DT, ROPE_MROPE, ROPE_NONE, LayerKV, _dtype_code, _with_workspace
 
@@ -205,7 +205,7 @@ def paged_plan(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torc
     args = (block_table.data_ptr(), w, stride, ctx_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), n_list,
             n_free.data_ptr(), n, n_tok, block, cu.data_ptr(), lens.data_ptr(), slots.data_ptr(), pos.data_ptr(),
             counts.data_ptr())
-    _launch(lib().yhip_paged_plan, args, there)
+    _launch(fast("yhip_paged_plan"), args, there)
     if out is None:
         return PagedStep(block_table, cu, lens, slots, pos, counts)
     out.block_table = block_table
@@ -246,8 +246,8 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
     rotated q (q_out, allocated in q_out_dtype or q's type if not given; q_out may be q itself), or None when q is
     None.  Rows without a slot (negative) are skipped."""
     kc, vc = cache.k, cache.v
-    return _store("qk_norm_rope_kv_store", lib().yhip_qk_norm_rope_kv_store, _pool(cache, "qk_norm_rope_kv_store"), (kc, vc),
-                  q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out, q_out_dtype)
+    return _store("qk_norm_rope_kv_store", fast("yhip_qk_norm_rope_kv_store"), _pool(cache, "qk_norm_rope_kv_store"), (kc, vc),
+                  (kc.data_ptr(), vc.data_ptr()), q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out, q_out_dtype)
 
 
 def qk_norm_rope_kv8_store(cache: PagedKV8, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -260,12 +260,14 @@ def qk_norm_rope_kv8_store(cache: PagedKV8, q: torch.Tensor | None, k: torch.Ten
     """qk_norm_rope_kv_store into a pool held in 8 bits: each row of k (after its norm and rotation) and v gets a scale
     2^k, the smallest (k in -14..7) whose 448 reaches its largest magnitude, and e4m3 codes to nearest even.  Magnitudes
     past 57344 are held as that, inf and NaN as NaN.  A row's bytes depend on that row alone."""
-    return _store("qk_norm_rope_kv8_store", lib().yhip_qk_norm_rope_kv8_store, _pool8(cache, "qk_norm_rope_kv8_store"),
-                  (cache.k, cache.v, cache.k_scale, cache.v_scale), q, k, v, n_heads, rope, theta, n_rot, positions, slots,
+    shape = _pool8(cache, "qk_norm_rope_kv8_store")
+    kc, vc, sk, sv = cache.k, cache.v, cache.k_scale, cache.v_scale
+    return _store("qk_norm_rope_kv8_store", fast("yhip_qk_norm_rope_kv8_store"), shape, (kc, vc, sk, sv),
+                  (kc.data_ptr(), vc.data_ptr(), sk.data_ptr(), sv.data_ptr()), q, k, v, n_heads, rope, theta, n_rot, positions, slots,
                   pos_start, q_norm, k_norm, eps, q_out, q_out_dtype)
 
 
-def _store(fn, f, shape, pools, q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out,
+def _store(fn, f, shape, pools, at, q, k, v, n_heads, rope, theta, n_rot, positions, slots, pos_start, q_norm, k_norm, eps, q_out,
            q_out_dtype):
     n_blocks, n_kv, block, d = shape
     dt = k.dtype
@@ -284,7 +286,7 @@ def _store(fn, f, shape, pools, q, k, v, n_heads, rope, theta, n_rot, positions,
         qp, qop = q.data_ptr(), q_out.data_ptr()
     else:
         q_out = None
-    pp = sp = wq = wk = None
+    pp = sp = wq = wk = 0
     if positions is not None:
         _ints(fn, "positions", positions, T)
         pp = positions.data_ptr()
@@ -302,7 +304,7 @@ def _store(fn, f, shape, pools, q, k, v, n_heads, rope, theta, n_rot, positions,
         norm = _DT[q_norm.dtype]
         wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
     args = (qop, qdt, qos, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DT[dt], wq, wk, norm, eps,
-            *[p.data_ptr() for p in pools], n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
+            *at, n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
             n_rot if rope == ROPE_MROPE else 0, theta if rope != ROPE_NONE else 1.0)
     _launch(f, args, elsewhere(fn, k.get_device(), *pools, q, v, q_out, positions, slots, q_norm, k_norm))
     return q_out
@@ -331,8 +333,9 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, kv_le
     fn = "paged_attn"
     if not isinstance(cache, PagedKV):
         raise YhipError(-22, f"{fn}: the cache must be a PagedKV")
-    return _attn(fn, lib().yhip_paged_attn, paged_attn_workspace_bytes, _pool(cache, fn), (cache.k, cache.v), q, block_table,
-                 kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype, workspace)
+    kc, vc = cache.k, cache.v
+    return _attn(fn, fast("yhip_paged_attn"), paged_attn_workspace_bytes, _pool(cache, fn), (kc, vc),
+                 (kc.data_ptr(), vc.data_ptr()), q, block_table, kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype, workspace)
 
 
 def paged_attn8_workspace_bytes(n_tok: int, n_seq: int, max_new: int, max_len: int, n_heads: int, n_kv: int,
@@ -354,12 +357,14 @@ def paged_attn8(q: torch.Tensor, cache: PagedKV8, block_table: torch.Tensor, kv_
     """paged_attn over a pool held in 8 bits, with the values that it holds as keys and values (workspaces by
     paged_attn8_workspace)."""
     fn = "paged_attn8"
-    return _attn(fn, lib().yhip_paged_attn8, paged_attn8_workspace_bytes, _pool8(cache, fn),
-                 (cache.k, cache.v, cache.k_scale, cache.v_scale), q, block_table, kv_lens, cu_new, n_heads, max_new, max_len,
+    shape = _pool8(cache, fn)
+    kc, vc, sk, sv = cache.k, cache.v, cache.k_scale, cache.v_scale
+    return _attn(fn, fast("yhip_paged_attn8"), paged_attn8_workspace_bytes, shape, (kc, vc, sk, sv),
+                 (kc.data_ptr(), vc.data_ptr(), sk.data_ptr(), sv.data_ptr()), q, block_table, kv_lens, cu_new, n_heads, max_new, max_len,
                  gate, out, out_dtype, workspace)
 
 
-def _attn(fn, f, space, shape, pools, q, block_table, kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype,
+def _attn(fn, f, space, shape, pools, at, q, block_table, kv_lens, cu_new, n_heads, max_new, max_len, gate, out, out_dtype,
           workspace):
     n_blocks, n_kv, block, d = shape
     n, w, stride = _table(fn, block_table)
@@ -375,7 +380,7 @@ def _attn(fn, f, space, shape, pools, q, block_table, kv_lens, cu_new, n_heads, 
     if out is None:
         out = torch.empty((T, width), dtype=out_dtype or q.dtype, device=q.device)
     os_ = _rows(fn, "out", out, T, width)
-    gp, gs = None, 0
+    gp = gs = 0
     if gate is not None:
         gs = _rows(fn, "gate", gate, T, width)
         gp = gate.data_ptr()
@@ -383,7 +388,7 @@ def _attn(fn, f, space, shape, pools, q, block_table, kv_lens, cu_new, n_heads, 
             raise YhipError(-22, f"{fn}: gate must be fp32")
     dev = q.get_device()
     there = elsewhere(fn, dev, *pools, block_table, kv_lens, cu_new, out, gate)
-    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, *[p.data_ptr() for p in pools],
+    args = (out.data_ptr(), _dtype_code(out), os_, q.data_ptr(), _dtype_code(q), qs, *at,
             n_blocks, block, block_table.data_ptr(), w, stride, kv_lens.data_ptr(), cu_new.data_ptr(), n, T, max_new,
             max_len, n_heads, n_kv, d, gp, gs)
     if there is None and workspace is not None and workspace.get_device() == dev:
@@ -424,6 +429,6 @@ def _pages(fn: str, kv8: PagedKV8, kv: PagedKV, dst: torch.Tensor, src: torch.Te
     _ints(fn, "src", src, n)
     eight = (kv8.k.data_ptr(), kv8.v.data_ptr(), kv8.k_scale.data_ptr(), kv8.v_scale.data_ptr(), n8)
     half = (kv.k.data_ptr(), kv.v.data_ptr(), n16)
-    f = lib().yhip_kv8_to_pages if to else lib().yhip_kv8_from_pages
+    f = fast("yhip_kv8_to_pages" if to else "yhip_kv8_from_pages")
     args = (*(half + eight if to else eight + half), dst.data_ptr(), src.data_ptr(), n, block, n_kv, d)
     _launch(f, args, elsewhere(fn, dst.get_device(), src, kv8.k, kv8.v, kv8.k_scale, kv8.v_scale, kv.k, kv.v))
