@@ -634,6 +634,37 @@ def test_attn_captured_chunks_replay_with_new_lengths(cuda):
         b.check()
 
 
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128), (32, 8, 128), (16, 2, 256)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("few,chunks", [(40, 0), (0, 5), (1, 9), (90, 1), (64, 1), (200, 6), (7, 2)])
+def test_attn_few_rows_beside_chunks(cuda, nh, nkv, d, dtype, few, chunks):
+    """One launch for both kinds of sequences, from all of one to all of the other, under bounds that let every one be a
+    chunk; a workspace with anything in it; a gate; empty sequences between."""
+    from yllm_amd.paged import paged_attn8_workspace
+
+    seqs = [(1 + 37 * i * i % 2900, 1 + i % 2) for i in range(few)]
+    seqs = [(max(L, n), n) for L, n in seqs]
+    for i in range(chunks):
+        seqs.insert(i * len(seqs) // chunks, (300 + 411 * i, (300, 40, 129)[i % 3]))
+    seqs.insert(len(seqs) // 2, (0, 0))
+    seqs.insert(0, (50, 0))
+    b = Batch8(seqs, nh, nkv, d, dtype=dtype, seed=few + chunks, gated=few % 2 == 1, behind=2, spread=4.0)
+    bound = min(512, b.T)
+    ws = paged_attn8_workspace(b.T, len(seqs), bound, b.max_len, nh, nkv, d)
+    out = b.check(max_new=bound, workspace=ws)
+    for fill in (0, 0xff, 0x01):
+        ws.fill_(fill)
+        assert torch.equal(b.run(max_new=bound, workspace=ws), out)
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(14, 2, 64), (28, 4, 128)])
+def test_attn_long_contexts_beside_chunks(cuda, nh, nkv, d):
+    """Pieces of both lines joined; twice the same bits."""
+    for seqs in ([(60000, 1), (40000, 300), (9, 3)], [(9000, 200)] + [(30000 + 77 * i, 2) for i in range(9)]):
+        b = Batch8(seqs, nh, nkv, d, dtype=BF16, seed=51)
+        assert torch.equal(b.check(), b.run())
+
+
 @pytest.mark.parametrize("nh,nkv,d", [(3, 2, 64), (28, 4, 128), (5, 3, 128), (16, 2, 256)])
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("L,new", [(0, 0), (50, 10), (300, 1), (130, 130), (129, 129), (700, 127), (640, 200), (90, 150)])

@@ -27,6 +27,7 @@ namespace yhip {
 namespace {
 
 constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
+constexpr uint32_t kFewMergeWgs = 4;
 
 // Workgroup (j, y): the y-th 256 / (D / 4) rows of the split item that chunk j
 // begins, if any.  Pieces are joined in their order; a thread holds four
@@ -36,15 +37,14 @@ constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
 // dependent round trips: 2048 tokens of 16 / 2 heads of 256 with a gate merged
 // in 22 us; so, in 19, 6 TB/s).
 template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
+__device__ __forceinline__ void paged_merge(const PagedAttnArgs& a, uint32_t j, uint32_t y)
 {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     constexpr uint32_t C4 = D / 4, RP = 256 / C4, kRound = 8;
-    const uint32_t j = blockIdx.x;
     const PagedDesc d = reinterpret_cast<const PagedDesc*>(a.desc)[j];
     if (d.n == 0) return;
-    const uint32_t dim = threadIdx.x % C4 * 4u, r0 = blockIdx.y * RP + threadIdx.x / C4;
-    if (d.n == 2 && blockIdx.y % kMergeRows != 0) return;
+    const uint32_t dim = threadIdx.x % C4 * 4u, r0 = y * RP + threadIdx.x / C4;
+    if (d.n == 2 && y % kMergeRows != 0) return;
     auto finish = [&](const PagedRow& rw, f32x4 O, float L, const f32x4& g) {
         f32x4 v = O * (L == 0.0f ? 0.0f : 1.0f / L);
         if (a.gate) {
@@ -120,6 +120,28 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
     }
 }
 
+template <int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
+{
+    paged_merge<D>(a, blockIdx.x, blockIdx.y);
+}
+
+// Both lines' (PagedMixed8Args): `tile_wgs` workgroups for the tiles', then four for each of the other's chunks
+template <int D>
+__global__ __launch_bounds__(256) void paged_mixed8_merge_kernel(PagedMixed8Args a, uint32_t tile_wgs)
+{
+    if (blockIdx.x < tile_wgs) {
+        paged_merge<D>(a, blockIdx.x % a.n_wg, blockIdx.x / a.n_wg);
+        return;
+    }
+    const uint32_t w = blockIdx.x - tile_wgs, j = w % a.part.n_wg;
+    if (reinterpret_cast<const PagedDesc*>(a.part.desc)[j].n == 0) return;
+    for (uint32_t r = w / a.part.n_wg; r < kRows; r += kFewMergeWgs) {
+        decode8_merge<D>(a.part, j, r);
+        __syncthreads();
+    }
+}
+
 }  // namespace
 
 namespace {
@@ -191,14 +213,19 @@ void launch_tiles(const A& a, uint32_t grid, hipStream_t st)
     hipLaunchKernelGGL((prefill_kernel<D, NG, false, QS, A>), dim3(grid), dim3(threads), 0, st, a);
 }
 
-template <class A>
-hipError_t launch_items(const A& in, hipStream_t st)
+// an item may be split (with more new tokens than keys its units go by its tokens, paged_items.hpp)
+bool may_split(const PagedAttnArgs& a) { return std::max(a.max_len, a.max_new) > a.snap_units * kUnitKeys; }
+uint32_t merge_wgs(const PagedAttnArgs& a)  // for a chunk
 {
-    A a = in;
-    const bool qs = a.q_dtype == kF32;
+    const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
+    return (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp;
+}
+
+// what the launcher sets
+void set_line(PagedAttnArgs& a, uint32_t per_cu)
+{
     a.gmax = (a.n_heads + a.n_kv - 1) / a.n_kv;
     a.min_units = min_units(a.max_len);
-    const uint32_t per_cu = a.D <= 128 && !qs ? 2 : 1;
     a.n_wg = paged_wgs(a.n_tok, a.n_seq, a.max_len, a.n_heads, a.n_kv, per_cu, a.min_units);
     a.snap_units = kSnapUnits;
     char* p = reinterpret_cast<char*>(a.ws);
@@ -206,6 +233,15 @@ hipError_t launch_items(const A& in, hipStream_t st)
     p += align256a((size_t)a.n_wg * sizeof(PagedDesc));
     a.part_ml = reinterpret_cast<float*>(p);
     a.part_o = reinterpret_cast<float*>(p + align256a((size_t)2 * a.n_wg * kItemRows * 2 * sizeof(float)));
+}
+
+template <class A>
+hipError_t launch_items(const A& in, hipStream_t st)
+{
+    A a = in;
+    const bool qs = a.q_dtype == kF32;
+    const uint32_t per_cu = a.D <= 128 && !qs ? 2 : 1;
+    set_line(a, per_cu);
     const uint32_t whole = paged_whole_wgs(a, per_cu, qs), grid = whole ? whole : a.n_wg;
     if (whole) a.n_wg = 0;
     switch (a.D) {
@@ -217,11 +253,8 @@ hipError_t launch_items(const A& in, hipStream_t st)
         break;
     default: return hipErrorInvalidValue;
     }
-    // an item may be split (with more new tokens than keys its units go by its tokens, paged_items.hpp)
-    const uint32_t longest = std::max(a.max_len, a.max_new);
-    if (!whole && longest > a.snap_units * kUnitKeys) {
-        const uint32_t rp = 1024u / a.D;  // rows of a merge workgroup
-        const dim3 merge(a.n_wg, (std::min(a.gmax * a.max_new, kItemRows) + rp - 1) / rp);
+    if (!whole && may_split(a)) {
+        const dim3 merge(a.n_wg, merge_wgs(a));
         switch (a.D) {
         case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, merge, dim3(256), 0, st, static_cast<const PagedAttnArgs&>(a)); break;
         case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, merge, dim3(256), 0, st, static_cast<const PagedAttnArgs&>(a)); break;
@@ -252,5 +285,21 @@ size_t paged_tiles8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, 
     return paged_bytes(paged_wgs(n_tok, n_seq, max_len, n_heads, n_kv, D <= 128 ? 2 : 1, kMinUnits), D);
 }
 hipError_t launch_paged_tiles8(const PagedAttn8Args& a, hipStream_t st) { return launch_items(a, st); }
+
+// (16-bit queries, head_dim 64 or 128: both kinds' workgroups are of 256 threads, two to a CU)
+hipError_t launch_paged_mixed8(const PagedAttn8Args& tiles, const PagedAttn8Args& few, hipStream_t st)
+{
+    PagedMixed8Args a;
+    static_cast<PagedAttn8Args&>(a) = tiles;
+    static_cast<PagedAttn8Args&>(a.part) = few;
+    set_line(a, 2);
+    const uint32_t grid = std::min(a.n_wg + a.part.n_wg, round8(2u * (uint32_t)n_cus()));
+    if (a.D == 64) hipLaunchKernelGGL((prefill_kernel<64, 1, false, false, PagedMixed8Args>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prefill_kernel<128, 1, false, false, PagedMixed8Args>), dim3(grid), dim3(256), 0, st, a);
+    const uint32_t tile_wgs = may_split(a) ? a.n_wg * merge_wgs(a) : 0, merge = tile_wgs + kFewMergeWgs * a.part.n_wg;
+    if (a.D == 64) hipLaunchKernelGGL(paged_mixed8_merge_kernel<64>, dim3(merge), dim3(256), 0, st, a, tile_wgs);
+    else hipLaunchKernelGGL(paged_mixed8_merge_kernel<128>, dim3(merge), dim3(256), 0, st, a, tile_wgs);
+    return hipGetLastError();
+}
 
 }  // namespace yhip

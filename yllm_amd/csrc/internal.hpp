@@ -236,12 +236,18 @@ struct PagedAttn8Args : PagedAttnArgs {
     // kernel's, the others the tiles'
     uint32_t few;
 };
+// Both at once: the tiles' launch, with the decode kernel's line beside it
+struct PagedFew8Args : PagedAttn8Args {};
+struct PagedMixed8Args : PagedAttn8Args {
+    PagedFew8Args part;
+};
 size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, uint32_t max_len, uint32_t n_heads,
                              uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_attn8(const PagedAttn8Args& a, hipStream_t st);
 // the part of the sequences that are not few
 size_t paged_tiles8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_len, uint32_t n_heads, uint32_t n_kv, uint32_t D);
 hipError_t launch_paged_tiles8(const PagedAttn8Args& a, hipStream_t st);
+hipError_t launch_paged_mixed8(const PagedAttn8Args& tiles, const PagedAttn8Args& few, hipStream_t st);
 
 // ---- o_proj.hip ----
 struct OProjArgs {

@@ -138,12 +138,13 @@ __device__ inline const PagedAttnArgs& fresh_args(const PagedAttnArgs&)
 // none.  Active chunks are spread over the XCDs (consecutive workgroups go to
 // the 8 XCDs in turn), neighbours on one XCD, whose L2 then holds the keys they
 // share.
-__device__ inline bool paged_chunk(const PagedAttnArgs& a, PagedCursor& C, uint64_t total, uint64_t& begin)
+__device__ inline bool paged_chunk(const PagedAttnArgs& a, PagedCursor& C, uint64_t total, uint64_t& begin, uint32_t wg,
+                                   uint32_t n_wg)
 {
-    const PagedChunks cut = paged_chunks(total, a.n_wg, a.min_units);
+    const PagedChunks cut = paged_chunks(total, n_wg, a.min_units);
     C.chunk = cut.units;
-    const uint32_t active = min(cut.n, a.n_wg);  // (more only if offsets that overlap pass the bounds checked on the host)
-    const uint32_t x = blockIdx.x % 8u, y = blockIdx.x / 8u, share = (active + 7u) / 8u;
+    const uint32_t active = min(cut.n, n_wg);  // (more only if offsets that overlap pass the bounds checked on the host)
+    const uint32_t x = wg % 8u, y = wg / 8u, share = (active + 7u) / 8u;
     C.j = y < share ? x * share + y : 8u * share + (y - share) * 8u + x;
     begin = (uint64_t)C.j * C.chunk;
     C.done = 0;
@@ -152,15 +153,15 @@ __device__ inline bool paged_chunk(const PagedAttnArgs& a, PagedCursor& C, uint6
     return C.j < active;
 }
 
-// This workgroup's place in the line; false if it has no chunk.  `scratch`: 24
-// words of LDS, free again after the call's last barrier.
+// The place in the line of workgroup `wg` of `n_wg`; false if it has no chunk.
+// `scratch`: 24 words of LDS, free again after the call's last barrier.
 template <int NT, class Line = PagedLine>
-__device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C)
+__device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C, uint32_t wg, uint32_t n_wg)
 {
     if (a.n_seq == 1) {  // nothing to scan
         C.seq = 0;
         uint64_t begin;
-        const bool any = paged_chunk(a, C, Line::units(a, cursor_seq(a, 0)), begin);
+        const bool any = paged_chunk(a, C, Line::units(a, cursor_seq(a, 0)), begin, wg, n_wg);
         C.off = (uint32_t)begin;
         return any;
     }
@@ -189,7 +190,7 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
         total = uni64(total);
     }
     uint64_t begin;
-    if (!paged_chunk(a, C, total, begin)) return false;  // workgroup-uniform
+    if (!paged_chunk(a, C, total, begin, wg, n_wg)) return false;  // workgroup-uniform
     const bool mine = before <= begin && begin < before + sum;
     if (small) {
         const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(mine));
@@ -212,6 +213,12 @@ __device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, Pa
         __syncthreads();
     }
     return true;
+}
+
+template <int NT, class Line = PagedLine>
+__device__ inline bool paged_start(const PagedAttnArgs& a, uint64_t* scratch, PagedCursor& C)
+{
+    return paged_start<NT, Line>(a, scratch, C, blockIdx.x, a.n_wg);
 }
 
 // An item of T units, the cursor at its unit t: moves the cursor past the

@@ -19,6 +19,20 @@ __device__ inline const PagedAttn8Args& fresh_args(const PagedAttn8Args&)
     return *(const PagedAttn8Args*)p;
 }
 
+__device__ inline const PagedMixed8Args& fresh_args(const PagedMixed8Args&)
+{
+    auto p = (const PagedMixed8Args __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedMixed8Args*)p;
+}
+static_assert(sizeof(PagedMixed8Args) == sizeof(PagedAttn8Args) + sizeof(PagedFew8Args), "the second part follows the first");
+__device__ inline const PagedFew8Args& fresh_args(const PagedFew8Args&)
+{
+    auto p = (const char __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr() + sizeof(PagedAttn8Args);
+    asm volatile("" : "+s"(p));
+    return *(const PagedFew8Args*)p;
+}
+
 // A sequence's units among the tiles' items: those with few tokens are the
 // decode kernel's (its line has the others' complement).
 __device__ inline bool few_rows(const PagedAttn8Args& a, const PagedSeq& s) { return a.gmax * s.nq <= a.few; }

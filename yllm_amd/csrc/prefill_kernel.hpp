@@ -33,6 +33,7 @@
 #include "common.hpp"
 #include "internal.hpp"
 #include "paged_items.hpp"
+#include "paged_decode8.hpp"
 #include "paged_items8.hpp"
 
 #include <math.h>
@@ -478,7 +479,9 @@ __device__ inline bool split_item(const PrefillArgs& a, PItem& I)
 template <int D, int NG, bool SPLIT, bool QS = false, class A = PrefillArgs>
 __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 && !QS) ? 2 : 1) void prefill_kernel(A args)
 {
-    constexpr bool PAGED = std::is_base_of<PagedAttnArgs, A>::value, KV8 = std::is_same<A, PagedAttn8Args>::value;
+    constexpr bool PAGED = std::is_base_of<PagedAttnArgs, A>::value, KV8 = std::is_base_of<PagedAttn8Args, A>::value;
+    // (sequences with few rows as well, by workgroups of their own)
+    constexpr bool MIXED = std::is_same<A, PagedMixed8Args>::value;
     constexpr bool PS = PAGED && QS;
     using Item = typename std::conditional<PAGED, PagedItem, PItem>::type;
     using Pos = typename std::conditional<PAGED, int, uint32_t>::type;  // positions of paged rows may be negative
@@ -574,7 +577,31 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     Item cur;
     if constexpr (PAGED) {
         using Line = typename std::conditional<KV8, Paged8Line, PagedLine>::type;
-        if (!paged_first<256 * NG * (PAIR ? 2 : 1), BN, Line>(args, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C, cur)) return;
+        if constexpr (MIXED) {
+            static_assert(NG == 1 && !PAIR && !QS && sizeof(Kl0) >= kDecode8Lds<D> * sizeof(float), "an LDS buffer for each of four waves");
+            const A& a = fresh_args(args);
+            uint64_t* const scratch = reinterpret_cast<uint64_t*>(&Kl0[0][0]);
+            const Mixed8Share share = mixed8_share<256>(a, scratch);
+            const uint32_t wg = blockIdx.x;
+            if (threadIdx.x == 0) {  // chunks without a workgroup
+                if (wg >= share.tiles && wg < a.n_wg) reinterpret_cast<PagedDesc*>(a.desc)[wg].n = 0;
+                if (wg >= share.few && wg < a.part.n_wg) reinterpret_cast<PagedDesc*>(a.part.desc)[wg].n = 0;
+            }
+            if (wg < share.few) {
+                decode8_pieces<D, false, 0>(args.part, wg, share.few, [&](int w) {
+                    return reinterpret_cast<float*>(w == 0 ? &Kl0[0][0] : w == 1 ? &Kl1[0][0] : w == 2 ? &Vl0[0][0] : &Vl1[0][0]);
+                });
+                return;
+            }
+            if (wg - share.few >= share.tiles) return;
+            const bool any = paged_start<256, Line>(fresh_args(args), scratch, C, wg - share.few, share.tiles);
+            if (!any || !paged_next<BN>(fresh_args(args), C, cur)) {
+                if (threadIdx.x == 0) reinterpret_cast<PagedDesc*>(fresh_args(args).desc)[C.j].n = 0;
+                return;
+            }
+        } else if (!paged_first<256 * NG * (PAIR ? 2 : 1), BN, Line>(args, reinterpret_cast<uint64_t*>(&Kl0[0][0]), C, cur)) {
+            return;
+        }
     } else {
         if (!item_of(0, cur)) return;  // uniform over the workgroup
     }
