@@ -69,7 +69,7 @@ def test_store_overlaps(hiplib, kw):
     ({"vs8": None}, "null"), ({"table": None}, "null"), ({"lens": None}, "null"), ({"cu": None}, "null"), ({"odt": 3}, "dtype"),
     ({"qdt": 4}, "dtype"), ({"block": 16}, "block"), ({"block": 192}, "block"), ({"d": 80}, "head_dim"), ({"nkv": 0}, "n_kv_heads"),
     ({"nh": 34, "os": 4352, "qs": 4352}, "16 query heads"), ({"w": 0}, "max_blocks"), ({"stride": 3}, "max_blocks"),
-    ({"max_len": 0}, "max_len"), ({"max_len": 257}, "max_len"), ({"n": 65536}, "n_seq"), ({"nb": 1 << 31}, "too many blocks"),
+    ({"max_len": 0}, "max_len"), ({"max_len": 257}, "max_len"), ({"n": 65536}, "n_seq"), ({"n": 65535, "nkv": 129, "nh": 129, "qs": 16512, "os": 16512}, "too many sequences"), ({"nb": 1 << 31}, "too many blocks"),
     ({"w": 1 << 22, "stride": 1 << 22, "max_len": 1 << 27, "T": 1 << 20, "max_new": 1 << 20, "q": _at(1 << 40)}, "in chunks"),
     ({"max_new": 6}, "max_new"), ({"qs": 1000}, "stride"), ({"os": 1028}, "stride"), ({"gate": _at(0x8800000), "gs": 1000}, "gate_stride"),
     ({"q": _at(0x2000008)}, "aligned"), ({"out": _at(0x1000004)}, "aligned"), ({"kp": _at(0x6000008)}, "aligned"),
@@ -147,7 +147,7 @@ def to_args(**kw):
     *[({k: None}, "null") for k in ("k8", "v8", "ks", "vs", "kc", "vc", "dst", "src")],
     *[({k: _at(0x9000008)}, "aligned") for k in ("k8", "v8", "ks", "vs", "kc", "vc")],
     ({"n8": 1 << 31}, "too many"), ({"n16": 1 << 31}, "too many"), ({"n": 1 << 31}, "too many"), ({"n": 1 << 30}, "too many"),
-    ({"n": 1 << 20, "block": 65536}, "too many"),
+    ({"n": 1 << 20, "block": 65536}, "too many"), ({"n": 1 << 23}, "too many"), ({"n": 1 << 22, "block": 128}, "too many"),
 ])
 def test_pages_refusals(hiplib, kw, msg):
     assert hiplib.yhip_kv8_from_pages(*from_args(**kw)) == -22 and msg in _err(hiplib)

@@ -1040,7 +1040,7 @@ int pages_common(const char* fn, yhip::Kv8PagesArgs& a, bool from, const uint8_t
     if (((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)ks | (uintptr_t)vs | (uintptr_t)kc | (uintptr_t)vc) % 16)
         return fail(YHIP_EINVAL, "%s: pools must be 16-byte aligned", fn);
     if ((uint64_t)n_blocks * n_kv > 0xffffffffull || (uint64_t)n_blocks8 * n_kv > 0xffffffffull ||
-        n_pages > 0x7fffffffu || (uint64_t)n_pages * n_kv > 0x7fffffffull / (block / 64))
+        n_pages > 0xffffffu || (uint64_t)n_pages * n_kv > 0xffffffull / (block / 64))  // (2^32 threads a launch)
         return fail(YHIP_EINVAL, "%s: too many pages", fn);
     if (n_pages == 0) {
         done(hipSuccess, "");
@@ -1112,6 +1112,8 @@ int yhip_paged_attn8(void* att_out, uint32_t out_dtype, uint32_t out_stride, con
                      size_t workspace_bytes, void* stream)
 {
     const char* fn = "yhip_paged_attn8";
+    if ((uint64_t)n_seq * n_kv_heads > 0x7fffffull)  // (a workgroup for each item of short sequences: 2^32 threads a launch)
+        return fail(YHIP_EINVAL, "%s: too many sequences", fn);
     yhip::PagedAttn8Args a = {};
     const uint64_t rows = (uint64_t)n_blocks * n_kv_heads * block, pool = rows * head_dim;
     const Span pools[] = {{kpool, pool}, {vpool, pool}, {kscale, rows}, {vscale, rows}};

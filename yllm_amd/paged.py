@@ -259,7 +259,7 @@ def qk_norm_rope_kv8_store(cache: PagedKV8, q: torch.Tensor | None, k: torch.Ten
                            q_out_dtype: torch.dtype | None = None) -> torch.Tensor | None:
     """qk_norm_rope_kv_store into a pool held in 8 bits: each row of k (after its norm and rotation) and v gets a scale
     2^k, the smallest (k in -14..7) whose 448 reaches its largest magnitude, and e4m3 codes to nearest even.  Magnitudes
-    past 57344 are held as that, inf and NaN as NaN.  A row's bytes depend on that row alone."""
+    past 57344 are held as that, inf and NaN as NaN.  A row's bytes depend on that row alone; each slot at most once."""
     shape = _pool8(cache, "qk_norm_rope_kv8_store")
     kc, vc, sk, sv = cache.k, cache.v, cache.k_scale, cache.v_scale
     return _store("qk_norm_rope_kv8_store", fast("yhip_qk_norm_rope_kv8_store"), shape, (kc, vc, sk, sv),
