@@ -31,6 +31,7 @@ from .attention import _DT, ROPE_MROPE, ROPE_NONE, LayerKV, _dtype_code, _with_w
 
 _I32 = torch.int32
 _F16 = torch.float16
+_F32 = torch.float32
 
 
 @dataclass
@@ -139,12 +140,14 @@ def _pool8(cache: PagedKV8, fn: str) -> tuple[int, int, int, int]:
         raise YhipError(-22, f"{fn}: the cache must be a PagedKV8")
     k, v, ks, vs = cache.k, cache.v, cache.k_scale, cache.v_scale
     shape = k.shape
-    if len(shape) != 4 or k.dtype is not _E4M3 or v.dtype is not _E4M3 or ks.dtype is not _E5M2 or vs.dtype is not _E5M2 \
-            or not k.is_contiguous() or not v.is_contiguous() or not ks.is_contiguous() or not vs.is_contiguous() \
-            or v.numel() != k.numel() or v.shape[-2:] != (shape[3], 64) or ks.shape != shape[:3] or vs.shape != shape[:3]:
-        raise YhipError(-22, f"{fn}: the cache must hold contiguous e4m3 K and V of one size, V in tiles of 64 positions, "
-                             "and an e5m2 scale of each for every position and kv head")
-    return shape
+    if len(shape) == 4:
+        n, h, b, d = shape
+        if k.dtype is _E4M3 and v.dtype is _E4M3 and ks.dtype is _E5M2 and vs.dtype is _E5M2 and k.is_contiguous() \
+                and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and not b & 63 \
+                and v.shape == (n, h, b >> 6, d, 64) and ks.shape == vs.shape == (n, h, b):
+            return n, h, b, d
+    raise YhipError(-22, f"{fn}: the cache must hold contiguous e4m3 K and V of one size, V in tiles of 64 positions, "
+                         "and an e5m2 scale of each for every position and kv head")
 
 
 def _ints(fn: str, name: str, t: torch.Tensor, n: int) -> None:
@@ -297,11 +300,10 @@ def _store(fn, f, shape, pools, at, q, k, v, n_heads, rope, theta, n_rot, positi
         sp = slots.data_ptr()
     norm = F32
     if q_norm is not None or k_norm is not None:
-        if q_norm is None or k_norm is None or q_norm.shape != (d,) or k_norm.shape != (d,) \
-                or not q_norm.is_contiguous() or not k_norm.is_contiguous() or k_norm.dtype is not q_norm.dtype \
-                or q_norm.dtype not in (torch.float32, _F16):
+        if q_norm is None or k_norm is None or q_norm.shape != (d,) or k_norm.shape != (d,) or not q_norm.is_contiguous() \
+                or not k_norm.is_contiguous() or k_norm.dtype is not (wt := q_norm.dtype) or (wt is not _F32 and wt is not _F16):
             raise YhipError(-22, f"{fn}: q_norm and k_norm must both be [{d}], f32 or f16")
-        norm = _DT[q_norm.dtype]
+        norm = _DT[wt]
         wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
     args = (qop, qdt, qos, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DT[dt], wq, wk, norm, eps,
             *at, n_blocks, block, pp, sp, pos_start, T, n_heads, n_kv, d, rope,
