@@ -6,16 +6,21 @@
 // Each row is read once and written once.  A lane holds eight elements of a
 // head as two runs of four, so that a head is D / 8 lanes and its sum of squares
 // and largest magnitude are a few DPP moves.  A wave takes heads in rounds of
-// three passes, the next round's loads in flight behind one's arithmetic, and
+// three passes (two of fp32: 96 registers, five waves a SIMD), the next round's
+// loads in flight behind one's arithmetic, and
 // forms the row's sines and cosines once for all of them.  V is d-major in the
 // pool: workgroups of their own turn 64 rows of a kv head over in LDS, sixteen
 // aligned positions a store; a row outside such a group (a decode token, the ends
 // of a sequence's new tokens) has its V stored a byte at a time by the waves of
 // its other heads.
 //
-// Measured: 8193 tokens of three prompts, 16 / 2 heads of 256 (M-RoPE over 64),
-// bf16: 39.2 us, 4.1 TB/s, where a large copy reaches 5.1 (31 us); of 32 / 8 heads
-// of 128 42.7 us, 4.3 TB/s; one decode token 4.0 us, 64 of 32 / 8 of 128 4.3.
+// Measured: 8166 tokens of three prompts, 16 / 2 heads of 256 (M-RoPE over 64),
+// bf16: 36 us, 4.4 TB/s, where a large copy reaches 5.1 (31 us); of 32 / 8 heads of
+// 128 40 us, 4.6 TB/s; 2070 fp32 rows, four chunks and 28 decode tokens, of 28 / 4 of
+// 128 15.4 us, 3.6 TB/s; one decode token 3.5 us, 64 of 32 / 8 of 128 4.4.  What they
+// wait for is asked for in the order of its use: the slots and the angles' factors
+// before the row, a lone row's V before the arithmetic (39, 42.5, 17.5 and 4.0 us with
+// the row first).
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv8.hpp"
@@ -27,8 +32,8 @@ namespace yhip {
 namespace {
 
 // Up to this many rows every row's V goes with its other heads (32 / 8 heads of 128,
-// decode tokens: 300 rows 9.4 us, 12.3 the other way; a prompt: 6.0 and 6.6, of 400
-// 6.8 and 6.3).
+// decode tokens: 300 rows 8.8 us so, 400 the other way 10.8, 28 / 4: 5.9 and 9.0; of a
+// prompt 6.1 and 5.6, 28 / 4: 4.8 and 5.4).
 constexpr uint32_t kFewRows8 = 384;
 
 // four elements as loaded, and widened
@@ -89,6 +94,39 @@ __device__ inline int group_exponent(const f32x4& y0, const f32x4& y1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = max(top, max(finite_mag(y0[e]), finite_mag(y1[e])));
     return kv8_exponent(group_max<N>(top));
+}
+
+// Of values that a head's lanes of one place formed between them, heads % 4 (head_dim 256: % 2, two each), all four
+template <int D>
+__device__ inline void share4(const float (&own)[D == 256 ? 2 : 1], float (&all)[4])
+{
+    auto bits = [](float x) { return __builtin_bit_cast(uint32_t, x); };
+    auto val = [](uint32_t x) { return __builtin_bit_cast(float, x); };
+    if constexpr (D == 256) {  // the halves of the wave
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const auto r = __builtin_amdgcn_permlane32_swap(bits(own[n]), bits(own[n]), false, false);
+            all[2 * n] = val(r[0]);
+            all[2 * n + 1] = val(r[1]);
+        }
+    } else if constexpr (D == 128) {  // rows of 16
+        const auto r = __builtin_amdgcn_permlane32_swap(bits(own[0]), bits(own[0]), false, false);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const auto q = __builtin_amdgcn_permlane16_swap(r[n], r[n], false, false);
+            all[2 * n] = val(q[0]);
+            all[2 * n + 1] = val(q[1]);
+        }
+    } else {  // the halves of rows, and the rows of a half wave
+        const bool upper = threadIdx.x & 8u;
+        const auto r = __builtin_amdgcn_permlane16_swap(bits(own[0]), bits(own[0]), false, false);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float x = val(r[n]), y = dpp_mov<0x128>(x);  // row_ror 8
+            all[2 * n] = upper ? y : x;
+            all[2 * n + 1] = upper ? x : y;
+        }
+    }
 }
 
 // A slot's place: of its scale in head 0 (K codes: D times that), and of V codes
@@ -193,7 +231,7 @@ __device__ void v8_block(const QkNormRope8Args& a, uint32_t vb)
 
 // FEW: a row a wave group, every row's V among its passes.
 template <uint32_t KIND, int D, uint32_t DT, bool FEW>
-__global__ __launch_bounds__(256) void qk_norm_rope8_kernel(QkNormRope8Args a)
+__global__ __launch_bounds__(256, FEW ? 1 : 5) void qk_norm_rope8_kernel(QkNormRope8Args a)
 {
     // the two roles alternate over the first 2 * min(rotation, V) workgroups (rope.hip)
     uint32_t blk = blockIdx.x;
@@ -213,7 +251,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope8_kernel(QkNormRope8Args a)
         }
     }
     constexpr uint32_t LPH = D / 8, HPP = 64 / LPH;  // lanes per head, heads per pass
-    constexpr uint32_t U = FEW ? 1 : 3;              // passes of a round: their loads are issued together
+    constexpr uint32_t U = FEW ? 1 : DT == kF32 ? 2 : 3;  // passes of a round: their loads are issued together
     const uint32_t lane = threadIdx.x & 63u, i = lane % LPH, sub = lane / LPH;
     const uint32_t w = blk * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t b = w / a.groups, g = w - b * a.groups;
@@ -251,8 +289,18 @@ __global__ __launch_bounds__(256) void qk_norm_rope8_kernel(QkNormRope8Args a)
             r.x[u][1] = raw4<DT>(src, h * D + e1);
         }
     };
-    Round ra, rb;
-    load(ra, p_lo);
+    // The sines and cosines of the lane's four pairs: each of the wave's lanes of the same place in their heads forms one
+    // (two at head_dim 256), e = sub % (4 / N) + 4 / N * n, and they pass them round.  What they are formed from is asked
+    // for first: only this is waited for while the row is on its way.
+    constexpr uint32_t N = D == 256 ? 2 : 1;
+    double turns[N] = {};
+    if (KIND != kRopeNone && turn) {
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n) {
+            const uint32_t e = sub % (4 / N) + 4 / N * n;
+            turns[n] = a.turns[KIND == kRopePairs ? (e < 2 ? 2u * i + e : D / 4 + 2u * i + (e - 2)) : 4u * i + e];
+        }
+    }
     // !FEW: the slots of the rows about this one, row b - 15 + lane's (31 lanes), say whether it is one of sixteen that a
     // V workgroup stores
     int near = -1;
@@ -260,16 +308,35 @@ __global__ __launch_bounds__(256) void qk_norm_rope8_kernel(QkNormRope8Args a)
         const int at = (int)(b + lane) - 15;
         if (lane < 31u && at >= 0 && (uint32_t)at < a.n_tok) near = slot_of(a, (uint32_t)at);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    Round ra, rb;
+    load(ra, p_lo);
     __builtin_amdgcn_sched_barrier(0);  // nothing below waits before these are issued
     if (slot < 0) return;  // wave-uniform
     const Place8 place = place_of<D>(a, (uint32_t)slot);
-    float c[4], s[4];
+    // !FEW: a lone row, and its V heads of pass g, asked for before the arithmetic
+    bool lone = false;
+    auto load_v = [&](uint32_t v, typename Raw4<DT>::type (&x)[2]) __attribute__((always_inline)) {
+        const uint32_t h = min(v * HPP + sub, a.n_kv - 1u);
+        x[0] = raw4<DT>(row_at(a.v, a.v_stride), h * D + e0);
+        x[1] = raw4<DT>(row_at(a.v, a.v_stride), h * D + e1);
+    };
+    typename Raw4<DT>::type vx[2] = {};
+    if constexpr (!FEW) {
+        const int l0 = 15 - (slot & 15);  // the lanes of the group's rows are l0 .. l0 + 15
+        const uint64_t same = __ballot(near == (slot & ~15) + ((int)lane - l0));
+        lone = (same >> l0 & 0xffffu) != 0xffffu;
+        if (lone && g < pk) load_v(g, vx);
+    }
+    float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (KIND != kRopeNone) {
+        float oc[N], os[N];
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        c[e] = 1.0f;
-        s[e] = 0.0f;
-        const uint32_t pair = KIND == kRopePairs ? (e < 2 ? 2u * i + e : D / 4 + 2u * i + (e - 2)) : 4u * i + e;  // the lane's e-th
-        if (turn) sincos_turns(a.turns[pair] * (double)pos, &s[e], &c[e]);
+        for (uint32_t n = 0; n < N; ++n) {
+            sincos_turns(turns[n] * (double)pos, &os[n], &oc[n]);  // (no turn: 1 and 0)
+        }
+        share4<D>(oc, c);
+        share4<D>(os, s);
     }
     f32x4 qw[2], kw[2];
     const bool norm = a.q_norm != nullptr;
@@ -372,13 +439,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope8_kernel(QkNormRope8Args a)
             round(rb, p0);
             if ((p0 += U) >= p_hi) break;
         }
-        const int l0 = 15 - (slot & 15);  // the lanes of the group's rows are l0 .. l0 + 15
-        const uint64_t same = __ballot(near == (slot & ~15) + ((int)lane - l0));
-        if ((same >> l0 & 0xffffu) == 0xffffu) return;
+        if (!lone) return;
         for (uint32_t v = g; v < pk; v += a.groups) {
-            const uint32_t h = v * HPP + sub, hc = min(h, a.n_kv - 1u);
-            const char* const vrow = row_at(a.v, a.v_stride);
-            store_v(h, widen4<DT>(raw4<DT>(vrow, hc * D + e0)), widen4<DT>(raw4<DT>(vrow, hc * D + e1)));
+            if (v != g) load_v(v, vx);
+            store_v(v * HPP + sub, widen4<DT>(vx[0]), widen4<DT>(vx[1]));
         }
     }
 }
@@ -418,10 +482,11 @@ hipError_t launch_qk_norm_rope8(QkNormRope8Args a, hipStream_t st)
         a.v_blocks = 0;
     } else {
         // A row's passes to one wave, which forms its sines and cosines once, but at most kMostPasses, and to more of
-        // them where the rows alone are less than about kWaves (8193 rows of 16 / 2 heads of 256, nine passes: 39.4 us
-        // with one wave, 44.1 with three; of 32 / 8 of 128, ten: 46.9, 42.3 with two, 48.3 with four; 1000 rows of 16 / 2
-        // of 256: 13.6, 11.0 with three, 10.1 with five, 12.9 with nine).  More than a row a wave was slower for all.
-        constexpr uint32_t kMostPasses = 9, kWaves = 5000;
+        // them where the rows alone are less than about kWaves (8166 rows of 16 / 2 heads of 256, nine passes: 36 us
+        // with one wave, 39 with two, 40 with three; of 32 / 8 of 128, ten: 40 with two, 44 with three, 49 with one;
+        // 2048 fp32 rows of 28 / 4 of 128, eight: 13.8 with two, 15.2 with three, 14.1 with four; 1000 of 16 / 2 of
+        // 256: 9.5 with three, 8.7 with five).  More than a row a wave was slower for all.
+        constexpr uint32_t kMostPasses = 9, kWaves = 3500;
         const uint32_t want = std::min(passes, std::max((kWaves + a.n_tok - 1) / a.n_tok, (passes + kMostPasses - 1) / kMostPasses));
         a.passes = (passes + want - 1) / want;
         a.groups = (passes + a.passes - 1) / a.passes;
