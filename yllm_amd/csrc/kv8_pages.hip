@@ -7,6 +7,10 @@
 // a position's largest magnitude is the maximum over a thread's dimensions, over
 // the lanes eight apart and over the four waves (LDS).  Bound by HBM: every byte
 // is read and written once.
+//
+// Measured: 128 pages of 64, 8 kv heads of 128, into 8 bits: 12.2 us, 4.1 TB/s (the
+// bytes alone 9.8 at a large copy's rate: one round of 1024 workgroups, whose loads
+// all go out before the first conversion); three pages of 2 of 256 back: 3.2 us.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv8.hpp"

@@ -13,6 +13,11 @@
 // conversion that takes its row's scale (v_cvt_scalef32_pk_f16_fp8), V's by the
 // same with 1 and a packed product with the positions' factors.
 //
+// Measured: 64 sequences of 1k to 32k keys, 32 / 8 heads of 128, bf16: 190 us, 6.3
+// TB/s (f16 pages 357); fp32 queries 203; 16 / 2 of 256 108, 14 / 2 of 64 35; one
+// context of 131072 keys 47 us, 5.7 TB/s, and 4.5 for its merge.  At head_dim 256
+// only one V block is in flight and vmcnt's 63 loads bound K: 5.6 TB/s.
+//
 // The work is dealt out as in paged_decode.hip, in units of 256 keys, to the
 // workgroups of a launch of their own (paged_decode8.hip) or to some of those
 // that walk the same batch's tiles (attn_paged.hip).
