@@ -27,7 +27,6 @@ namespace yhip {
 namespace {
 
 constexpr uint32_t kMergeRows = 4;  // rows of a merge thread
-constexpr uint32_t kFewMergeWgs = 4;
 
 // Workgroup (j, y): the y-th 256 / (D / 4) rows of the split item that chunk j
 // begins, if any.  Pieces are joined in their order; a thread holds four
@@ -126,7 +125,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a)
     paged_merge<D>(a, blockIdx.x, blockIdx.y);
 }
 
-// Both lines' (PagedMixed8Args): `tile_wgs` workgroups for the tiles', then four for each of the other's chunks
+// Both lines' (PagedMixed8Args): `tile_wgs` workgroups for the tiles', then one for each row of the other's chunks (four
+// of four rows: 46.5 us for 45.0, a mixed step of 14 / 2 heads of 64)
 template <int D>
 __global__ __launch_bounds__(256) void paged_mixed8_merge_kernel(PagedMixed8Args a, uint32_t tile_wgs)
 {
@@ -134,12 +134,8 @@ __global__ __launch_bounds__(256) void paged_mixed8_merge_kernel(PagedMixed8Args
         paged_merge<D>(a, blockIdx.x % a.n_wg, blockIdx.x / a.n_wg);
         return;
     }
-    const uint32_t w = blockIdx.x - tile_wgs, j = w % a.part.n_wg;
-    if (reinterpret_cast<const PagedDesc*>(a.part.desc)[j].n == 0) return;
-    for (uint32_t r = w / a.part.n_wg; r < kRows; r += kFewMergeWgs) {
-        decode8_merge<D>(a.part, j, r);
-        __syncthreads();
-    }
+    const uint32_t w = blockIdx.x - tile_wgs;
+    decode8_merge<D>(a.part, w % a.part.n_wg, w / a.part.n_wg);
 }
 
 }  // namespace
@@ -296,7 +292,7 @@ hipError_t launch_paged_mixed8(const PagedAttn8Args& tiles, const PagedAttn8Args
     const uint32_t grid = std::min(a.n_wg + a.part.n_wg, round8(2u * (uint32_t)n_cus()));
     if (a.D == 64) hipLaunchKernelGGL((prefill_kernel<64, 1, false, false, PagedMixed8Args>), dim3(grid), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((prefill_kernel<128, 1, false, false, PagedMixed8Args>), dim3(grid), dim3(256), 0, st, a);
-    const uint32_t tile_wgs = may_split(a) ? a.n_wg * merge_wgs(a) : 0, merge = tile_wgs + kFewMergeWgs * a.part.n_wg;
+    const uint32_t tile_wgs = may_split(a) ? a.n_wg * merge_wgs(a) : 0, merge = tile_wgs + kRows * a.part.n_wg;
     if (a.D == 64) hipLaunchKernelGGL(paged_mixed8_merge_kernel<64>, dim3(merge), dim3(256), 0, st, a, tile_wgs);
     else hipLaunchKernelGGL(paged_mixed8_merge_kernel<128>, dim3(merge), dim3(256), 0, st, a, tile_wgs);
     return hipGetLastError();

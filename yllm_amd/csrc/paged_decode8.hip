@@ -157,8 +157,8 @@ size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, u
 // Sequences with few rows go to the decode kernel, the others to the tiles; which
 // are which is known on the device only.  One launch walks both lines where their
 // workgroups are alike, two to a CU (28 / 4 heads of 128, 28 decode tokens and
-// four chunks of 512: 87 us; one line after the other, each with its merge, 103;
-// 32 / 8, 63 of up to 32768 and a chunk of 256: 257 and 280; 14 / 2 heads of 64: 47
+// four chunks of 512: 86 us; one line after the other, each with its merge, 103;
+// 32 / 8, 63 of up to 32768 and a chunk of 256: 257 and 280; 14 / 2 heads of 64: 45
 // and 56); elsewhere the lines follow each other.  One sequence (a prompt's chunk)
 // is the tiles' whatever it brings.
 hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
