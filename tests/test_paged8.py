@@ -281,3 +281,48 @@ def test_calls_that_are_none(hiplib):
     assert hiplib.yhip_call(7, words, 16) == -22 and "no call" in _err(hiplib)
     assert hiplib.yhip_call(0, words, 15) == -22 and "words" in _err(hiplib)
     assert hiplib.yhip_call(0, None, 16) == -22 and "words" in _err(hiplib)
+
+
+@pytest.mark.parametrize("name", ["yhip_paged_plan", "yhip_qk_norm_rope_kv_store", "yhip_paged_attn", "yhip_qk_norm_rope_kv8_store",
+                                  "yhip_paged_attn8", "yhip_kv8_from_pages", "yhip_kv8_to_pages"])
+def test_only_a_pointer_may_be_none(hiplib, name):
+    """None for a number is refused wherever it stands, as the entry point's own binding refuses it; for a pointer it is null."""
+    import ctypes
+
+    from yllm_amd import YhipError
+    from yllm_amd._lib import SIGNATURES, fast
+
+    base = [getattr(a, "value", a) for a in _calls()[name]()]
+    direct, types = getattr(hiplib, name), SIGNATURES[name][1]
+    # (block or head_dim 0 is refused before anything would launch)
+    k = next(k for k in range(len(base)) if base[k] == 64 and direct(*base[:k], 0, *base[k + 1:]) == -22)
+    nothing = list(base)
+    nothing[k] = 0
+    for i, t in enumerate(types):
+        for a in (list(base), list(nothing)):
+            a[i] = None
+            if t is ctypes.c_void_p:
+                if a[k] == 0:
+                    assert fast(name)(*a) == direct(*a) == -22
+                continue
+            with pytest.raises(ctypes.ArgumentError):
+                direct(*a)
+            with pytest.raises(YhipError, match=f"argument {i} .*None") as e:
+                fast(name)(*a)
+            assert e.value.code == -22
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_attention_without_a_number(hiplib, monkeypatch, eight):
+    """A max_new of None is refused with a workspace as without one (max_len alone may be None)."""
+    torch = pytest.importorskip("torch")
+    from yllm_amd import YhipError
+    from yllm_amd import paged as PG
+
+    monkeypatch.setattr(PG, "elsewhere", lambda *a: None)           # (as if these tensors were on the current GPU)
+    monkeypatch.setattr(PG, "_stream", lambda: 0)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    cache = (PG.PagedKV8 if eight else PG.PagedKV).empty(4, 2, 128, device="cpu")
+    f = PG.paged_attn8 if eight else PG.paged_attn
+    with pytest.raises(YhipError, match="None"):
+        f(torch.zeros(5, 1024), cache, i(3, 4), i(3), i(4), 8, None, 256, workspace=torch.zeros(1 << 20, dtype=torch.uint8))

@@ -135,13 +135,17 @@ def fast(name: str):
 def _packed(name: str):
     code, types, call = CALLS.index(name), SIGNATURES[name][1], lib().yhip_call
     pack, n = struct.Struct("=" + "".join("d" if t is c_float else "Q" for t in types)).pack, len(types)
+    pointers = frozenset(i for i, t in enumerate(types) if t is c_void_p)
 
     def f(*args):
         try:
             return call(code, pack(*args), n)
         except struct.error:
             pass
-        try:  # (a null pointer may be None)
+        for i, a in enumerate(args):  # (a null pointer may be None, a number may not)
+            if a is None and i not in pointers:
+                raise YhipError(EINVAL, f"{name}: argument {i} is a number and must not be None")
+        try:
             words = pack(*[0 if a is None else a for a in args])
         except struct.error as e:
             raise YhipError(EINVAL, f"{name}: {e}") from None
