@@ -326,3 +326,29 @@ def test_attention_without_a_number(hiplib, monkeypatch, eight):
     f = PG.paged_attn8 if eight else PG.paged_attn
     with pytest.raises(YhipError, match="None"):
         f(torch.zeros(5, 1024), cache, i(3, 4), i(3), i(4), 8, None, 256, workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("start", [0, -1, -(1 << 31), 1 << 32])
+def test_a_start_that_slots_make_unused(hiplib, monkeypatch, eight, start):
+    """With slots a row's place and position are its own: pos_start may hold any number (-1 for "none", say).  The call gets as
+    far as its last check, that q_out overlaps k."""
+    torch = pytest.importorskip("torch")
+    from yllm_amd import YhipError
+    from yllm_amd import paged as PG
+
+    monkeypatch.setattr(PG, "elsewhere", lambda *a: None)           # (as if these tensors were on the current GPU)
+    monkeypatch.setattr(PG, "_stream", lambda: 0)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    cache = (PG.PagedKV8 if eight else PG.PagedKV).empty(4, 2, 128, device="cpu")
+    f = PG.qk_norm_rope_kv8_store if eight else PG.qk_norm_rope_kv_store
+    row = torch.zeros(5, 1024)
+    args = (torch.zeros(5, 1024), row[:, 512:768], torch.zeros(5, 256), 8, 2, 1e6)
+    with pytest.raises(YhipError, match="q_out overlaps"):
+        f(cache, *args, positions=i(5), slots=i(5), pos_start=start, q_out=row)
+    for wrong in (None, "0", 1.5):
+        with pytest.raises(YhipError):
+            f(cache, *args, positions=i(5), slots=i(5), pos_start=wrong, q_out=row)
+    if start < 0:
+        with pytest.raises(YhipError, match="range"):
+            f(cache, *args, pos_start=start, q_out=row)

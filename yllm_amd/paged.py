@@ -242,7 +242,7 @@ def qk_norm_rope_kv_store(cache: PagedKV | LayerKV, q: torch.Tensor | None, k: t
                           q_out_dtype: torch.dtype | None = None) -> torch.Tensor | None:
     """RMSNorm of every query and key head with the weights q_norm and k_norm [head_dim] (f32 / f16; both None: no
     norm), RoPE by `positions`, and k and v stored into the cache at `slots` (int32 [T], as paged_plan gives them).
-    Without slots the rows are the positions pos_start.. and slots of a contiguous cache (LayerKV).
+    Without slots the rows are the positions pos_start.. (unused otherwise) and slots of a contiguous cache (LayerKV).
 
     q [T, n_heads*head_dim], k and v [T, n_kv*head_dim] of one type (f32 / f16 / bf16); rows may be strided slices of
     one projection output.  rope: ROPE_PAIRS, ROPE_HALF, ROPE_MROPE (first n_rot dims) or ROPE_NONE.  Returns the
@@ -298,6 +298,8 @@ def _store(fn, f, shape, pools, at, q, k, v, n_heads, rope, theta, n_rot, positi
             raise YhipError(-22, f"{fn}: slots come with positions")
         _ints(fn, "slots", slots, T)
         sp = slots.data_ptr()
+        if isinstance(pos_start, int) and not 0 <= pos_start <= 0xffffffff:
+            pos_start = 0  # (not used with slots: whatever it is)
     norm = F32
     if q_norm is not None or k_norm is not None:
         if q_norm is None or k_norm is None or q_norm.shape != (d,) or k_norm.shape != (d,) or not q_norm.is_contiguous() \
