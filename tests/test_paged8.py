@@ -352,3 +352,22 @@ def test_a_start_that_slots_make_unused(hiplib, monkeypatch, eight, start):
     if start < 0:
         with pytest.raises(YhipError, match="range"):
             f(cache, *args, pos_start=start, q_out=row)
+
+
+def test_a_waves_share_of_the_lds_holds_all_that_is_put_into_it(tmp_path):
+    """The few-row kernel's shares (csrc/paged_decode8_lds.hpp, compiled for the host): each holds a wave's rows [16][D + 4] with
+    16 maxima, 16 sums and a flag, and the first one before that the queries as f16 [1 or 2 parts][16][D + 8], whatever lies
+    behind it; a multiple of 16 bytes."""
+    import subprocess
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parent.parent / "yllm_amd" / "csrc"
+    src, exe = tmp_path / "lds.cpp", tmp_path / "lds"
+    sizes = [(d, prec) for d in (64, 128, 256) for prec in ("false", "true")]
+    src.write_text('#include "paged_decode8_lds.hpp"\n#include <stdio.h>\nint main() {\n'
+                   + "".join(f'printf("%d\\n", yhip::kDecode8Lds<{d}, {p}>);\n' for d, p in sizes) + "}\n")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", f"-I{csrc}", str(src), "-o", str(exe)], check=True)
+    got = [4 * int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    for (d, prec), have in zip(sizes, got, strict=True):
+        rows, queries = 4 * (16 * (d + 4) + 16 + 16 + 1), 2 * (2 if prec == "true" else 1) * 16 * (d + 8)
+        assert have >= max(rows, queries) and have % 16 == 0, (d, prec, have, rows, queries)

@@ -13,7 +13,7 @@ namespace {
 template <int D, bool PREC, int POL>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_decode8_kernel(PagedAttn8Args args)
 {
-    __shared__ __attribute__((aligned(16))) float s_lds[4][kDecode8Lds<D>];
+    __shared__ __attribute__((aligned(16))) float s_lds[4][kDecode8Lds<D, PREC>];
     decode8_pieces<D, PREC, POL>(args, blockIdx.x, args.n_wg, [&](int w) { return &s_lds[w][0]; });
 }
 

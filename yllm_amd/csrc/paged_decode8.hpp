@@ -26,6 +26,7 @@
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv8.hpp"
+#include "paged_decode8_lds.hpp"
 #include "paged_items8.hpp"
 
 namespace yhip {
@@ -33,7 +34,7 @@ namespace {
 
 constexpr uint32_t kUnit8 = 256;      // keys of a unit: one 64-key block a wave
 constexpr uint32_t kItem8Units = 1;   // an item's fixed cost
-constexpr int kRows = 16;
+constexpr int kRows = kDecode8Rows;
 
 __device__ inline f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c)
 {
@@ -191,16 +192,15 @@ struct FragV8 {
     u32x4 v[D / 16], s;
 };
 
-// Floats of a wave's share of the LDS: its O rows, their maxima and sums, a flag
-template <int D>
-constexpr int kDecode8Lds = kRows * (D + 4) + 2 * kRows + 4;
-
-// The pieces of workgroup `wg` of `n_wg` (0: its whole item).  lds(w): wave w's share, 16-byte aligned; lds(0) takes the
-// line's scratch and then the queries as well, (hi, lo) [2][16][D + 8], or their hi part alone for 16-bit ones.
+// The pieces of workgroup `wg` of `n_wg` (0: its whole item).  lds(w): wave w's share, kDecode8Lds floats, 16-byte aligned
+// (the shares may lie anywhere); lds(0) takes the line's scratch and then the queries as well, (hi, lo) [2][16][D + 8], or
+// their hi part alone for 16-bit ones.
 template <int D, bool PREC, int POL, class A, class Lds>
 __device__ __forceinline__ void decode8_pieces(const A& args, uint32_t wg, uint32_t n_wg, Lds lds)
 {
     constexpr int kWaves = 4, D4 = D / 4, NC = D / 64, NB = D / 16, QROW = D + 8;
+    static_assert((PREC ? 2 : 1) * kRows * QROW * sizeof(_Float16) <= kDecode8Lds<D, PREC> * sizeof(float) &&
+                  24 * sizeof(uint64_t) <= kDecode8Lds<D, PREC> * sizeof(float), "the first share holds the queries and the scratch");
     // (head_dim 256: one block of V at a time, the next one's loads go out behind its products; two are too many registers)
     constexpr bool ONE = D > 128;
     auto s_o = [&](int w, uint32_t r, uint32_t d) { return lds(w) + r * (D + 4) + d; };

@@ -581,7 +581,9 @@ __global__ __launch_bounds__(256 * NG * (D > 128 ? 2 : 1), (NG == 1 && D <= 128 
     if constexpr (PAGED) {
         using Line = typename std::conditional<KV8, Paged8Line, PagedLine>::type;
         if constexpr (MIXED) {
-            static_assert(NG == 1 && !PAIR && !QS && sizeof(Kl0) >= kDecode8Lds<D> * sizeof(float), "an LDS buffer for each of four waves");
+            constexpr size_t share8 = kDecode8Lds<D, false> * sizeof(float);
+            static_assert(NG == 1 && !PAIR && !QS && sizeof(Kl0) >= share8 && sizeof(Kl1) >= share8 && sizeof(Vl0) >= share8 &&
+                          sizeof(Vl1) >= share8, "an LDS buffer for each of four waves");
             const A& a = fresh_args(args);
             uint64_t* const scratch = reinterpret_cast<uint64_t*>(&Kl0[0][0]);
             const Mixed8Share share = mixed8_share<256>(a, scratch);
