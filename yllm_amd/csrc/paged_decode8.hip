@@ -159,8 +159,9 @@ size_t paged_attn8_workspace(uint32_t n_tok, uint32_t n_seq, uint32_t max_new, u
 // workgroups are alike, two to a CU (28 / 4 heads of 128, 28 decode tokens and
 // four chunks of 512: 86 us; one line after the other, each with its merge, 103;
 // 32 / 8, 63 of up to 32768 and a chunk of 256: 257 and 280; 14 / 2 heads of 64: 45
-// and 56); elsewhere the lines follow each other.  One sequence (a prompt's chunk)
-// is the tiles' whatever it brings.
+// and 56); elsewhere the lines follow each other (28 decode tokens and four chunks
+// of 512, 28 / 4 heads of 128, fp32 queries 141; 16 / 2 of 256 with a gate 131, fp32
+// 178).  One sequence (a prompt's chunk) is the tiles' whatever it brings.
 hipError_t launch_paged_attn8(const PagedAttn8Args& in, hipStream_t st)
 {
     PagedAttn8Args a = in;
